@@ -10,7 +10,7 @@ Three operators share one storage format (the "packed" format, 4.5 bits per valu
 
 Packed format of a row of K values (K a multiple of 128): group g holds values 32 g .. 32 g + 31.
 Its scale is s = x* / -8 in fp16, where x* is the value of largest magnitude (the positive one
-if both signs reach it); a value's code is n = round-half-even(x / s) clamped to [-8, 7] and
+if both signs reach it); a value's code is n = floor(x / s + 1/2) clamped to [-8, 7] and
 stands for n * s.  A group holding a value that fp16 cannot hold finitely gets a NaN scale.
 Codes are stored as n + 8, eight to a 32-bit word and 16 words to a block of 128 values: word
 4 i + g of a block holds values 32 g + 8 i + e, e = 0..7, with value e at nibble e / 2 + 4 (e % 2).
@@ -117,8 +117,8 @@ def _pack(x):
     hi, lo = g.amax(-1), g.amin(-1)
     s = (torch.where(hi >= -lo, hi, lo) / -8).half()
     s = torch.where(g.abs().amax(-1) <= 65504, s, torch.full_like(s, math.nan))
-    # a 16-bit value over a 16-bit scale is at a border in fp32 only if it is exactly there
-    n = torch.round(g / s.float().unsqueeze(-1))
+    # the quotient of two 16-bit values is at a border between codes exactly, or 2^-13 away from it
+    n = torch.floor(g / s.float().unsqueeze(-1) + 0.5)
     n = torch.where(torch.isnan(n) | (s == 0).unsqueeze(-1), torch.zeros_like(n), n).clamp(-8, 7)
     n = (n + 8).to(torch.uint8).flatten(-2).unflatten(-1, (-1, 4, 4, 8))  # block, g, i, e
     n = n.transpose(-3, -2)  # words in the order i, g
@@ -238,7 +238,7 @@ def exact(case, seed):
         top = g.max(-1).values
         big = torch.where(top >= g.abs().max(-1).values, top, g.min(-1).values)
         s = (big * -0.125).half().double()
-        n = torch.where(s[..., None] == 0, 0.0, g / s[..., None]).round().clamp(-8, 7)
+        n = torch.where(s[..., None] == 0, 0.0, (g / s[..., None] + 0.5).floor()).clamp(-8, 7)
         values.append((n * s[..., None]).reshape(x.shape))
         scales.append(s)
     return {"values": torch.cat(values), "scales": torch.cat(scales)}
