@@ -12,7 +12,9 @@ Import from the repository root with the distribution folder on sys.path:
 from . import _lib
 from ._lib import AnimaError, last_error
 from .ops import apply_rope, attention, attention_core, device_info, prologue, sdpa, status, version
+from .packed import Packed4, attention_core_kv4, dequantize4, matvec4, quantize4
 from .rope import rope_freqs_3d
 
-__all__ = ["AnimaError", "apply_rope", "attention", "attention_core", "device_info", "last_error",
-           "prologue", "rope_freqs_3d", "sdpa", "status", "version", "_lib"]
+__all__ = ["AnimaError", "Packed4", "apply_rope", "attention", "attention_core",
+           "attention_core_kv4", "dequantize4", "device_info", "last_error", "matvec4",
+           "prologue", "quantize4", "rope_freqs_3d", "sdpa", "status", "version", "_lib"]

@@ -53,6 +53,24 @@ class QkvProjArgs(ct.Structure):
                 ("k_out", _P), ("v_out", _P)]
 
 
+_I64x2 = ct.c_int64 * 2
+
+
+class Matvec4Args(ct.Structure):
+    _fields_ = [("x", _P), ("x_dtype", ct.c_int), ("x_stride", _I64x2), ("codes", _P),
+                ("scales", _P), ("add", _P), ("add_stride", _I64x2), ("out", _P),
+                ("out_dtype", ct.c_int), ("out_stride", _I64x2), ("E", ct.c_int),
+                ("M", ct.c_int), ("N", ct.c_int), ("K", ct.c_int), ("silu", ct.c_int)]
+
+
+class AttnKv4Args(ct.Structure):
+    _fields_ = [("q", _P), ("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P),
+                ("dtype", ct.c_int), ("out", _P), ("out_stride", _I64x3), ("B", ct.c_int),
+                ("H", ct.c_int), ("S_q", ct.c_int), ("S_kv", ct.c_int), ("D", ct.c_int),
+                ("scale", ct.c_float), ("flags", ct.c_uint), ("kv_valid_len", _P),
+                ("workspace", _P), ("workspace_bytes", ct.c_uint64)]
+
+
 # Every symbol the headers declare, with its ctypes signature.
 SIGNATURES = {
     # include/anima_rt.h -- argtypes as the reference binds them (anima_rt_ops.py:11-34)
@@ -98,6 +116,11 @@ SIGNATURES = {
                                              ct.c_int, ct.c_int64, ct.c_int, ct.c_int, ct.c_float, _P],
                                             ct.c_int),
     "anima_dit_gelu": ([_P, _P, ct.c_int, ct.c_int64, _P], ct.c_int),
+    "anima_quantize4": ([_P, ct.c_int] + [ct.c_int64] * 6 + [ct.c_int, _P, _P, _P], ct.c_int),
+    "anima_dequantize4": ([_P, _P, _P, ct.c_int, ct.c_int64, ct.c_int, _P], ct.c_int),
+    "anima_matvec4": ([ct.POINTER(Matvec4Args), _P], ct.c_int),
+    "anima_attn_kv4_fwd": ([ct.POINTER(AttnKv4Args), _P], ct.c_int),
+    "anima_attn_kv4_workspace_size": ([ct.c_int] * 4, ct.c_uint64),
     "anima_attn_device_info": ([ct.POINTER(ct.c_int), ct.POINTER(ct.c_int)], ct.c_int),
     "anima_attn_version": ([], ct.c_char_p),
 }

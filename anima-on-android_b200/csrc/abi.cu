@@ -70,6 +70,14 @@ int softmax_launch(const float* x, float* y, long long outer, int dim, int sm_co
                    cudaStream_t st);
 int gemm_nt_launch(const float* A, const void* Bm, bool b_bf16, float* C, int M, int N, int K,
                    cudaStream_t st);
+int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long long n2,
+                     long long s0, long long s1, long long s2, int K, void* codes, void* scales,
+                     int sm_count, cudaStream_t st);
+int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype, long long rows,
+                       int K, int sm_count, cudaStream_t st);
+int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st);
+int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st);
+size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv);
 }  // namespace anima
 
 using namespace anima;
@@ -1081,6 +1089,95 @@ int anima_dit_gelu(const void* x, void* y, int dtype, int64_t n, void* stream) {
   DeviceState* d = current_device(&rc);
   if (!d) return rc;
   return gelu16_launch(x, y, dtype, n, d->sm_count, static_cast<cudaStream_t>(stream));
+}
+
+// ---- 4-bit storage
+static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+static bool any_dtype(int d) {
+  return d == ANIMA_DTYPE_F32 || d == ANIMA_DTYPE_F16 || d == ANIMA_DTYPE_BF16;
+}
+// Rows of K values within 2^46 values, so that no offset of a call passes 64 bits.
+static bool rows_fit(long long a, long long b, long long c, int K) {
+  const double n = (double)a * (double)b * (double)c * (double)K;
+  return n <= 70368744177664.0;
+}
+static int done4(int rc, const char* who) {
+  if (rc != ANIMA_OK) set_error(std::string(who) + ": " + code_name(rc));
+  return rc;
+}
+
+int anima_quantize4(const void* x, int dtype, int64_t n0, int64_t n1, int64_t n2, int64_t s0,
+                    int64_t s1, int64_t s2, int K, void* codes, void* scales, void* stream) {
+  if (dtype != ANIMA_DTYPE_F16 && dtype != ANIMA_DTYPE_BF16) return ANIMA_ERR_ARG;
+  if (n0 < 0 || n1 < 0 || n2 < 0 || K <= 0 || K % 128 || !rows_fit(n0, n1, n2, K)) return ANIMA_ERR_SHAPE;
+  if (n0 == 0 || n1 == 0 || n2 == 0) return ANIMA_OK;
+  if (!x || !codes || !scales || !al16(x) || !al16(codes) || !aligned(scales, 8)) return ANIMA_ERR_ARG;
+  if (s0 < 0 || s1 < 0 || s2 < 0 || (s0 | s1 | s2) % 8) return ANIMA_ERR_ARG;
+  int rc = ANIMA_OK;
+  DeviceState* d = current_device(&rc);
+  if (!d) return rc;
+  return done4(quantize4_launch(x, dtype, n0, n1, n2, s0, s1, s2, K, codes, scales, d->sm_count,
+                                static_cast<cudaStream_t>(stream)),
+               "anima_quantize4");
+}
+
+int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype, int64_t rows,
+                      int K, void* stream) {
+  if (!any_dtype(dtype)) return ANIMA_ERR_ARG;
+  if (rows < 0 || K <= 0 || K % 128 || !rows_fit(rows, 1, 1, K)) return ANIMA_ERR_SHAPE;
+  if (rows == 0) return ANIMA_OK;
+  if (!codes || !scales || !y || !al16(codes) || !aligned(scales, 8) || !al16(y)) return ANIMA_ERR_ARG;
+  int rc = ANIMA_OK;
+  DeviceState* d = current_device(&rc);
+  if (!d) return rc;
+  return done4(dequantize4_launch(codes, scales, y, dtype, rows, K, d->sm_count,
+                                  static_cast<cudaStream_t>(stream)),
+               "anima_dequantize4");
+}
+
+int anima_matvec4(const AnimaMatvec4Args* a, void* stream) {
+  if (!a || !any_dtype(a->x_dtype) || !any_dtype(a->out_dtype)) return ANIMA_ERR_ARG;
+  if (a->E < 0 || a->M < 0 || a->N < 0 || a->K <= 0 || a->K % 128 || a->K > ANIMA_MATVEC4_MAX_K ||
+      !rows_fit(a->E, a->N, 1, a->K))
+    return ANIMA_ERR_SHAPE;
+  if (a->E == 0 || a->M == 0 || a->N == 0) return ANIMA_OK;
+  if (!a->x || !a->codes || !a->scales || !a->out || !al16(a->codes) || !aligned(a->scales, 8))
+    return ANIMA_ERR_ARG;
+  if (!aligned(a->x, a->x_dtype == ANIMA_DTYPE_F32 ? 4 : 2) ||
+      !aligned(a->out, a->out_dtype == ANIMA_DTYPE_F32 ? 4 : 2) || (a->add && !aligned(a->add, 4)))
+    return ANIMA_ERR_ARG;
+  int rc = ANIMA_OK;
+  DeviceState* d = current_device(&rc);
+  if (!d) return rc;
+  return done4(matvec4_launch(a, d->sm_count, static_cast<cudaStream_t>(stream)), "anima_matvec4");
+}
+
+int anima_attn_kv4_fwd(const AnimaAttnKv4Args* a, void* stream) {
+  if (!a || !a->q || !a->k_codes || !a->k_scales || !a->v_codes || !a->v_scales || !a->out)
+    return ANIMA_ERR_ARG;
+  if (a->dtype != ANIMA_DTYPE_F16 && a->dtype != ANIMA_DTYPE_BF16) return ANIMA_ERR_ARG;
+  if (a->flags & ~ANIMA_FLAG_MASK) return ANIMA_ERR_ARG;
+  if (!(a->scale > 0.f && a->scale <= 3.402823466e38f)) return ANIMA_ERR_ARG;  // as the core needs it
+  if ((a->flags & ANIMA_FLAG_MASK) && !a->kv_valid_len) return ANIMA_ERR_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (a->out_stride[i] < 0 || a->out_stride[i] % 8) return ANIMA_ERR_ARG;
+  if (!al16(a->q) || !al16(a->k_codes) || !al16(a->v_codes) || !al16(a->out) ||
+      !aligned(a->k_scales, 8) || !aligned(a->v_scales, 8) || !aligned(a->workspace, 256))
+    return ANIMA_ERR_ARG;
+  if (a->D != 128 || a->B <= 0 || a->H <= 0 || a->S_q <= 0 || a->S_kv <= 0 ||
+      (long long)a->B * a->H > 0x7fffffffLL || !rows_fit((long long)a->B * a->H, a->S_kv, 1, 128) ||
+      !rows_fit((long long)a->B * a->H, a->S_q, 1, 128))
+    return ANIMA_ERR_SHAPE;
+  int rc = ANIMA_OK;
+  DeviceState* d = current_device(&rc);
+  if (!d) return rc;
+  return done4(attn_kv4_launch(a, d->status, d->sm_count, static_cast<cudaStream_t>(stream)),
+               "anima_attn_kv4_fwd");
+}
+
+uint64_t anima_attn_kv4_workspace_size(int B, int H, int S_q, int S_kv) {
+  if (B <= 0 || H <= 0 || S_q <= 0 || S_kv <= 0) return 0;
+  return attn_kv4_workspace_bytes(B, H, S_q, S_kv);
 }
 
 int anima_attn_selftest_timeout(unsigned timeout_us, void* stream) {

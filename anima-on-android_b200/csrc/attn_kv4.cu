@@ -1,0 +1,528 @@
+// attn_kv4.cu -- attention over K and V held packed in 4 bits (format: packed4.cuh):
+// out = softmax(q K^T * scale) V per (batch, head), D = 128, key-padding lengths per sample.
+//
+// Few query rows (up to kRowsFew per head): kv4_rows_kernel reads the packed cache directly.
+// Many: the cache is unpacked once to 16 bits (expand_kernel) and the attention core of
+// attn_fwd.cu runs on it; each key tile is then read by every 256-row unit of its head, and
+// unpacking it again in each would cost issue slots that the softmax needs.
+//
+// kv4_rows_kernel.  One cluster per (batch, head, block of query rows); its CTAs and their
+// warps take 32-key blocks in turn, each warp with its own running maximum, sum and output, so
+// there is no synchronisation inside the loop.  A warp streams its blocks through a private ring
+// of cp.async stages.  Per block:
+//   S^T = K Q^T   m16n8k16 with 16 keys as rows and 8 query rows as columns.  The products of
+//                 codes and 16-bit q are exact; a group's sum comes from a zeroed
+//                 accumulator and is multiplied by the key's scale of that group in fp32.
+//   P             exp2 of the scaled scores against a running maximum that only moves when a
+//                 score exceeds it by more than 8 (a factor 256), as in the core kernel.
+//   O^T += V^T P^T  16 dims as rows, 16 keys as k.  All rows of a tile lie in one group of V, so
+//                 the key's scale of that group goes into P in fp32, and the product P s is
+//                 split into two bf16 parts, hi + lo (16 bits of it): V's codes stay exact
+//                 and small scales do not underflow, as they would in fp16.  movmatrix turns the
+//                 accumulator's layout of P^T into the operand's.
+// At the end the warps' outputs meet in shared memory, then the cluster's CTAs read one
+// another's over distributed shared memory, each writing its share of the output.  No
+// workspace, no atomics; the order of all sums is fixed.
+#include <algorithm>
+
+#include "packed4.cuh"
+
+namespace anima {
+
+int attn_fwd_launch(const AnimaAttnArgs* a, int* status, int sm_count, cudaStream_t st,
+                    void* const* peers = nullptr, int n_peers = 0, int peer_rows = 0,
+                    long long peer_row_stride = 0, int peer_head0 = 0);
+
+namespace kv4 {
+
+constexpr int kD = 128;
+constexpr int kKeys = 32;                  // keys per block
+constexpr int kCodeBytes = kKeys * 64;     // codes of one block of K or V
+constexpr int kScaleBytes = kKeys * 8;
+constexpr int kStageBytes = 2 * kCodeBytes + 2 * kScaleBytes;
+constexpr float kRescale = 8.0f;           // log2 units
+
+struct Params {
+  const uint16_t* q;
+  const uint8_t* kc;
+  const uint8_t* ks;
+  const uint8_t* vc;
+  const uint8_t* vs;
+  const int* valid;
+  void* out;
+  long long ob, oh, os;
+  int H, BH, S_q, S_kv;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;  // the rest of the 16 bytes is zero-filled
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 8 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+// Transposes an 8 x 8 matrix of 16-bit values held two to a lane (row lane / 4).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Bytes of the merge area: per warp O [rows][128], m [rows], l [rows]; then the CTA's own.
+__host__ __device__ constexpr int part_floats(int rows) { return rows * kD + 2 * rows; }
+template <int kW, int kNB>
+constexpr size_t smem_bytes(int stages) {
+  const size_t ring = (size_t)kW * stages * kStageBytes;
+  const size_t merge = (size_t)(kW + 1) * part_floats(8 * kNB) * sizeof(float);
+  return ring > merge ? ring : merge;
+}
+
+// kBf16: type of q and out (else fp16); kW: warps; kNB: blocks of eight query rows; kNS: stages.
+template <bool kBf16, int kW, int kNB, int kNS>
+__global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kRows = 8 * kNB;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j = lane >> 2, i = lane & 3;
+  uint32_t ncta;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
+  const int rank = (int)cluster_rank();
+  const int unit = blockIdx.x / ncta;
+  const int bh = unit % p.BH, row0 = unit / p.BH * kRows;
+  const int b = bh / p.H;
+  const int len = p.valid ? min(max(__ldg(p.valid + b), 0), p.S_kv) : p.S_kv;
+  const int nblk = (len + kKeys - 1) / kKeys;
+  const int step = (int)ncta * kW;
+
+  // Query rows as B fragments: word order and pairs match packed4's (group g, lane i).
+  uint32_t qf[kNB][4][4];
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+    const int r = row0 + nb * 8 + j;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < p.S_q)
+        v = __ldg(reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + r) * kD + 32 * g + 8 * i));
+      qf[nb][g][0] = v.x;
+      qf[nb][g][1] = v.y;
+      qf[nb][g][2] = v.z;
+      qf[nb][g][3] = v.w;
+    }
+  }
+
+  const uint32_t ring = smem_u32(smem) + warp * kNS * kStageBytes;
+  const long long row_base = (long long)bh * p.S_kv;
+  // 16-byte code chunk c of key k sits at chunk c ^ ((k >> 1) & 3): the four even (or odd)
+  // keys that a V fragment reads at once then lie in different banks.
+  auto load = [&](int t, int slot) {
+    const uint32_t st = ring + slot * kStageBytes;
+    const int key0 = t * kKeys;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int id = c * 32 + lane, k = id >> 2, ch = id & 3;
+      const bool take = key0 + k < len;
+      const long long at = (row_base + (take ? key0 + k : 0)) * 64 + ch * 16;
+      const uint32_t dst = st + k * 64 + ((ch ^ ((k >> 1) & 3)) << 4);
+      cp16(dst, p.kc + at, take);
+      cp16(dst + kCodeBytes, p.vc + at, take);
+    }
+    const bool take = key0 + lane < len;
+    const long long at = (row_base + (take ? key0 + lane : 0)) * 8;
+    cp8(st + 2 * kCodeBytes + lane * 8, p.ks + at, take);
+    cp8(st + 2 * kCodeBytes + kScaleBytes + lane * 8, p.vs + at, take);
+  };
+
+  float o[kNB][8][4];  // O^T: tile 2 g + h of dims, rows j and j + 8; columns 2 i, 2 i + 1
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[nb][t][c] = 0.f;
+  float m[kNB][2], l[kNB][2];  // of query rows 2 i, 2 i + 1; l: this lane's keys only
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+
+  const int first = rank * kW + warp;
+  int ahead = first;
+#pragma unroll
+  for (int s = 0; s < kNS - 1; ++s) {
+    if (ahead < nblk) load(ahead, s);
+    cp_commit();
+    ahead += step;
+  }
+  int slot = 0;
+  for (int t = first; t < nblk; t += step) {
+    cp_wait<kNS - 2>();
+    __syncwarp();
+    {
+      const int put = slot == 0 ? kNS - 1 : slot - 1;  // the slot read in the last round
+      if (ahead < nblk) load(ahead, put);
+      cp_commit();
+      ahead += step;
+    }
+    const uint32_t st = ring + slot * kStageBytes;
+    slot = slot + 1 == kNS ? 0 : slot + 1;
+
+    float sc[2][kNB][4];  // scores of keys 16 u + j (0, 1) and 16 u + j + 8 (2, 3)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k0 = 16 * u + j;
+      const uint32_t swz = (uint32_t)(i ^ ((k0 >> 1) & 3)) << 4;  // the same for key k0 + 8
+      const uint4 c0 = lds16(st + k0 * 64 + swz), c1 = lds16(st + (k0 + 8) * 64 + swz);
+      const float4 f0 = p4::scales4(lds8(st + 2 * kCodeBytes + k0 * 8));
+      const float4 f1 = p4::scales4(lds8(st + 2 * kCodeBytes + (k0 + 8) * 8));
+      const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+      const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[u][nb][c] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t a[4], c[4];
+        p4::numbers<kBf16>(w0[g], a);
+        p4::numbers<kBf16>(w1[g], c);
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          p4::mma16816<kBf16>(d, a[0], c[0], a[1], c[1], qf[nb][g][0], qf[nb][g][1]);
+          p4::mma16816<kBf16>(d, a[2], c[2], a[3], c[3], qf[nb][g][2], qf[nb][g][3]);
+          sc[u][nb][0] = fmaf(g0[g], d[0], sc[u][nb][0]);
+          sc[u][nb][1] = fmaf(g0[g], d[1], sc[u][nb][1]);
+          sc[u][nb][2] = fmaf(g1[g], d[2], sc[u][nb][2]);
+          sc[u][nb][3] = fmaf(g1[g], d[3], sc[u][nb][3]);
+        }
+      }
+    }
+    // scores in log2 units; keys at or past len are masked
+    const int left = len - t * kKeys;
+    bool over = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float v = sc[u][nb][c] * p.scale_log2;
+          sc[u][nb][c] = 16 * u + j + 8 * (c >> 1) < left ? v : -INFINITY;
+          over = over || sc[u][nb][c] > m[nb][c & 1] + kRescale;
+        }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = fmaxf(fmaxf(sc[0][nb][r], sc[0][nb][r + 2]), fmaxf(sc[1][nb][r], sc[1][nb][r + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+          const float mn = fmaxf(m[nb][r], x);
+          const float alpha = m[nb][r] == -INFINITY ? 0.f : ex2_approx(m[nb][r] - mn);
+          m[nb][r] = mn;
+          l[nb][r] *= alpha;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) o[nb][q][r] *= alpha, o[nb][q][r + 2] *= alpha;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // the four V rows of this lane: keys 2 i, 2 i + 1 and those plus 8
+      uint4 vw[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int k = 16 * u + 2 * i + (c & 1) + 8 * (c >> 1);
+        vw[c] = lds16(st + kCodeBytes + k * 64 + (((j >> 1) ^ ((k >> 1) & 3)) << 4));
+      }
+      const int k0 = 16 * u + j;
+      const float4 f0 = p4::scales4(lds8(st + 2 * kCodeBytes + kScaleBytes + k0 * 8));
+      const float4 f1 = p4::scales4(lds8(st + 2 * kCodeBytes + kScaleBytes + (k0 + 8) * 8));
+      const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
+      const uint32_t w[4][4] = {{vw[0].x, vw[1].x, vw[2].x, vw[3].x}, {vw[0].y, vw[1].y, vw[2].y, vw[3].y},
+                                {vw[0].z, vw[1].z, vw[2].z, vw[3].z}, {vw[0].w, vw[1].w, vw[2].w, vw[3].w}};
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float mu = m[nb][c & 1];
+          const float e = ex2_approx(sc[u][nb][c] - (mu == -INFINITY ? 0.f : mu));
+          sc[u][nb][c] = e;
+          l[nb][c & 1] += e;
+        }
+      const uint32_t half = (j & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        // a lane's dims in group g: 32 g + 8 (j / 2) + j % 2 + {0, 2, 4, 6}, one half word
+        uint32_t x[4], y[4];
+        p4::numbers_bf16(__byte_perm(w[g][0], w[g][1], half), x);
+        p4::numbers_bf16(__byte_perm(w[g][2], w[g][3], half), y);
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          const float p0 = sc[u][nb][0] * g0[g], p1 = sc[u][nb][1] * g0[g];
+          const float p2 = sc[u][nb][2] * g1[g], p3 = sc[u][nb][3] * g1[g];
+          const uint32_t h0 = pack_bf16x2(p0, p1), h1 = pack_bf16x2(p2, p3);
+          const uint32_t l0 = pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xffff0000u));
+          const uint32_t l1 = pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xffff0000u));
+          const uint32_t b0 = transpose8(h0), b1 = transpose8(h1), e0 = transpose8(l0), e1 = transpose8(l1);
+          p4::mma16816<true>(o[nb][2 * g], x[0], x[1], y[0], y[1], b0, b1);
+          p4::mma16816<true>(o[nb][2 * g + 1], x[2], x[3], y[2], y[3], b0, b1);
+          p4::mma16816<true>(o[nb][2 * g], x[0], x[1], y[0], y[1], e0, e1);
+          p4::mma16816<true>(o[nb][2 * g + 1], x[2], x[3], y[2], y[3], e0, e1);
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();  // the rings become the merge area
+
+  // Per-warp results to shared memory: O [row][dim], m, l.
+  constexpr int kPart = part_floats(kRows);
+  float* const parts = reinterpret_cast<float*>(smem);
+  {
+    float* const mine = parts + warp * kPart;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x = l[nb][r];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        const int row = nb * 8 + 2 * i + r;
+        if (j == 0) {
+          mine[kRows * kD + row] = m[nb][r];
+          mine[kRows * kD + kRows + row] = x;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          // tile q = 2 g + h: row j is nibble 2 h of the half word, row j + 8 nibble 2 h + 1
+          const int d0 = 32 * (q >> 1) + 8 * (j >> 1) + (j & 1) + 4 * (q & 1);
+          mine[row * kD + d0] = o[nb][q][r];
+          mine[row * kD + d0 + 2] = o[nb][q][r + 2];
+        }
+      }
+  }
+  __syncthreads();
+  float* const own = parts + kW * kPart;
+  for (int e = threadIdx.x; e < kRows * kD; e += 32 * kW) {
+    const int row = e / kD;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) mx = fmaxf(mx, parts[w * kPart + kRows * kD + row]);
+    float acc = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const float mw = parts[w * kPart + kRows * kD + row];
+      const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - mx);
+      acc = fmaf(f, parts[w * kPart + e], acc);
+      sum = fmaf(f, parts[w * kPart + kRows * kD + kRows + row], sum);
+    }
+    own[e] = acc;
+    if (e % kD == 0) {
+      own[kRows * kD + row] = mx;
+      own[kRows * kD + kRows + row] = sum;
+    }
+  }
+  cluster_sync();
+  const uint32_t own_a = smem_u32(own);
+  const int per = (kRows * kD + (int)ncta - 1) / (int)ncta;
+  const int end = min(kRows * kD, (rank + 1) * per);
+  for (int e = rank * per + threadIdx.x; e < end; e += 32 * kW) {
+    const int row = e / kD;
+    float mx = -INFINITY;
+    for (uint32_t c = 0; c < ncta; ++c)
+      mx = fmaxf(mx, ld_cluster(mapa_shared(own_a + (kRows * kD + row) * 4, c)));
+    float acc = 0.f, sum = 0.f;
+    for (uint32_t c = 0; c < ncta; ++c) {
+      const uint32_t base = mapa_shared(own_a, c);
+      const float mc = ld_cluster(base + (kRows * kD + row) * 4);
+      const float f = mc == -INFINITY ? 0.f : ex2_approx(mc - mx);
+      acc = fmaf(f, ld_cluster(base + e * 4), acc);
+      sum = fmaf(f, ld_cluster(base + (kRows * kD + kRows + row) * 4), sum);
+    }
+    if (row0 + row < p.S_q) {
+      const float v = sum == 0.f ? 0.f : acc / sum;  // no valid key: zeros
+      const long long at = b * p.ob + (bh % p.H) * p.oh + (long long)(row0 + row) * p.os + e % kD;
+      static_cast<uint16_t*>(p.out)[at] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
+                                                : __half_as_ushort(__float2half_rn(v));
+    }
+  }
+  cluster_sync();  // no CTA leaves while another reads its shared memory
+}
+
+// ---------------------------------------------------------------- many rows: unpack once
+// Packed rows of K (blockIdx.y = 0) and V (1) to the attention core's 16-bit operands; rows at
+// or past a sample's length are written as zeros, whatever the cache holds there.
+template <bool kBf16>
+__global__ void __launch_bounds__(256)
+    expand_kernel(const uint4* kc, const uint2* ks, const uint4* vc, const uint2* vs, uint16_t* ko,
+                  uint16_t* vo, const int* valid, int H, int S_kv, long long quads) {
+  const uint4* codes = blockIdx.y ? vc : kc;
+  const uint2* scales = blockIdx.y ? vs : ks;
+  uint16_t* out = blockIdx.y ? vo : ko;
+  for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < quads;
+       u += (long long)gridDim.x * blockDim.x) {
+    const long long row = u >> 2;
+    uint16_t* const at = out + row * kD + 8 * (u & 3);
+    uint4 c = make_uint4(0u, 0u, 0u, 0u);
+    uint2 s2 = make_uint2(0u, 0u);
+    bool take = true;
+    if (valid) {
+      const long long bh = row / S_kv;
+      take = row - bh * S_kv < __ldg(valid + bh / H);
+    }
+    if (take) {
+      c = __ldg(codes + u);
+      s2 = __ldg(scales + row);
+    }
+    const float4 s = p4::scales4(s2);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    const float sg[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint32_t n[4], r[4];
+      p4::numbers_f16(w[g], n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&n[k]));
+        r[k] = kBf16 ? pack_bf16x2(v.x * sg[g], v.y * sg[g]) : pack_f16x2(v.x * sg[g], v.y * sg[g]);
+      }
+      *reinterpret_cast<uint4*>(at + 32 * g) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+  }
+}
+
+}  // namespace kv4
+
+// Query rows per head up to which the packed cache is read directly.
+constexpr int kRowsFew = 64;
+
+template <bool kBf16, int kW, int kNB, int kNS>
+static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
+  auto kern = kv4::kv4_rows_kernel<kBf16, kW, kNB, kNS>;
+  constexpr size_t smem = kv4::smem_bytes<kW, kNB>(kNS);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return ANIMA_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * ncta));
+  cfg.blockDim = dim3(32 * kW);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ncta;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
+    cudaGetLastError();
+    return ANIMA_ERR_CUDA;
+  }
+  return ANIMA_OK;
+}
+
+static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }
+
+// Bytes of workspace: none for few rows, else K and V in 16 bits.
+size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv) {
+  return S_q <= kRowsFew ? 0 : 2 * expanded_bytes((long long)B * H, S_kv);
+}
+
+int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st) {
+  const long long bh = (long long)a->B * a->H;
+  const bool bf = a->dtype == ANIMA_DTYPE_BF16;
+  const int* valid = (a->flags & ANIMA_FLAG_MASK) ? a->kv_valid_len : nullptr;
+  if (a->S_q <= kRowsFew) {
+    kv4::Params p;
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.kc = static_cast<const uint8_t*>(a->k_codes);
+    p.ks = static_cast<const uint8_t*>(a->k_scales);
+    p.vc = static_cast<const uint8_t*>(a->v_codes);
+    p.vs = static_cast<const uint8_t*>(a->v_scales);
+    p.valid = valid;
+    p.out = a->out;
+    p.ob = a->out_stride[0];
+    p.oh = a->out_stride[1];
+    p.os = a->out_stride[2];
+    p.H = a->H;
+    p.BH = (int)bh;
+    p.S_q = a->S_q;
+    p.S_kv = a->S_kv;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    const int nb = a->S_q > 8 ? 2 : 1;
+    const long long units = bh * ((a->S_q + 8 * nb - 1) / (8 * nb));
+    if (units * 8 > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
+    // CTAs per cluster: one 32-key block per warp before a second, up to the portable eight.
+    const int nblk = (a->S_kv + kv4::kKeys - 1) / kv4::kKeys;
+    const bool wide = nblk >= 8 * 8 * 2;
+    int ncta = 1;
+    while (ncta < 8 && ncta * (wide ? 8 : 4) < nblk && units * ncta < 2 * sm_count) ncta *= 2;
+    if (wide) {
+      if (nb == 1)
+        return bf ? rows_t<true, 8, 1, 3>(p, (int)units, ncta, st) : rows_t<false, 8, 1, 3>(p, (int)units, ncta, st);
+      return bf ? rows_t<true, 8, 2, 3>(p, (int)units, ncta, st) : rows_t<false, 8, 2, 3>(p, (int)units, ncta, st);
+    }
+    if (nb == 1)
+      return bf ? rows_t<true, 4, 1, 3>(p, (int)units, ncta, st) : rows_t<false, 4, 1, 3>(p, (int)units, ncta, st);
+    return bf ? rows_t<true, 4, 2, 3>(p, (int)units, ncta, st) : rows_t<false, 4, 2, 3>(p, (int)units, ncta, st);
+  }
+  const size_t side = expanded_bytes(bh, a->S_kv);
+  if (!a->workspace || a->workspace_bytes < 2 * side) return ANIMA_ERR_NOMEM;
+  uint16_t* const k16 = static_cast<uint16_t*>(a->workspace);
+  uint16_t* const v16 = k16 + side / 2;
+  const long long quads = bh * a->S_kv * 4;
+  const dim3 grid((unsigned)std::min<long long>((quads + 255) / 256, (long long)sm_count * 8), 2);
+  auto kern = bf ? kv4::expand_kernel<true> : kv4::expand_kernel<false>;
+  kern<<<grid, 256, 0, st>>>(static_cast<const uint4*>(a->k_codes), static_cast<const uint2*>(a->k_scales),
+                             static_cast<const uint4*>(a->v_codes), static_cast<const uint2*>(a->v_scales),
+                             k16, v16, valid, a->H, a->S_kv, quads);
+  if (cudaGetLastError() != cudaSuccess) return ANIMA_ERR_CUDA;
+  AnimaAttnArgs c = {};
+  c.q = a->q;
+  c.k = k16;
+  c.v = v16;
+  c.op_dtype = a->dtype;
+  c.out = a->out;
+  c.out_dtype = a->dtype;
+  for (int k = 0; k < 3; ++k) c.out_stride[k] = a->out_stride[k];
+  c.B = a->B;
+  c.H = a->H;
+  c.S_q = a->S_q;
+  c.S_kv = a->S_kv;
+  c.D = kv4::kD;
+  c.scale = a->scale;
+  c.flags = a->flags;
+  c.kv_valid_len = a->kv_valid_len;
+  // No workspace for the core's cut schedule: its merge adds the slices in the order in which
+  // they finish, and these results are to repeat bit for bit.
+  return attn_fwd_launch(&c, status, sm_count, st);
+}
+
+}  // namespace anima

@@ -1,0 +1,91 @@
+// packed4.cuh -- the packed 4-bit format and its unpacking in registers.
+//
+// A packed row holds K values (K a multiple of 128) as 4-bit codes and one fp16 scale per
+// 32 values: value = n * s with n in [-8, 7], 4.5 bits a value.  Codes are stored offset by
+// 8.  A block of 128 values is 64 bytes, sixteen 32-bit words; word 4 i + g holds values
+// 32 g + 8 i + e, e = 0..7 (group g, i = 0..3), value e at nibble (e >> 1) + 4 (e & 1).
+//
+// The order is chosen for the matrix instructions.  In an m16n8k16 operand fragment the four
+// lanes of a quad hold different k of one row; lane i reads words 4 i .. 4 i + 3 of a block,
+// one 16-byte load, and has eight consecutive values of every group.  Since both operands
+// may list k in any common order, word g then feeds two k-steps that lie wholly in group g,
+// and the group's scale can be applied to the fp32 accumulator: the products are of whole
+// numbers n, exact in fp16 and bf16.  Within a word, nibbles p and p + 4 are neighbours e =
+// 2 p, 2 p + 1, so masking with 0x000f000f leaves a pair in consecutive order.
+#pragma once
+#include "common.cuh"
+
+namespace anima {
+namespace p4 {
+
+constexpr int kGroup = 32;   // values that share a scale
+constexpr int kBlock = 128;  // values of one 64-byte code block
+
+// Eight codes of word w as whole numbers n, four pairs in value order.  In fp16, 0x6400 | c is
+// 1024 + c and 0x6400 | 16 c is 1024 + 16 c, so one subtraction, or one fused multiply-add
+// with 1/16 for the codes that sit four bits up, leaves n = c - 8 exactly.
+__device__ __forceinline__ void numbers_f16(uint32_t w, uint32_t (&n)[4]) {
+  const uint32_t w8 = w >> 8;
+  const __half2 lo = __half2half2(__ushort_as_half(0x6408));         // 1032
+  const __half2 sc = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
+  const __half2 hi = __half2half2(__ushort_as_half(0xd480));         // -72
+  uint32_t t[4];
+  t[0] = (w & 0x000f000fu) | 0x64006400u;
+  t[1] = (w & 0x00f000f0u) | 0x64006400u;
+  t[2] = (w8 & 0x000f000fu) | 0x64006400u;
+  t[3] = (w8 & 0x00f000f0u) | 0x64006400u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __half2 v = *reinterpret_cast<const __half2*>(&t[k]);
+    const __half2 r = (k & 1) ? __hfma2(v, sc, hi) : __hsub2(v, lo);
+    n[k] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// The same in bf16: 0x4300 | c is 128 + c (seven mantissa bits hold the four of c).
+__device__ __forceinline__ void numbers_bf16(uint32_t w, uint32_t (&n)[4]) {
+  const __nv_bfloat162 off = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));  // 136
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t t = ((w >> (4 * k)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), off);
+    n[k] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void numbers(uint32_t w, uint32_t (&n)[4]) {
+  if (kBf16)
+    numbers_bf16(w, n);
+  else
+    numbers_f16(w, n);
+}
+
+// The four fp16 scales of a 128-value block, as fp32.
+__device__ __forceinline__ float4 scales4(uint2 u) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// D += A B, m16n8k16 with fp32 accumulation.  Lane 4 j + i holds A rows j (a0, a2) and j + 8
+// (a1, a3), B column j, and D rows j (d0, d1) and j + 8 (d2, d3) of columns 2 i, 2 i + 1.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+}  // namespace p4
+}  // namespace anima

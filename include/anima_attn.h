@@ -299,6 +299,90 @@ int anima_dit_gate_residual_ln_modulate(float* x, const float* gate, int64_t gat
                                         float eps, void* stream);
 int anima_dit_gelu(const void* x, void* y, int dtype, int64_t n, void* stream);
 
+/*
+ * 4-bit storage (no counterpart in the reference, which keeps bf16 weights and projects the
+ * context's K/V in every step).  For what a sampling server keeps resident and reads with few
+ * rows or once a step: the K/V of text contexts and the adaLN modulation weights.
+ *
+ * Packed row of K values, K a multiple of 128: codes (K / 2 bytes, 16-byte aligned) and fp16
+ * scales (K / 32, 8-byte aligned), 4.5 bits a value.  Group g holds values 32 g .. 32 g + 31;
+ * its scale is s = x* / -8 rounded to fp16, x* its value of largest magnitude (the positive
+ * one if both signs reach it); the code n = floor(x / s + 1/2) clamped to [-8, 7] stands for
+ * n * s.  A group with a NaN or a magnitude above 65504 gets a NaN scale.  A block of 128
+ * values is 64 bytes, sixteen little-endian 32-bit words of eight codes n + 8: word 4 i + g
+ * holds values 32 g + 8 i + e, e = 0..7, value e at bits 4 ((e >> 1) + 4 (e & 1)).  Rows are
+ * contiguous; a tensor is two arrays [.., K/2] and [.., K/32].
+ *
+ * anima_quantize4: x of dtype F16 or BF16, rows [n0][n1][n2] at element strides s0, s1, s2
+ *   (multiples of 8, >= 0), each K contiguous values, 16-byte aligned -> codes
+ *   [n0*n1*n2, K/2], scales [n0*n1*n2, K/32].
+ * anima_dequantize4: back to y [rows, K] contiguous, dtype F32 (exact), F16 or BF16 (rounded
+ *   once), 16-byte aligned.
+ * Zero rows are allowed.  Asynchronous on `stream`.
+ */
+int anima_quantize4(const void* x, int dtype, int64_t n0, int64_t n1, int64_t n2, int64_t s0,
+                    int64_t s1, int64_t s2, int K, void* codes, void* scales, void* stream);
+int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype, int64_t rows,
+                      int K, void* stream);
+
+/*
+ * Matrix-vector products with packed weights: for e < E, m < M, n < N
+ *   out[e, m, n] = sum_k f(x[e, m, k]) W[e, n, k] + add[e, m, n],  f = SiLU if silu, else x.
+ * W: packed rows [E, N] of K values.  x, add (fp32, or NULL) and out are addressed by element
+ * strides {e, m} (0 repeats), their last axis contiguous; x and out F32, F16 or BF16.  The
+ * products are exact, sums are fp32; fp32 rows (and SiLU of any) enter as three bf16 parts
+ * (magnitudes up to 3.38e38), so the result has fp32 accuracy before its one rounding.
+ * Up to 8 fp32 or 16 16-bit rows share one pass over W; more rows take further passes.  K up
+ * to ANIMA_MATVEC4_MAX_K.  E, M or N = 0 does nothing.  Asynchronous on `stream`.
+ */
+#define ANIMA_MATVEC4_MAX_K 32768
+typedef struct AnimaMatvec4Args {
+  const void* x;
+  int x_dtype;
+  int64_t x_stride[2];
+  const void* codes;
+  const void* scales;
+  const float* add;
+  int64_t add_stride[2];
+  void* out;
+  int out_dtype;
+  int64_t out_stride[2];
+  int E, M, N, K;
+  int silu;
+} AnimaMatvec4Args;
+
+int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
+
+/*
+ * Attention over packed K and V: anima_attn_fwd with k/v [B*H, S_kv] packed rows of D = 128.
+ * q [B*H, S_q, 128] contiguous and out (strides {b, h, s} as in anima_attn_fwd, multiples of
+ * 8) are of dtype (F16 or BF16); scale is positive.  flags: ANIMA_FLAG_MASK with kv_valid_len (keys at or past it
+ * are not read or do not count, whatever is stored there; none left gives zero rows).
+ * Calls of few query rows read the packed rows directly and have fp32 accuracy up to the output's
+ * rounding; others unpack K and V into `workspace` (anima_attn_kv4_workspace_size bytes,
+ * 256-byte aligned, contents irrelevant; 0 for few rows) and run the attention core on them.
+ * Calls that share a workspace must be ordered.  Asynchronous on `stream`.
+ */
+typedef struct AnimaAttnKv4Args {
+  const void* q;
+  const void* k_codes;
+  const void* k_scales;
+  const void* v_codes;
+  const void* v_scales;
+  int dtype;
+  void* out;
+  int64_t out_stride[3];
+  int B, H, S_q, S_kv, D;
+  float scale;
+  unsigned flags;
+  const int* kv_valid_len;
+  void* workspace;
+  uint64_t workspace_bytes;
+} AnimaAttnKv4Args;
+
+int anima_attn_kv4_fwd(const AnimaAttnKv4Args* args, void* stream);
+uint64_t anima_attn_kv4_workspace_size(int B, int H, int S_q, int S_kv);
+
 /* Self-test of the bounded-wait path (no reference counterpart): launches one block
  * whose mbarrier wait can never complete and gives up after timeout_us microseconds
  * (1..1000000), recording ANIMA_ERR_TIMEOUT in the status word exactly as a stalled
