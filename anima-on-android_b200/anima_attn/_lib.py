@@ -118,8 +118,9 @@ SIGNATURES = {
     "anima_dit_gelu": ([_P, _P, ct.c_int, ct.c_int64, _P], ct.c_int),
     "anima_quantize4": ([_P, ct.c_int] + [ct.c_int64] * 6 + [ct.c_int, _P, _P, _P], ct.c_int),
     "anima_dequantize4": ([_P, _P, _P, ct.c_int, ct.c_int64, ct.c_int, _P], ct.c_int),
-    "anima_matvec4": ([ct.POINTER(Matvec4Args), _P], ct.c_int),
-    "anima_attn_kv4_fwd": ([ct.POINTER(AttnKv4Args), _P], ct.c_int),
+    # (the two structures by address: ctypes.byref of one, or its packed bytes)
+    "anima_matvec4": ([_P, _P], ct.c_int),
+    "anima_attn_kv4_fwd": ([_P, _P], ct.c_int),
     "anima_attn_kv4_workspace_size": ([ct.c_int] * 4, ct.c_uint64),
     "anima_attn_device_info": ([ct.POINTER(ct.c_int), ct.POINTER(ct.c_int)], ct.c_int),
     "anima_attn_version": ([], ct.c_char_p),

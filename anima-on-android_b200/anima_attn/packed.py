@@ -12,16 +12,24 @@ current torch stream, no fallback.
 """
 from __future__ import annotations
 
-import ctypes as ct
 import math
+import struct
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib as L
-from .ops import _TORCH_DT, _stream
+from .ops import _TORCH_DT
 
 _HALF = (torch.float16, torch.bfloat16)
+
+# The smallest of these calls run for a few microseconds on the GPU, so the host side is kept
+# short: the argument structures of the C entries are packed in one step (native alignment,
+# the layouts of _lib's Structures), and the stream is asked for as a raw handle.
+_MATVEC_ARGS = struct.Struct("@Pi2qPPP2qPi2qiiiii0q")
+_ATTN_ARGS = struct.Struct("@PPPPPiP3qiiiiifIPPQ")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class Packed4(NamedTuple):
@@ -40,22 +48,33 @@ class Packed4(NamedTuple):
         return self
 
 
-def _here(*ts) -> None:
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+def _here(*ts) -> int:
+    """The current stream of the current device, on which every tensor must be."""
+    if not ts[0].is_cuda:
+        raise ValueError("anima_attn ops take CUDA tensors on the current device")
+    dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and not (t.is_cuda and t.device.index == dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError("anima_attn ops take CUDA tensors on the current device")
+    return _raw_stream(dev)
 
 
-def _check_packed(p: Packed4, what: str) -> int:
-    """K of a packed tensor, after checking that its two arrays belong together."""
+def _check_packed(p: Packed4, what: str) -> tuple:
+    """Shape [..., K] of a packed tensor, after checking that its two arrays belong together."""
     c, s = p
-    K = 2 * c.shape[-1]
-    if c.dtype != torch.uint8 or s.dtype != torch.float16 or not (c.is_contiguous() and s.is_contiguous()):
+    if c.dtype is not torch.uint8 or s.dtype is not torch.float16 or not c.is_contiguous() or not s.is_contiguous():
         raise ValueError(f"{what}: packed codes are contiguous uint8, scales contiguous float16")
-    if K == 0 or K % 128 or c.shape[:-1] != s.shape[:-1] or s.shape[-1] * 32 != K:
+    *lead, half = c.shape
+    *slead, groups = s.shape
+    if half == 0 or half % 64 or groups * 16 != half or lead != slead:
         raise ValueError(f"{what}: codes [..., K/2] and scales [..., K/32], K a multiple of 128")
-    return K
+    lead.append(2 * half)
+    return lead
+
+
+@lru_cache(maxsize=1024)
+def _kv4_workspace(B: int, H: int, Sq: int, Skv: int) -> int:
+    return int(L.lib.anima_attn_kv4_workspace_size(B, H, Sq, Skv))
 
 
 def _row_strides(x: torch.Tensor) -> Optional[list]:
@@ -79,7 +98,7 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
     elements and amount to at most three axes (a [B, S, H, 128] projection or a slice of
     one).  ``out`` is filled if given.  A group of 32 with a NaN or a magnitude above 65504 reads
     back as NaN."""
-    _here(x)
+    stream = _here(x)
     if x.dtype not in _HALF:
         raise ValueError("x must be float16 or bfloat16")
     if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 128:
@@ -101,7 +120,7 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
                          "most three of them, and 16-byte alignment")
     (n0, s0), (n1, s1), (n2, s2) = axes
     L.check(L.lib.anima_quantize4(x.data_ptr(), _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K,
-                                  out.codes.data_ptr(), out.scales.data_ptr(), _stream()),
+                                  out.codes.data_ptr(), out.scales.data_ptr(), stream),
             "anima_quantize4")
     return out
 
@@ -109,13 +128,14 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
 def dequantize4(p: Packed4, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values [..., K] that a packed tensor stands for: exact in float32, rounded once in
     float16 and bfloat16."""
-    _here(*p)
-    K = _check_packed(p, "p")
+    stream = _here(*p)
+    shape = _check_packed(p, "p")
     if dtype not in _TORCH_DT:
         raise ValueError("dtype must be float32, float16 or bfloat16")
-    y = torch.empty(p.codes.shape[:-1] + (K,), device=p.codes.device, dtype=dtype)
+    y = torch.empty(shape, device=p.codes.device, dtype=dtype)
+    K = shape[-1]
     L.check(L.lib.anima_dequantize4(p.codes.data_ptr(), p.scales.data_ptr(), y.data_ptr(),
-                                    _TORCH_DT[dtype], y.numel() // K, K, _stream()),
+                                    _TORCH_DT[dtype], y.numel() // K, K, stream),
             "anima_dequantize4")
     return y
 
@@ -131,9 +151,9 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     ``out_dtype``'s type.  Sums are fp32 over exact products and fp32 x keeps its 24 bits, so
     the result is an fp32 one rounded once.  8 float32 rows or 16 16-bit ones share a
     pass over W."""
-    _here(x, add, out, *w)
-    K = _check_packed(w, "w")
-    ws = w.codes.shape
+    stream = _here(x, add, out, *w)
+    ws = _check_packed(w, "w")
+    K = ws[-1]
     if x.dtype not in _TORCH_DT:
         raise ValueError("x must be float32, float16 or bfloat16")
     if len(ws) == 2 and x.dim() in (1, 2):
@@ -157,7 +177,7 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
         raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous")
     ostr = out.stride()
     oe, om = ((0, 0) if len(shape) == 1 else (0, ostr[0])) if len(ws) == 2 else (ostr[0], ostr[1])
-    aptr, ae, am = None, 0, 0
+    aptr = ae = am = 0
     if add is not None:
         if add.dtype != torch.float32 or (N > 1 and (add.dim() == 0 or add.shape[-1] != N or add.stride(-1) != 1)):
             raise ValueError("add must be float32 with a contiguous last axis of N values")
@@ -166,10 +186,10 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
         except RuntimeError:
             raise ValueError("add must broadcast to the result") from None
         aptr, (ae, am, _) = av.data_ptr(), av.stride()
-    a = L.Matvec4Args(x.data_ptr(), _TORCH_DT[x.dtype], (xe, xm), w.codes.data_ptr(), w.scales.data_ptr(),
-                      aptr, (ae, am), out.data_ptr(), _TORCH_DT[out.dtype], (oe, om), E, M, N, K,
-                      1 if silu else 0)
-    L.check(L.lib.anima_matvec4(ct.byref(a), _stream()), "anima_matvec4")
+    a = _MATVEC_ARGS.pack(x.data_ptr(), _TORCH_DT[x.dtype], xe, xm, w.codes.data_ptr(),
+                          w.scales.data_ptr(), aptr, ae, am, out.data_ptr(), _TORCH_DT[out.dtype],
+                          oe, om, E, M, N, K, 1 if silu else 0)
+    L.check(L.lib.anima_matvec4(a, stream), "anima_matvec4")
     return out
 
 
@@ -186,16 +206,16 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     Few query rows read the packed cache directly, with fp32 accuracy up to the output's rounding;
     more rows unpack K and V once into 16-bit scratch of this call and run the attention
     core (anima_attn_kv4_fwd)."""
-    _here(q, kv_valid_len, out, *k, *v)
+    stream = _here(q, kv_valid_len, out, *k, *v)
     if q.dim() != 3 or q.dtype not in _HALF or not q.is_contiguous():
         raise ValueError("q must be [B*H, S_q, 128], contiguous, float16 or bfloat16")
     BH, Sq, D = q.shape
     if BH != B * H or D != 128 or BH == 0 or Sq == 0:
         raise ValueError("q must be [B*H, S_q, 128] with at least one row")
-    if _check_packed(k, "k") != D or _check_packed(v, "v") != D or k.codes.dim() != 3 or \
-            k.codes.shape[0] != BH or v.codes.shape != k.codes.shape or k.codes.shape[1] == 0:
+    ks = _check_packed(k, "k")
+    if ks != _check_packed(v, "v") or len(ks) != 3 or ks[0] != BH or ks[1] == 0 or ks[2] != D:
         raise ValueError("k and v must be packed [B*H, S_kv, 128] with at least one key")
-    Skv = k.codes.shape[1]
+    Skv = ks[1]
     if out_layout not in ("bshd", "bhsd"):
         raise ValueError("out_layout must be 'bshd' or 'bhsd'")
     shape = (B, Sq, H, D) if out_layout == "bshd" else (B, H, Sq, D)
@@ -214,13 +234,13 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")
         flags = L.FLAG_MASK
-    nbytes = L.lib.anima_attn_kv4_workspace_size(B, H, Sq, Skv)
+    nbytes = _kv4_workspace(B, H, Sq, Skv)
     # Scratch of this call alone, from the caching allocator: freed on return, its block goes
     # to work enqueued later on this stream, and a captured graph keeps it in its own pool.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    a = L.AttnKv4Args(q.data_ptr(), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
-                      v.scales.data_ptr(), _TORCH_DT[q.dtype], out.data_ptr(), strides, B, H, Sq, Skv, D,
-                      scale, flags,
-                      None if vl is None else vl.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-    L.check(L.lib.anima_attn_kv4_fwd(ct.byref(a), _stream()), "anima_attn_kv4_fwd")
+    a = _ATTN_ARGS.pack(q.data_ptr(), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
+                        v.scales.data_ptr(), _TORCH_DT[q.dtype], out.data_ptr(), *strides, B, H, Sq, Skv,
+                        D, scale, flags, 0 if vl is None else vl.data_ptr(),
+                        0 if ws is None else ws.data_ptr(), nbytes)
+    L.check(L.lib.anima_attn_kv4_fwd(a, stream), "anima_attn_kv4_fwd")
     return out

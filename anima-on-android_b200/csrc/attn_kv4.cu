@@ -55,32 +55,14 @@ struct Params {
   float scale_log2;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 16 : 0;  // the rest of the 16 bytes is zero-filled
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 8 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kN>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
-}
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
+using p4::cp16;
+using p4::cp16_if;
+using p4::cp8;
+using p4::cp8_if;
+using p4::cp_commit;
+using p4::cp_wait;
+using p4::lds16;
+using p4::lds8;
 // Transposes an 8 x 8 matrix of 16-bit values held two to a lane (row lane / 4).
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -95,18 +77,26 @@ __device__ __forceinline__ float ld_cluster(uint32_t a) {
 
 // Bytes of the merge area: per warp O [rows][128], m [rows], l [rows]; then the CTA's own.
 __host__ __device__ constexpr int part_floats(int rows) { return rows * kD + 2 * rows; }
+constexpr int rows_of(int nb) { return nb ? 8 * nb : 1; }
 template <int kW, int kNB>
 constexpr size_t smem_bytes(int stages) {
   const size_t ring = (size_t)kW * stages * kStageBytes;
-  const size_t merge = (size_t)(kW + 1) * part_floats(8 * kNB) * sizeof(float);
+  const size_t merge = (size_t)(kW + 1) * part_floats(rows_of(kNB)) * sizeof(float);
   return ring > merge ? ring : merge;
 }
 
 // kBf16: type of q and out (else fp16); kW: warps; kNB: blocks of eight query rows; kNS: stages.
-template <bool kBf16, int kW, int kNB, int kNS>
+// kNB = 0 is the form for a single row.  Its row fills all eight columns of Q, so that every
+// lane has the scores of its keys, and the columns of P are the row's four group-scaled forms, high
+// parts in columns 0 .. 3 and low parts in 4 .. 7: one operand, made once, serves all
+// eight dim tiles, and of a tile of group g columns g and 4 + g count.
+template <bool kBf16, int kW, int kNB_, int kNS>
 __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kRows = 8 * kNB;
+  constexpr bool kOne = kNB_ == 0;
+  constexpr int kNB = kOne ? 1 : kNB_;
+  constexpr int kRows = kOne ? 1 : 8 * kNB;
+  constexpr int kStep = kOne ? 2 : 1;  // of the four accumulators, those that differ
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = lane >> 2, i = lane & 3;
   uint32_t ncta;
@@ -123,7 +113,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   uint32_t qf[kNB][4][4];
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
-    const int r = row0 + nb * 8 + j;
+    const int r = kOne ? 0 : row0 + nb * 8 + j;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -140,22 +130,34 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   const long long row_base = (long long)bh * p.S_kv;
   // 16-byte code chunk c of key k sits at chunk c ^ ((k >> 1) & 3): the four even (or odd)
   // keys that a V fragment reads at once then lie in different banks.
+  // This lane's chunks of a block lie 8 keys apart: offsets of the first, and of its scales.
+  const uint32_t put0 = (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  const uint8_t* const kc = p.kc + row_base * 64 + lane * 16;
+  const uint8_t* const vc = p.vc + row_base * 64 + lane * 16;
+  const uint8_t* const ks = p.ks + row_base * 8 + lane * 8;
+  const uint8_t* const vs = p.vs + row_base * 8 + lane * 8;
   auto load = [&](int t, int slot) {
     const uint32_t st = ring + slot * kStageBytes;
-    const int key0 = t * kKeys;
+    const long long at = (long long)t * kCodeBytes, sat = (long long)t * kScaleBytes;
+    if ((t + 1) * kKeys <= len) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int id = c * 32 + lane, k = id >> 2, ch = id & 3;
-      const bool take = key0 + k < len;
-      const long long at = (row_base + (take ? key0 + k : 0)) * 64 + ch * 16;
-      const uint32_t dst = st + k * 64 + ((ch ^ ((k >> 1) & 3)) << 4);
-      cp16(dst, p.kc + at, take);
-      cp16(dst + kCodeBytes, p.vc + at, take);
+      for (int c = 0; c < 4; ++c) {
+        cp16(st + put0 + c * 512, kc + at + c * 512);
+        cp16(st + kCodeBytes + put0 + c * 512, vc + at + c * 512);
+      }
+      cp8(st + 2 * kCodeBytes + lane * 8, ks + sat);
+      cp8(st + 2 * kCodeBytes + kScaleBytes + lane * 8, vs + sat);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool take = t * kKeys + 8 * c + (lane >> 2) < len;
+        cp16_if(st + put0 + c * 512, take ? kc + at + c * 512 : p.kc, take);
+        cp16_if(st + kCodeBytes + put0 + c * 512, take ? vc + at + c * 512 : p.vc, take);
+      }
+      const bool take = t * kKeys + lane < len;
+      cp8_if(st + 2 * kCodeBytes + lane * 8, take ? ks + sat : p.ks, take);
+      cp8_if(st + 2 * kCodeBytes + kScaleBytes + lane * 8, take ? vs + sat : p.vs, take);
     }
-    const bool take = key0 + lane < len;
-    const long long at = (row_base + (take ? key0 + lane : 0)) * 8;
-    cp8(st + 2 * kCodeBytes + lane * 8, p.ks + at, take);
-    cp8(st + 2 * kCodeBytes + kScaleBytes + lane * 8, p.vs + at, take);
   };
 
   float o[kNB][8][4];  // O^T: tile 2 g + h of dims, rows j and j + 8; columns 2 i, 2 i + 1
@@ -211,13 +213,11 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
         p4::numbers<kBf16>(w1[g], c);
 #pragma unroll
         for (int nb = 0; nb < kNB; ++nb) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          p4::mma16816<kBf16>(d, a[0], c[0], a[1], c[1], qf[nb][g][0], qf[nb][g][1]);
+          float d[4];
+          p4::mma16816_zero<kBf16>(d, a[0], c[0], a[1], c[1], qf[nb][g][0], qf[nb][g][1]);
           p4::mma16816<kBf16>(d, a[2], c[2], a[3], c[3], qf[nb][g][2], qf[nb][g][3]);
-          sc[u][nb][0] = fmaf(g0[g], d[0], sc[u][nb][0]);
-          sc[u][nb][1] = fmaf(g0[g], d[1], sc[u][nb][1]);
-          sc[u][nb][2] = fmaf(g1[g], d[2], sc[u][nb][2]);
-          sc[u][nb][3] = fmaf(g1[g], d[3], sc[u][nb][3]);
+#pragma unroll
+          for (int c = 0; c < 4; c += kStep) sc[u][nb][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], sc[u][nb][c]);
         }
       }
     }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; c += kStep) {
           const float v = sc[u][nb][c] * p.scale_log2;
           sc[u][nb][c] = 16 * u + j + 8 * (c >> 1) < left ? v : -INFINITY;
           over = over || sc[u][nb][c] > m[nb][c & 1] + kRescale;
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < (kOne ? 1 : 2); ++r) {
           float x = fmaxf(fmaxf(sc[0][nb][r], sc[0][nb][r + 2]), fmaxf(sc[1][nb][r], sc[1][nb][r + 2]));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
@@ -247,7 +247,10 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
           m[nb][r] = mn;
           l[nb][r] *= alpha;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) o[nb][q][r] *= alpha, o[nb][q][r + 2] *= alpha;
+          for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (kOne || (c & 1) == r) o[nb][q][c] *= alpha;
         }
     }
 #pragma unroll
@@ -260,27 +263,50 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
         vw[c] = lds16(st + kCodeBytes + k * 64 + (((j >> 1) ^ ((k >> 1) & 3)) << 4));
       }
       const int k0 = 16 * u + j;
-      const float4 f0 = p4::scales4(lds8(st + 2 * kCodeBytes + kScaleBytes + k0 * 8));
-      const float4 f1 = p4::scales4(lds8(st + 2 * kCodeBytes + kScaleBytes + (k0 + 8) * 8));
-      const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
+      const uint2 s0 = lds8(st + 2 * kCodeBytes + kScaleBytes + k0 * 8);
+      const uint2 s1 = lds8(st + 2 * kCodeBytes + kScaleBytes + (k0 + 8) * 8);
       const uint32_t w[4][4] = {{vw[0].x, vw[1].x, vw[2].x, vw[3].x}, {vw[0].y, vw[1].y, vw[2].y, vw[3].y},
                                 {vw[0].z, vw[1].z, vw[2].z, vw[3].z}, {vw[0].w, vw[1].w, vw[2].w, vw[3].w}};
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; c += kStep) {
           const float mu = m[nb][c & 1];
           const float e = ex2_approx(sc[u][nb][c] - (mu == -INFINITY ? 0.f : mu));
           sc[u][nb][c] = e;
           l[nb][c & 1] += e;
         }
       const uint32_t half = (j & 1) ? 0x7632u : 0x5410u;
+      float g0[4], g1[4];
+      uint32_t one0 = 0, one1 = 0;  // the single row's operand
+      if constexpr (kOne) {
+        // columns 2 i, 2 i + 1: groups 2 (i % 2) and the next, high parts for i < 2
+        const uint32_t h0 = (i & 1) ? s0.y : s0.x, h1 = (i & 1) ? s1.y : s1.x;
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+        const float p0 = sc[u][0][0] * a.x, p1 = sc[u][0][0] * a.y;
+        const float p2 = sc[u][0][2] * c.x, p3 = sc[u][0][2] * c.y;
+        one0 = pack_bf16x2(p0, p1);
+        one1 = pack_bf16x2(p2, p3);
+        const uint32_t l0 = pack_bf16x2(p0 - __uint_as_float(one0 << 16), p1 - __uint_as_float(one0 & 0xffff0000u));
+        const uint32_t l1 = pack_bf16x2(p2 - __uint_as_float(one1 << 16), p3 - __uint_as_float(one1 & 0xffff0000u));
+        one0 = transpose8(i < 2 ? one0 : l0);
+        one1 = transpose8(i < 2 ? one1 : l1);
+      } else {
+        const float4 f0 = p4::scales4(s0), f1 = p4::scales4(s1);
+        g0[0] = f0.x, g0[1] = f0.y, g0[2] = f0.z, g0[3] = f0.w;
+        g1[0] = f1.x, g1[1] = f1.y, g1[2] = f1.z, g1[3] = f1.w;
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         // a lane's dims in group g: 32 g + 8 (j / 2) + j % 2 + {0, 2, 4, 6}, one half word
         uint32_t x[4], y[4];
         p4::numbers_bf16(__byte_perm(w[g][0], w[g][1], half), x);
         p4::numbers_bf16(__byte_perm(w[g][2], w[g][3], half), y);
+        if constexpr (kOne) {
+          p4::mma16816<true>(o[0][2 * g], x[0], x[1], y[0], y[1], one0, one1);
+          p4::mma16816<true>(o[0][2 * g + 1], x[2], x[3], y[2], y[3], one0, one1);
+        } else
 #pragma unroll
         for (int nb = 0; nb < kNB; ++nb) {
           const float p0 = sc[u][nb][0] * g0[g], p1 = sc[u][nb][1] * g0[g];
@@ -305,6 +331,27 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   float* const parts = reinterpret_cast<float*>(smem);
   {
     float* const mine = parts + warp * kPart;
+    if constexpr (kOne) {
+      float x = l[0][0];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      if (lane == 0) {
+        mine[kD] = m[0][0];
+        mine[kD + 1] = x;
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        // column g in lanes i = g / 2, column 4 + g two lanes on
+        const int g = q >> 1;
+        const float lo = o[0][q][g & 1] + __shfl_xor_sync(0xffffffffu, o[0][q][g & 1], 2);
+        const float hi = o[0][q][(g & 1) + 2] + __shfl_xor_sync(0xffffffffu, o[0][q][(g & 1) + 2], 2);
+        const int d0 = 32 * g + 8 * (j >> 1) + (j & 1) + 4 * (q & 1);
+        if (i == (g >> 1)) {
+          mine[d0] = lo;
+          mine[d0 + 2] = hi;
+        }
+      }
+    } else
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
@@ -425,10 +472,8 @@ template <bool kBf16, int kW, int kNB, int kNS>
 static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
   auto kern = kv4::kv4_rows_kernel<kBf16, kW, kNB, kNS>;
   constexpr size_t smem = kv4::smem_bytes<kW, kNB>(kNS);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return ANIMA_ERR_CUDA;
-  }
+  static SmemAttr attr;
+  if (!attr.raise((const void*)kern, smem, true)) return ANIMA_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ncta));
   cfg.blockDim = dim3(32 * kW);
@@ -443,6 +488,8 @@ static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
     cudaGetLastError();
+    // a device that cannot place a cluster past the portable size takes one within it
+    if (ncta > 8) return rows_t<kBf16, kW, kNB, kNS>(p, units, 8, st);
     return ANIMA_ERR_CUDA;
   }
   return ANIMA_OK;
@@ -476,22 +523,26 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     p.S_q = a->S_q;
     p.S_kv = a->S_kv;
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    const int nb = a->S_q > 8 ? 2 : 1;
-    const long long units = bh * ((a->S_q + 8 * nb - 1) / (8 * nb));
-    if (units * 8 > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
-    // CTAs per cluster: one 32-key block per warp before a second, up to the portable eight.
+    const int nb = a->S_q > 8 ? 2 : a->S_q > 1 ? 1 : 0, rows = kv4::rows_of(nb);
+    const long long units = bh * ((a->S_q + rows - 1) / rows);
+    if (units * 16 > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
+    // CTAs per cluster: as many as the SMs hold at once, two to an SM, while each of their warps
+    // has a 32-key block or more; eight warps where there are blocks for them.
     const int nblk = (a->S_kv + kv4::kKeys - 1) / kv4::kKeys;
-    const bool wide = nblk >= 8 * 8 * 2;
-    int ncta = 1;
-    while (ncta < 8 && ncta * (wide ? 8 : 4) < nblk && units * ncta < 2 * sm_count) ncta *= 2;
+    const bool wide = nblk >= 128;
+    const int warps = wide ? 8 : 4;
+    const int by_work = (nblk + warps - 1) / warps;
+    const int by_room = (int)std::max(1LL, 2LL * sm_count / units);
+    const int ncta = std::min(std::min(by_work, by_room), 8);
+    const int u = (int)units;
     if (wide) {
-      if (nb == 1)
-        return bf ? rows_t<true, 8, 1, 3>(p, (int)units, ncta, st) : rows_t<false, 8, 1, 3>(p, (int)units, ncta, st);
-      return bf ? rows_t<true, 8, 2, 3>(p, (int)units, ncta, st) : rows_t<false, 8, 2, 3>(p, (int)units, ncta, st);
+      if (nb == 0) return bf ? rows_t<true, 8, 0, 3>(p, u, ncta, st) : rows_t<false, 8, 0, 3>(p, u, ncta, st);
+      if (nb == 1) return bf ? rows_t<true, 8, 1, 3>(p, u, ncta, st) : rows_t<false, 8, 1, 3>(p, u, ncta, st);
+      return bf ? rows_t<true, 8, 2, 3>(p, u, ncta, st) : rows_t<false, 8, 2, 3>(p, u, ncta, st);
     }
-    if (nb == 1)
-      return bf ? rows_t<true, 4, 1, 3>(p, (int)units, ncta, st) : rows_t<false, 4, 1, 3>(p, (int)units, ncta, st);
-    return bf ? rows_t<true, 4, 2, 3>(p, (int)units, ncta, st) : rows_t<false, 4, 2, 3>(p, (int)units, ncta, st);
+    if (nb == 0) return bf ? rows_t<true, 4, 0, 3>(p, u, ncta, st) : rows_t<false, 4, 0, 3>(p, u, ncta, st);
+    if (nb == 1) return bf ? rows_t<true, 4, 1, 3>(p, u, ncta, st) : rows_t<false, 4, 1, 3>(p, u, ncta, st);
+    return bf ? rows_t<true, 4, 2, 3>(p, u, ncta, st) : rows_t<false, 4, 2, 3>(p, u, ncta, st);
   }
   const size_t side = expanded_bytes(bh, a->S_kv);
   if (!a->workspace || a->workspace_bytes < 2 * side) return ANIMA_ERR_NOMEM;

@@ -153,10 +153,12 @@ __global__ void __launch_bounds__(256)
 // with x1 and x2 the rounded remainders: 24 bits together, so nothing of x is lost, and the three
 // column sums are added at the end.
 //
-// A CTA of 8 warps takes tiles of 16 rows of W; `split` warps share a tile, taking its 128-value
-// blocks in turn, and their sums meet in shared memory in a fixed order.  The columns are
-// staged in shared memory once per matrix, rows 64 bytes past a multiple of 256 so that the
-// quads of two columns fill the 128 bytes of a wavefront.
+// A CTA of 8 warps works on one matrix, on a run of tiles of 16 rows of W; `split` warps share a
+// tile, taking its 128-value blocks in turn, and their sums meet in shared memory in a fixed
+// order.  A warp streams its blocks (1 KB of codes, 128 bytes of scales) through a private ring
+// of cp.async stages that runs on across tiles; each lane fetches the codes that it will read
+// itself.  The columns are staged in shared memory once, rows 64 bytes past a multiple of 256 so
+// that the quads of two columns fill the 128 bytes of a wavefront.
 struct Mv4Params {
   const void* x;
   const uint8_t* codes;
@@ -164,13 +166,15 @@ struct Mv4Params {
   const float* add;
   void* out;
   long long xe, xm, ae, am, oe, om;
-  long long items;       // E * tile groups
-  int N, K, M, groups;   // groups: tile groups of one matrix
-  int split, tiles;      // warps per tile, tiles per group (8 / split)
+  int N, K, M;
+  int parts;             // CTAs per matrix
+  int groups;            // tile groups of one matrix (8 / split tiles each)
+  int split;             // warps per tile
   int silu, x_dtype, out_dtype;
 };
 
 constexpr int kMvThreads = 256;
+constexpr int kMvStage = 16 * 64 + 16 * 8;  // bytes of a block of 16 rows
 
 __device__ __forceinline__ float load_x(const Mv4Params& p, long long at) {
   if (p.x_dtype == ANIMA_DTYPE_F32) return __ldg(static_cast<const float*>(p.x) + at);
@@ -179,62 +183,141 @@ __device__ __forceinline__ float load_x(const Mv4Params& p, long long at) {
                                        : __half2float(__ushort_as_half(u));
 }
 
-// kParts: columns per row of x (3: bf16 parts of an fp32 value, 1: the 16-bit value itself);
-// kNB: blocks of eight columns.
-template <bool kBf16, int kParts, int kNB>
-__global__ void __launch_bounds__(kMvThreads) matvec4_kernel(const Mv4Params p) {
+// kParts: columns per row of x (3: bf16 parts of an fp32 value, which take columns 4 m .. 4 m + 2,
+// so that a row's sum needs one exchange between neighbour lanes; 1: the 16-bit value itself);
+// kNB: blocks of eight columns; kStages: ring stages (4; 3 for rows so long that their columns
+// need the room).  Columns without a row repeat another one's data: columns do not mix.
+template <bool kBf16, int kParts, int kNB, int kStages>
+__global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kOuts = kParts == 3 ? 1 : 4;  // results of a lane per block of columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = lane >> 2, i = lane & 3;
-  const int cols = p.M * kParts;
   const int stride = p.K + 32;  // elements between staged columns
-  uint16_t* const xs = reinterpret_cast<uint16_t*>(smem);
-  float* const red = reinterpret_cast<float*>(smem + (size_t)cols * stride * 2);
-  const int s = warp % p.split, t = warp / p.split;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * kMvStage;
+  float* const red = reinterpret_cast<float*>(smem + 8 * kStages * kMvStage);
+  uint16_t* const xs = reinterpret_cast<uint16_t*>(red + 8 * 32 * kNB * kOuts);
+  const int s = warp % p.split, t = warp / p.split, tiles = 8 / p.split;
   const int blocks = p.K / p4::kBlock;
-  const long long lo = p.items * blockIdx.x / gridDim.x, hi = p.items * (blockIdx.x + 1) / gridDim.x;
-  long long staged = -1;
-  for (long long it = lo; it < hi; ++it) {
-    const long long e = it / p.groups;
-    const int tile = (int)(it - e * p.groups) * p.tiles + t;
-    if (e != staged) {
-      __syncthreads();  // the previous matrix's columns are no longer read
-      for (int c = threadIdx.x; c < p.M * p.K; c += kMvThreads) {
-        const int m = c / p.K, k = c - m * p.K;
-        float v = load_x(p, e * p.xe + m * p.xm + k);
-        if (p.silu) v = v / (1.0f + expf(-v));
-        if (kParts == 1) {
-          xs[m * stride + k] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
-                                     : __half_as_ushort(__float2half_rn(v));
+  const int e = blockIdx.x / p.parts, part = blockIdx.x - e * p.parts;
+  const int g_lo = (int)((long long)p.groups * part / p.parts);
+  const int g_hi = (int)((long long)p.groups * (part + 1) / p.parts);
+
+  // The block sequence of this warp: (group, block) with block = s, s + split, ...  A lane
+  // fetches its 16 bytes of rows j and j + 8, lanes i = 0, 1 their scales.  Rows past the
+  // matrix repeat its last one; their results are not stored.
+  const uint8_t* const codes = p.codes + (long long)e * p.N * (p.K / 2) + i * 16;
+  const uint8_t* const scales = reinterpret_cast<const uint8_t*>(p.scales) + (long long)e * p.N * (p.K / 16);
+  const uint8_t *c0 = codes, *c1 = codes, *sp = scales;
+  int ld_g = g_lo, ld_blk = s;
+  uint32_t ld_at = ring;
+  const int tile_rows = 16 * tiles;  // from a warp's tile to its next
+  const long long c_next = (long long)tile_rows * (p.K / 2) - (long long)((blocks - s - 1) / p.split + 1) * p.split * 64;
+  const long long s_next = (long long)tile_rows * (p.K / 16) - (long long)((blocks - s - 1) / p.split + 1) * p.split * 8;
+  int ld_n = (g_lo * tiles + t) * 16;  // first row of the tile being fetched
+  auto tile_start = [&]() {
+    const int n = ld_n + j;
+    const int n0 = min(n, p.N - 1), n1 = min(n + 8, p.N - 1);
+    c0 = codes + (long long)n0 * (p.K / 2) + s * 64;
+    c1 = codes + (long long)n1 * (p.K / 2) + s * 64;
+    sp = scales + (long long)(i == 0 ? n0 : n1) * (p.K / 16) + s * 8;
+  };
+  auto fetch = [&]() {
+    if (ld_g < g_hi) {
+      p4::cp16(ld_at + lane * 16, c0);
+      p4::cp16(ld_at + 512 + lane * 16, c1);
+      if (i < 2) p4::cp8(ld_at + 1024 + (i * 8 + j) * 8, sp);
+      c0 += p.split * 64;
+      c1 += p.split * 64;
+      sp += p.split * 8;
+      ld_blk += p.split;
+      if (ld_blk >= blocks) {
+        ld_blk = s;
+        ++ld_g;
+        ld_n += tile_rows;
+        if (ld_n + 16 <= p.N) {
+          c0 += c_next;
+          c1 += c_next;
+          sp += s_next;
         } else {
-#pragma unroll
-          for (int q = 0; q < kParts; ++q) {
-            const __nv_bfloat16 b = __float2bfloat16_rn(v);
-            xs[(m * kParts + q) * stride + k] = __bfloat16_as_ushort(b);
-            const float f = __bfloat162float(b);
-            v = isinf(f) ? 0.f : v - f;
-          }
+          tile_start();
         }
       }
-      staged = e;
-      __syncthreads();
     }
+    p4::cp_commit();
+    ld_at = ld_at == ring + (kStages - 1) * kMvStage ? ring : ld_at + kMvStage;
+  };
+  tile_start();
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch();
+
+  for (int m = 0; m < p.M; ++m) {
+    const long long from = (long long)e * p.xe + (long long)m * p.xm;
+    uint16_t* const to = xs + m * kParts * stride;
+#pragma unroll 4
+    for (int k = 2 * threadIdx.x; k < p.K; k += 2 * kMvThreads) {
+      float v0 = load_x(p, from + k), v1 = load_x(p, from + k + 1);
+      if (p.silu) {
+        v0 = __fdividef(v0, 1.0f + expf(-v0));
+        v1 = __fdividef(v1, 1.0f + expf(-v1));
+      }
+      if (kParts == 1) {
+        *reinterpret_cast<uint32_t*>(to + k) = kBf16 ? pack_bf16x2(v0, v1) : pack_f16x2(v0, v1);
+      } else {
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+          const uint32_t b = pack_bf16x2(v0, v1);
+          *reinterpret_cast<uint32_t*>(to + q * stride + k) = b;
+          const float f0 = __uint_as_float(b << 16), f1 = __uint_as_float(b & 0xffff0000u);
+          v0 = isinf(f0) ? 0.f : v0 - f0;
+          v1 = isinf(f1) ? 0.f : v1 - f1;
+        }
+      }
+    }
+  }
+  uint32_t xa[kNB];  // this lane's column of x, at its eight values of a group
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+    const int col = kParts == 3 ? min(nb * 2 + (j >> 2), p.M - 1) * 3 + min(j & 3, 2) : min(nb * 8 + j, p.M - 1);
+    xa[nb] = smem_u32(xs + col * stride + 8 * i);
+  }
+  __syncthreads();
+
+  // Result r of this lane for column block nb is row `row + out_row(r)`, row m = out_m(nb, r) of x.
+  auto out_row = [&](int r) { return kParts == 3 ? 0 : 8 * (r >> 1); };
+  auto out_m = [&](int nb, int r) { return kParts == 3 ? nb * 2 + (i >> 1) : nb * 8 + 2 * i + (r & 1); };
+  int row = (g_lo * tiles + t) * 16 + j + (kParts == 3 ? 8 * (i & 1) : 0);
+  long long out_at[kNB], add_at[kNB];
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+    out_at[nb] = (long long)e * p.oe + (long long)out_m(nb, 0) * p.om + row;
+    add_at[nb] = (long long)e * p.ae + (long long)out_m(nb, 0) * p.am + row;
+  }
+
+  uint32_t at = ring;
+  for (int grp = g_lo; grp < g_hi; ++grp) {
+    float y[kNB][kOuts];
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int r = 0; r < kOuts; ++r) {
+        y[nb][r] = 0.f;
+        if (p.add && s == 0 && row + out_row(r) < p.N && out_m(nb, r) < p.M)
+          y[nb][r] = __ldg(p.add + add_at[nb] + (r & 1) * p.am + out_row(r));
+      }
     float acc[kNB][4];
 #pragma unroll
     for (int b = 0; b < kNB; ++b)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[b][c] = 0.f;
-    const int n0 = tile * 16;
-    // rows past the matrix read its last row; their sums are not stored
-    const long long r0 = e * p.N + min(n0 + j, p.N - 1), r1 = e * p.N + min(n0 + j + 8, p.N - 1);
-    const uint4* c0 = reinterpret_cast<const uint4*>(p.codes + r0 * (p.K / 2)) + i;
-    const uint4* c1 = reinterpret_cast<const uint4*>(p.codes + r1 * (p.K / 2)) + i;
-    const uint2* s0 = reinterpret_cast<const uint2*>(p.scales + r0 * (p.K / p4::kGroup));
-    const uint2* s1 = reinterpret_cast<const uint2*>(p.scales + r1 * (p.K / p4::kGroup));
-#pragma unroll 2
     for (int blk = s; blk < blocks; blk += p.split) {
-      const uint4 u0 = __ldg(c0 + 4 * blk), u1 = __ldg(c1 + 4 * blk);
-      const float4 f0 = p4::scales4(__ldg(s0 + blk)), f1 = p4::scales4(__ldg(s1 + blk));
+      p4::cp_wait<kStages - 2>();
+      __syncwarp();
+      fetch();  // into the slot read in the last round
+      const uint4 u0 = p4::lds16(at + lane * 16), u1 = p4::lds16(at + 512 + lane * 16);
+      const float4 f0 = p4::scales4(p4::lds8(at + 1024 + j * 8));
+      const float4 f1 = p4::scales4(p4::lds8(at + 1024 + (8 + j) * 8));
+      at = at == ring + (kStages - 1) * kMvStage ? ring : at + kMvStage;
       const uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
       const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
@@ -244,12 +327,9 @@ __global__ void __launch_bounds__(kMvThreads) matvec4_kernel(const Mv4Params p) 
         p4::numbers<kBf16>(w1[g], b);
 #pragma unroll
         for (int nb = 0; nb < kNB; ++nb) {
-          uint4 xv = make_uint4(0u, 0u, 0u, 0u);
-          if (nb * 8 + j < cols)
-            xv = *reinterpret_cast<const uint4*>(xs + (nb * 8 + j) * stride + blk * p4::kBlock +
-                                                 32 * g + 8 * i);
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          p4::mma16816<kBf16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+          const uint4 xv = p4::lds16(xa[nb] + blk * (2 * p4::kBlock) + 64 * g);
+          float d[4];
+          p4::mma16816_zero<kBf16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
           p4::mma16816<kBf16>(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
           acc[nb][0] = fmaf(g0[g], d[0], acc[nb][0]);
           acc[nb][1] = fmaf(g0[g], d[1], acc[nb][1]);
@@ -258,36 +338,57 @@ __global__ void __launch_bounds__(kMvThreads) matvec4_kernel(const Mv4Params p) 
         }
       }
     }
-    // red[warp][row][column]
-    constexpr int kCols = 8 * kNB;
-    float* const mine = red + warp * 16 * kCols;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
-      *reinterpret_cast<float2*>(mine + j * kCols + nb * 8 + 2 * i) = make_float2(acc[nb][0], acc[nb][1]);
-      *reinterpret_cast<float2*>(mine + (j + 8) * kCols + nb * 8 + 2 * i) =
-          make_float2(acc[nb][2], acc[nb][3]);
-    }
-    __syncthreads();
-    for (int o = threadIdx.x; o < p.tiles * 16 * p.M; o += kMvThreads) {
-      const int row = o & 15, m = (o >> 4) % p.M, tt = (o >> 4) / p.M;
-      const int n = ((int)(it - e * p.groups) * p.tiles + tt) * 16 + row;
-      if (n >= p.N) continue;
-      float y = 0.f;
-      for (int q = 0; q < p.split; ++q)
+      if (kParts == 3) {
+        float v0 = acc[nb][0] + ((i & 1) ? 0.f : acc[nb][1]);
+        float v1 = acc[nb][2] + ((i & 1) ? 0.f : acc[nb][3]);
+        v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+        v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+        y[nb][0] += (i & 1) ? v1 : v0;
+      } else {
 #pragma unroll
-        for (int c = 0; c < kParts; ++c)
-          y += red[((tt * p.split + q) * 16 + row) * kCols + m * kParts + c];
-      if (p.add) y += __ldg(p.add + e * p.ae + m * p.am + n);
-      const long long at = e * p.oe + m * p.om + n;
-      if (p.out_dtype == ANIMA_DTYPE_F32)
-        static_cast<float*>(p.out)[at] = y;
-      else
-        static_cast<uint16_t*>(p.out)[at] = p.out_dtype == ANIMA_DTYPE_BF16
-                                                ? __bfloat16_as_ushort(__float2bfloat16_rn(y))
-                                                : __half_as_ushort(__float2half_rn(y));
+        for (int r = 0; r < kOuts; ++r) y[nb][r] += acc[nb][r];
+      }
     }
-    __syncthreads();  // the sums are read before the next tile's are written
+    if (p.split > 1) {  // the warps of a tile are neighbours: the first adds the others' results
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int r = 0; r < kOuts; ++r) red[((warp * kNB + nb) * kOuts + r) * 32 + lane] = y[nb][r];
+      __syncthreads();
+      if (s == 0)
+        for (int q = 1; q < p.split; ++q)
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+            for (int r = 0; r < kOuts; ++r) y[nb][r] += red[(((warp + q) * kNB + nb) * kOuts + r) * 32 + lane];
+    }
+    if (s == 0) {
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int r = 0; r < kOuts; ++r) {
+          if (row + out_row(r) >= p.N || out_m(nb, r) >= p.M) continue;
+          const float v = y[nb][r];
+          const long long o = out_at[nb] + (r & 1) * p.om + out_row(r);
+          if (p.out_dtype == ANIMA_DTYPE_F32)
+            static_cast<float*>(p.out)[o] = v;
+          else
+            static_cast<uint16_t*>(p.out)[o] = p.out_dtype == ANIMA_DTYPE_BF16
+                                                   ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
+                                                   : __half_as_ushort(__float2half_rn(v));
+        }
+    }
+    if (p.split > 1) __syncthreads();  // the sums are read before the next tile's are written
+    row += tile_rows;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+      out_at[nb] += tile_rows;
+      add_at[nb] += tile_rows;
+    }
   }
+  p4::cp_wait<0>();
 }
 
 // ---------------------------------------------------------------- launchers
@@ -334,34 +435,56 @@ int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 
-template <bool kBf16, int kParts, int kNB>
-static int mv4_t(const Mv4Params& p, int sm_count, cudaStream_t st) {
-  auto kern = matvec4_kernel<kBf16, kParts, kNB>;
-  const size_t smem = (size_t)p.M * kParts * (p.K + 32) * 2 + 8 * 16 * 8 * kNB * sizeof(float);
-  if (smem > 227 * 1024) return ANIMA_ERR_SHAPE;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return ANIMA_ERR_CUDA;
+constexpr size_t kMaxSmem = 227 * 1024;
+constexpr size_t mv4_fixed_smem(int nb, int outs, int stages) {
+  return 8 * stages * kMvStage + 8 * 32 * nb * outs * sizeof(float);
+}
+
+template <bool kBf16, int kParts, int kNB, int kStages>
+static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
+  auto kern = matvec4_kernel<kBf16, kParts, kNB, kStages>;
+  const size_t smem = mv4_fixed_smem(kNB, kParts == 3 ? 1 : 4, kStages) + (size_t)p.M * kParts * (p.K + 32) * 2;
+  if (smem > kMaxSmem) return ANIMA_ERR_SHAPE;
+  static SmemAttr attr;
+  if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
+  // Warps that share a tile, and CTAs per matrix: the split whose busiest warp has the least to do,
+  // in blocks, a tile's ends counted as one.
+  const int ntiles = (p.N + 15) / 16, blocks = p.K / p4::kBlock;
+  const int per_sm = std::max(1, std::min(3, (int)(kMaxSmem / (smem + 1024))));
+  const long long slots = (long long)per_sm * sm_count;
+  long long best = 0;
+  for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+    const long long groups = ((long long)ntiles * split + 7) / 8;
+    const long long parts = std::min(groups, std::max(1LL, slots / E));
+    const long long waves = (E * parts + slots - 1) / slots;
+    const long long cost = waves * ((groups + parts - 1) / parts) * ((blocks + split - 1) / split + 1);
+    if (split == 1 || cost < best) {
+      best = cost;
+      p.split = split;
+      p.groups = (int)groups;
+      p.parts = (int)parts;
+    }
   }
-  int per_sm = (int)(227 * 1024 / (smem + 1024));
-  if (per_sm > 4) per_sm = 4;
-  const int grid = (int)std::min<long long>(p.items, (long long)sm_count * per_sm);
-  kern<<<grid, kMvThreads, smem, st>>>(p);
+  if ((long long)E * p.parts > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
+  kern<<<E * p.parts, kMvThreads, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 
-// Rows of x of one launch: eight fp32 rows are 24 columns, sixteen 16-bit rows 16; fewer where
-// their columns would not fit shared memory.
-static int mv4_rows(int K, int parts) {
-  const int most = parts == 3 ? 8 : 16;
-  const int fit = (int)((227 * 1024 - 8 * 16 * 24 * 4) / ((size_t)parts * (K + 32) * 2));
-  return most < fit ? most : fit;
+// Rows of x of one launch: eight fp32 rows or sixteen 16-bit ones; fewer where their columns
+// would not fit shared memory, and a shorter ring where not even one would.
+static int mv4_rows(int K, int parts, int* stages) {
+  const size_t row = (size_t)parts * (K + 32) * 2;
+  *stages = 4;
+  const int fit = (int)((kMaxSmem - mv4_fixed_smem(2, 4, 4)) / row);
+  if (fit >= 1) return std::min(parts == 3 ? 8 : 16, fit);
+  *stages = 3;
+  return kMaxSmem - mv4_fixed_smem(1, 4, 3) >= row ? 1 : 0;
 }
 
 int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
   const int parts = a->x_dtype == ANIMA_DTYPE_F32 || a->silu ? 3 : 1;
-  const int rows = mv4_rows(a->K, parts);
+  int stages;
+  const int rows = mv4_rows(a->K, parts, &stages);
   if (rows < 1) return ANIMA_ERR_SHAPE;
   Mv4Params p;
   p.codes = static_cast<const uint8_t*>(a->codes);
@@ -377,28 +500,27 @@ int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
   p.silu = a->silu;
   p.x_dtype = a->x_dtype;
   p.out_dtype = a->out_dtype;
-  // Warps that share a tile: as many as leave each two blocks of its rows.
-  p.split = 1;
-  while (p.split < 8 && p.K / p4::kBlock >= 4 * p.split) p.split *= 2;
-  p.tiles = 8 / p.split;
-  const int ntiles = (p.N + 15) / 16;
-  p.groups = (ntiles + p.tiles - 1) / p.tiles;
-  p.items = (long long)a->E * p.groups;
   const int xs = a->x_dtype == ANIMA_DTYPE_F32 ? 4 : 2, os = a->out_dtype == ANIMA_DTYPE_F32 ? 4 : 2;
   for (int m0 = 0; m0 < a->M; m0 += rows) {
     p.M = std::min(rows, a->M - m0);
     p.x = static_cast<const char*>(a->x) + m0 * p.xm * xs;
     p.out = static_cast<char*>(a->out) + m0 * p.om * os;
     p.add = a->add ? static_cast<const float*>(a->add) + m0 * p.am : nullptr;
-    const int nb = (p.M * parts + 7) / 8;
+    const int nb = parts == 3 ? (p.M + 1) / 2 : (p.M + 7) / 8;
+    const bool bf = parts == 3 || a->x_dtype == ANIMA_DTYPE_BF16;
     int rc;
-    if (parts == 3)
-      rc = nb == 1 ? mv4_t<true, 3, 1>(p, sm_count, st)
-                   : nb == 2 ? mv4_t<true, 3, 2>(p, sm_count, st) : mv4_t<true, 3, 3>(p, sm_count, st);
-    else if (a->x_dtype == ANIMA_DTYPE_BF16)
-      rc = nb == 1 ? mv4_t<true, 1, 1>(p, sm_count, st) : mv4_t<true, 1, 2>(p, sm_count, st);
+    if (stages == 3)
+      rc = parts == 3 ? mv4_t<true, 3, 1, 3>(p, a->E, sm_count, st)
+           : bf       ? mv4_t<true, 1, 1, 3>(p, a->E, sm_count, st)
+                      : mv4_t<false, 1, 1, 3>(p, a->E, sm_count, st);
+    else if (parts == 3)
+      rc = nb == 1   ? mv4_t<true, 3, 1, 4>(p, a->E, sm_count, st)
+           : nb == 2 ? mv4_t<true, 3, 2, 4>(p, a->E, sm_count, st)
+                     : mv4_t<true, 3, 4, 4>(p, a->E, sm_count, st);
+    else if (bf)
+      rc = nb == 1 ? mv4_t<true, 1, 1, 4>(p, a->E, sm_count, st) : mv4_t<true, 1, 2, 4>(p, a->E, sm_count, st);
     else
-      rc = nb == 1 ? mv4_t<false, 1, 1>(p, sm_count, st) : mv4_t<false, 1, 2>(p, sm_count, st);
+      rc = nb == 1 ? mv4_t<false, 1, 1, 4>(p, a->E, sm_count, st) : mv4_t<false, 1, 2, 4>(p, a->E, sm_count, st);
     if (rc != ANIMA_OK) return rc;
   }
   return ANIMA_OK;

@@ -13,6 +13,8 @@
 // numbers n, exact in fp16 and bf16.  Within a word, nibbles p and p + 4 are neighbours e =
 // 2 p, 2 p + 1, so masking with 0x000f000f leaves a pair in consecutive order.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace anima {
@@ -20,6 +22,14 @@ namespace p4 {
 
 constexpr int kGroup = 32;   // values that share a scale
 constexpr int kBlock = 128;  // values of one 64-byte code block
+
+// (w & mask) | bits in one instruction.
+template <uint32_t kMask, uint32_t kBits>
+__device__ __forceinline__ uint32_t mask_or(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(kMask), "r"(kBits));
+  return r;
+}
 
 // Eight codes of word w as whole numbers n, four pairs in value order.  In fp16, 0x6400 | c is
 // 1024 + c and 0x6400 | 16 c is 1024 + 16 c, so one subtraction, or one fused multiply-add
@@ -29,11 +39,8 @@ __device__ __forceinline__ void numbers_f16(uint32_t w, uint32_t (&n)[4]) {
   const __half2 lo = __half2half2(__ushort_as_half(0x6408));         // 1032
   const __half2 sc = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
   const __half2 hi = __half2half2(__ushort_as_half(0xd480));         // -72
-  uint32_t t[4];
-  t[0] = (w & 0x000f000fu) | 0x64006400u;
-  t[1] = (w & 0x00f000f0u) | 0x64006400u;
-  t[2] = (w8 & 0x000f000fu) | 0x64006400u;
-  t[3] = (w8 & 0x00f000f0u) | 0x64006400u;
+  const uint32_t t[4] = {mask_or<0x000f000fu, 0x64006400u>(w), mask_or<0x00f000f0u, 0x64006400u>(w),
+                         mask_or<0x000f000fu, 0x64006400u>(w8), mask_or<0x00f000f0u, 0x64006400u>(w8)};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const __half2 v = *reinterpret_cast<const __half2*>(&t[k]);
@@ -44,11 +51,12 @@ __device__ __forceinline__ void numbers_f16(uint32_t w, uint32_t (&n)[4]) {
 
 // The same in bf16: 0x4300 | c is 128 + c (seven mantissa bits hold the four of c).
 __device__ __forceinline__ void numbers_bf16(uint32_t w, uint32_t (&n)[4]) {
-  const __nv_bfloat162 off = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));  // 136
+  const __nv_bfloat162 one = __bfloat162bfloat162(__ushort_as_bfloat16(0x3f80));
+  const __nv_bfloat162 off = __bfloat162bfloat162(__ushort_as_bfloat16(0xc308));  // -136
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t t = ((w >> (4 * k)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), off);
+    const uint32_t t = mask_or<0x000f000fu, 0x43004300u>(w >> (4 * k));
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&t), one, off);
     n[k] = *reinterpret_cast<const uint32_t*>(&r);
   }
 }
@@ -66,6 +74,41 @@ __device__ __forceinline__ float4 scales4(uint2 u) {
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
   return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Asynchronous copies of 16 and 8 bytes to shared memory; the _if forms write zeros, and read
+// nothing, where `take` is false.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp8_if(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 8 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
 }
 
 // D += A B, m16n8k16 with fp32 accumulation.  Lane 4 j + i holds A rows j (a0, a2) and j + 8
@@ -87,5 +130,52 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// D = A B of the same shapes.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 }  // namespace p4
+
+// Largest dynamic shared memory asked for a kernel so far, per device: the attribute is set when
+// a launch needs more, not at every launch.
+struct SmemAttr {
+  std::atomic<size_t> most[64];
+  SmemAttr() {
+    for (auto& m : most) m.store(0);
+  }
+  bool raise(const void* kern, size_t bytes, bool large_clusters = false) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (bytes <= most[dev].load(std::memory_order_acquire)) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    if (large_clusters &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    // a larger size set by another thread in between stays recorded or is set again
+    size_t seen = most[dev].load();
+    while (seen < bytes && !most[dev].compare_exchange_weak(seen, bytes)) {
+    }
+    return true;
+  }
+};
+
 }  // namespace anima

@@ -160,10 +160,20 @@ def test_struct_layouts(cls, cname, tmp_path):
         assert c[f] == getattr(cls, f).offset, f
 
 
+def test_packed_argument_layouts():
+    """The bytes that the Python entries pass are the structures of the header."""
+    m = P._MATVEC_ARGS.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18)
+    a = L.Matvec4Args(1, 2, (3, 4), 5, 6, 7, (8, 9), 10, 11, (12, 13), 14, 15, 16, 17, 18)
+    assert len(m) == ct.sizeof(a) and bytes(a) == m
+    m = P._ATTN_ARGS.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 0.5, 16, 17, 18, 19)
+    a = L.AttnKv4Args(1, 2, 3, 4, 5, 6, 7, (8, 9, 10), 11, 12, 13, 14, 15, 0.5, 16, 17, 18, 19)
+    assert len(m) == ct.sizeof(a) and bytes(a) == m
+
+
 @pytest.fixture
 def any_device(monkeypatch):
     """Lets the argument checks of the Python entries run on CPU tensors; the library is not called."""
-    monkeypatch.setattr(P, "_here", lambda *ts: None)
+    monkeypatch.setattr(P, "_here", lambda *ts: 0)
 
 
 def _pk(*shape):
