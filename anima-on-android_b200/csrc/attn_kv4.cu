@@ -25,6 +25,7 @@
 // workspace, no atomics; the order of all sums is fixed.
 #include <algorithm>
 
+#include "attn_kv4.cuh"
 #include "packed4.cuh"
 
 namespace anima {
@@ -466,7 +467,8 @@ __global__ void __launch_bounds__(256)
 }  // namespace kv4
 
 // Query rows per head up to which the packed cache is read directly.
-constexpr int kRowsFew = 64;
+constexpr int kRowsFew = 16;
+constexpr bool kUseTile = true;
 
 template <bool kBf16, int kW, int kNB, int kNS>
 static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
@@ -497,9 +499,11 @@ static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
 
 static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }
 
-// Bytes of workspace: none for few rows, else K and V in 16 bits.
-size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv) {
-  return S_q <= kRowsFew ? 0 : 2 * expanded_bytes((long long)B * H, S_kv);
+// Bytes of workspace: none for few rows.
+size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv, int sm_count) {
+  if (S_q <= kRowsFew) return 0;
+  if (kUseTile) return kv4_tile_plan(B * H, S_q, S_kv, sm_count).bytes;
+  return 2 * expanded_bytes((long long)B * H, S_kv);
 }
 
 int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st) {
@@ -543,6 +547,11 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     if (nb == 0) return bf ? rows_t<true, 4, 0, 3>(p, u, ncta, st) : rows_t<false, 4, 0, 3>(p, u, ncta, st);
     if (nb == 1) return bf ? rows_t<true, 4, 1, 3>(p, u, ncta, st) : rows_t<false, 4, 1, 3>(p, u, ncta, st);
     return bf ? rows_t<true, 4, 2, 3>(p, u, ncta, st) : rows_t<false, 4, 2, 3>(p, u, ncta, st);
+  }
+  if (kUseTile) {
+    const Kv4TilePlan t = kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count);
+    if (t.bytes > 0 && (!a->workspace || a->workspace_bytes < t.bytes)) return ANIMA_ERR_NOMEM;
+    return kv4_tile_launch(a, t, status, sm_count, st);
   }
   const size_t side = expanded_bytes(bh, a->S_kv);
   if (!a->workspace || a->workspace_bytes < 2 * side) return ANIMA_ERR_NOMEM;

@@ -1,0 +1,20 @@
+// attn_kv4.cuh -- host interface between the two kernels of the attention over packed K/V.
+#pragma once
+#include <stddef.h>
+
+#include "common.cuh"
+
+namespace anima {
+
+// A call of many query rows (attn_kv4_tile.cu).
+struct Kv4TilePlan {
+  int nt;           // 128-row query tiles per unit
+  int nqb;          // units per (batch, head)
+  long long units;
+  int nsplit;       // slices of a unit's keys
+  size_t bytes;     // workspace for the slices' partials
+};
+Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count);
+int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st);
+
+}  // namespace anima

@@ -1,0 +1,643 @@
+// attn_kv4_tile.cu -- attention over packed K and V (packed4.cuh) for many query rows, on the
+// tensor cores: tcgen05 MMAs with TMEM accumulators, K and V unpacked into shared memory by the
+// CTA itself.  out = softmax(q K^T * scale) V per (batch, head), D = 128.
+//
+// Work unit = kNT 128-row query tiles of one (batch, head) against a slice of its keys, in 128-key
+// tiles.  A unit whose keys are cut into several slices writes fp32 partials (O, running max, running
+// sum), which kv4_merge_kernel joins in slice order, so results repeat bit for bit.
+//
+// Operands are fp16 whatever q's type.  K and V: n * s rounded once (most codes make it exact).
+// q: fp16 as it is; bf16 rows are first scaled by the power of two that brings their largest
+// magnitude to [2^14, 2^15), which the row's softmax scale takes back, so a bf16 value keeps its
+// eight bits down to 2^-31 of the row's largest.
+//
+// Warp roles (16 warps):
+//   warps 0-3    softmax of query tile 0: thread = query row = TMEM lane.  Stages its q row,
+//                then per key tile reads its S row, updates max / sum, writes P over S.
+//   warps 4-7    softmax of query tile 1 (kNT = 2), or unpack (kNT = 1, where a key tile feeds
+//                half the MMA work and unpacking would bound it).
+//   warps 8-11   unpack: stream packed tiles through cp.async stages into 16-bit K / V tiles in the
+//                128-byte-swizzled layout of the MMA operands.
+//   warp 12      MMA issuer (one thread) + TMEM owner; warps 13-15 only fill its warpgroup.
+// Tensor memory: S_0, S_1, O_0, O_1 of 128 columns; P_i overlays S_i.  With two query tiles their
+// MMAs alternate, so one tile's softmax runs beside the other's MMAs; with one, its key tiles
+// alternate between S_0 and S_1, and a tile's QK^T runs beside the softmax of the tile before it.
+#include <algorithm>
+
+#include "attn_kv4.cuh"
+#include "attn_shared.cuh"
+#include "packed4.cuh"
+
+namespace anima {
+namespace kv4t {
+
+using namespace attn;  // kD, kBM, drain_wait, stage/store_block, pack2
+
+constexpr int kKeys = 128;                  // keys per tile
+constexpr int kSlots = 4;                   // unpacked K / V tiles
+constexpr int kRaw = 3;                     // packed tiles in flight
+constexpr int kPanel = 128 * 128;           // [128 rows][64 x 16-bit]
+constexpr int kTile = 2 * kPanel;
+constexpr int kRawBytes = kKeys * 64 + kKeys * 8;
+constexpr int kMmaWarp12 = 12;
+constexpr int kThreads16 = 512;
+// 512 threads launch with 128 registers each: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
+constexpr uint32_t kRegsSoft = 192, kRegsUnpack = 72, kRegsMma = 56;
+static_assert(2 * kRegsSoft + kRegsUnpack + kRegsMma == 4 * 128, "register split");
+
+struct Params {
+  const uint16_t* q;
+  const uint8_t* kc;
+  const uint8_t* ks;
+  const uint8_t* vc;
+  const uint8_t* vs;
+  const int* valid;
+  void* out;
+  float* part;         // partials, or nullptr: write the output
+  long long ob, oh, os;
+  int* status;
+  int H, S_q, S_kv;
+  int nqb;             // units per (batch, head)
+  int units;
+  int nsplit;
+  float scale_log2;
+};
+
+struct Smem {
+  uint8_t q[2][kTile];
+  uint8_t kv[kSlots][kTile];
+  uint8_t raw[kRaw][kRawBytes];
+  uint64_t q_full;
+  uint64_t kv_full[kSlots];
+  uint64_t kv_empty[kSlots];
+  uint64_t s_full[2];
+  uint64_t p_full[2];
+  uint64_t o_full[2];
+  uint64_t pv_done;
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+
+// Floats of one slice's partial of a unit: O [rows][128], m [rows], l [rows].
+__host__ __device__ constexpr long long part_floats(int rows) { return (long long)rows * (kD + 2); }
+
+// A thread's query row (256 bytes) into its swizzled place of the Q tile as fp16.  Returns the factor
+// that undoes the row's scaling.
+template <bool kBf16>
+__device__ __forceinline__ float stage_q(uint8_t* tile, int row, const uint4* src, bool take) {
+  uint4 v[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c) v[c] = take ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+  float back = 1.f;
+  if (kBf16) {
+    uint32_t top = 0;  // largest magnitude's bits (as bf16)
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+    }
+    // exponent e of the largest: scale by 2^(14 - e), in two steps so that neither factor leaves
+    // fp32; zero, subnormal and non-finite rows are left as they are
+    const int ex = (int)(top >> 7);
+    const int shift = ex == 0 || ex == 255 ? 0 : 14 - (ex - 127);
+    const int s0 = shift / 2, s1 = shift - s0;
+    const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
+    back = __int_as_float((127 - s0) << 23);
+    back *= __int_as_float((127 - s1) << 23);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = pack_f16x2(__uint_as_float(w[k] << 16) * f0 * f1, __uint_as_float(w[k] & 0xffff0000u) * f0 * f1);
+      v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 16; ++c)
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[c];
+  return back;
+}
+
+template <bool kBf16, int kNT>
+__global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + pad);
+  constexpr int kUnpackWarps = kNT == 2 ? 4 : 8;
+  constexpr int kRows = kNT * kBM;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &sm.abort;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, kRows);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&sm.kv_full[s], kUnpackWarps);
+      mbar_init(&sm.kv_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], kBM);
+      mbar_init(&sm.o_full[i], 1);
+    }
+    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.mma_done, 1);
+    sm.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp12) {
+    tmem_alloc(&sm.tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  const int slice = blockIdx.x / p.units, unit = blockIdx.x - slice * p.units;
+  const int bh = unit / p.nqb, q0 = (unit - bh * p.nqb) * kRows;
+  const int b = bh / p.H;
+  const int len = p.valid ? min(max(__ldg(p.valid + b), 0), p.S_kv) : p.S_kv;
+  const int ntiles = (len + kKeys - 1) / kKeys;
+  const int k0 = (int)((long long)ntiles * slice / p.nsplit);
+  const int n = (int)((long long)ntiles * (slice + 1) / p.nsplit) - k0;  // key tiles of this slice
+
+  if (warp >= kMmaWarp12) {
+    regs_dec<kRegsMma>();
+    if (warp == kMmaWarp12 && lane == 0 && n > 0) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_qk = make_idesc_f16(0u, kBM, kKeys, 0);
+      constexpr uint32_t idesc_pv = make_idesc_f16(0u, kBM, kD, 1);
+      const uint64_t dk0 = sdesc_sw128(smem_u32(sm.kv[0]), 16, 1024);
+      const uint64_t dv0 = sdesc_sw128(smem_u32(sm.kv[0]), kPanel, 1024);
+      const uint64_t dq0 = sdesc_sw128(smem_u32(sm.q[0]), 16, 1024);
+      auto issue_qk = [&](int i, int slot) {
+        const uint64_t kb = desc_plus(dk0, (uint32_t)slot * kTile);
+        uint64_t bd[8], aq[8];
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
+          aq[kk] = desc_plus(dq0, (uint32_t)i * kTile + (kk >> 2) * kPanel + (kk & 3) * 32);
+        }
+        umma_ss_x8(tmem + i * 128, aq, bd, idesc_qk, 0u);
+      };
+      auto issue_pv = [&](int i, int slot, bool acc) {
+        const uint64_t vb = desc_plus(dv0, (uint32_t)slot * kTile);
+        uint64_t bd[8];
+        uint32_t a[8];
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          bd[kk] = desc_plus(vb, kk * 2048);
+          a[kk] = tmem + i * 128 + kk * 8;
+        }
+        umma_ts_x8(tmem + 256 + i * 128, a, bd, idesc_pv, acc ? 1u : 0u);
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait(bar, parity, abort, p.status, ANIMA_ERR_TIMEOUT);
+      };
+      auto slot_of = [](int item) { return item % kSlots; };
+      auto par_of = [](int item) { return (uint32_t)(item / kSlots) & 1u; };
+      bool ok = wait(&sm.q_full, 0);
+      auto key_tile = [&](int item) {
+        ok = ok && wait(&sm.kv_full[slot_of(item)], par_of(item));
+        tc_fence_after();
+      };
+      if (kNT == 2) {
+        for (int g = 0; g <= n && ok; ++g) {
+          const int ik = 2 * g, iv = 2 * g - 1;  // K of step g, V of step g - 1
+          const uint32_t pp = (uint32_t)(g - 1) & 1u;
+          if (g > 0) key_tile(iv);
+#pragma unroll
+          for (int i = 0; i < kNT; ++i) {
+            if (g > 0) {
+              if (!(ok = ok && wait(&sm.p_full[i], pp))) break;
+              tc_fence_after();
+              issue_pv(i, slot_of(iv), g > 1);
+              if (g == n) umma_commit(&sm.o_full[i]);
+              if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(iv)]);
+            }
+            if (g < n) {
+              if (i == 0) key_tile(ik);
+              if (!ok) break;
+              issue_qk(i, slot_of(ik));
+              umma_commit(&sm.s_full[i]);
+              if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(ik)]);
+            }
+          }
+        }
+      } else {
+        // S of step g in columns 128 (g % 2); Q is tile 0 and O columns 256 .. 383 throughout.
+        auto qk = [&](int g) {
+          key_tile(2 * g);
+          if (!ok) return;
+          const uint64_t kb = desc_plus(dk0, (uint32_t)slot_of(2 * g) * kTile);
+          uint64_t bd[8], aq[8];
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
+            aq[kk] = desc_plus(dq0, (kk >> 2) * kPanel + (kk & 3) * 32);
+          }
+          umma_ss_x8(tmem + (g & 1) * 128, aq, bd, idesc_qk, 0u);
+          umma_commit(&sm.s_full[g & 1]);
+          umma_commit(&sm.kv_empty[slot_of(2 * g)]);
+        };
+        if (ok) qk(0);
+        for (int g = 0; g < n && ok; ++g) {
+          if (g + 1 < n) qk(g + 1);
+          if (!ok) break;
+          key_tile(2 * g + 1);
+          if (!(ok = ok && wait(&sm.p_full[g & 1], (uint32_t)(g >> 1) & 1u))) break;
+          tc_fence_after();
+          const uint64_t vb = desc_plus(dv0, (uint32_t)slot_of(2 * g + 1) * kTile);
+          uint64_t bd[8];
+          uint32_t a[8];
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            bd[kk] = desc_plus(vb, kk * 2048);
+            a[kk] = tmem + (g & 1) * 128 + kk * 8;
+          }
+          umma_ts_x8(tmem + 256, a, bd, idesc_pv, g > 0 ? 1u : 0u);
+          umma_commit(&sm.pv_done);
+          umma_commit(&sm.kv_empty[slot_of(2 * g + 1)]);
+        }
+        if (ok) umma_commit(&sm.o_full[0]);
+      }
+      umma_commit(&sm.mma_done);
+      drain_wait(&sm.mma_done, 0);
+    }
+    __syncwarp();
+  } else if (warp >= 4 * kNT) {
+    if (warp >= 8) regs_dec<kRegsUnpack>();
+    // ------------------------------------------------------------ unpack
+    // Eight rows at a time: lane 4 j + i has 16-byte chunk i (values 32 g + 8 i .. + 7 of the four
+    // groups) of row 8 c + r(j), r exchanging bits 0 and 2 of j's order so that the two rows of
+    // a quarter-warp's store lie in different halves of the swizzled 128 bytes.
+    const int w = warp - 4 * kNT;
+    const int i = lane & 3, jr = (((lane >> 2) & 1) << 2) | (lane >> 3);
+    constexpr int kGroups = 16 / kUnpackWarps;  // of eight rows, per item and warp
+    const uint32_t raw0 = smem_u32(sm.raw[0]);
+    const long long row_base = (long long)bh * p.S_kv + (long long)k0 * kKeys;
+    const int items = 2 * n, r0 = w * kGroups * 8 + jr;
+    const uint8_t* const kc = p.kc + (row_base + r0) * 64 + i * 16;
+    const uint8_t* const vc = p.vc + (row_base + r0) * 64 + i * 16;
+    const uint8_t* const ks = p.ks + (row_base + r0) * 8;
+    const uint8_t* const vs = p.vs + (row_base + r0) * 8;
+    const int left0 = len - k0 * kKeys - r0;  // valid keys from this lane's first row on
+    int ld_slot = 0;
+    auto load = [&](int item) {
+      if (item < items) {
+        const int tile = item >> 1;
+        const uint8_t* const codes = ((item & 1) ? vc : kc) + (long long)tile * (kKeys * 64);
+        const uint8_t* const scales = ((item & 1) ? vs : ks) + (long long)tile * (kKeys * 8);
+        const uint32_t dst = raw0 + ld_slot * kRawBytes + r0 * 64 + i * 16;
+        const uint32_t sdst = raw0 + ld_slot * kRawBytes + kKeys * 64 + r0 * 8;
+        const int left = left0 - tile * kKeys;
+        if ((tile + k0 + 1) * kKeys <= len) {
+#pragma unroll
+          for (int c = 0; c < kGroups; ++c) {
+            p4::cp16(dst + c * 512, codes + c * 512);
+            if (i == 0) p4::cp8(sdst + c * 64, scales + c * 64);
+          }
+        } else {  // keys past the length read as zeros
+#pragma unroll
+          for (int c = 0; c < kGroups; ++c) {
+            const bool take = 8 * c < left;
+            p4::cp16_if(dst + c * 512, take ? codes + c * 512 : p.kc, take);
+            if (i == 0) p4::cp8_if(sdst + c * 64, take ? scales + c * 64 : p.ks, take);
+          }
+        }
+      }
+      p4::cp_commit();
+      ld_slot = ld_slot + 1 == kRaw ? 0 : ld_slot + 1;
+    };
+    // where this lane's eight values of group g go: 16-byte chunk 4 (g % 2) + i of panel g / 2
+    uint32_t put[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) put[g] = r0 * 128 + (((4 * g + i) ^ (jr & 7)) << 4);
+#pragma unroll
+    for (int k = 0; k < kRaw - 1; ++k) load(k);
+    bool ok = true;
+    int raw = 0;
+    for (int item = 0; item < items; ++item) {
+      const int slot = item % kSlots;
+      p4::cp_wait<kRaw - 2>();
+      __syncwarp();
+      const uint32_t src = raw0 + raw * kRawBytes + r0 * 64 + i * 16;
+      const uint32_t ssrc = raw0 + raw * kRawBytes + kKeys * 64 + r0 * 8;
+      uint4 u[kGroups];
+      uint2 s2[kGroups];
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
+        u[c] = p4::lds16(src + c * 512);
+        s2[c] = p4::lds8(ssrc + c * 64);
+      }
+      raw = raw + 1 == kRaw ? 0 : raw + 1;
+      load(item + kRaw - 1);  // into the slot of the item before this one
+      const bool got = mbar_wait(&sm.kv_empty[slot], ((uint32_t)(item / kSlots) & 1u) ^ 1u, abort, p.status,
+                                 ANIMA_ERR_TIMEOUT);
+      if (!(ok = __all_sync(0xffffffffu, got))) break;
+      const uint32_t dst = smem_u32(sm.kv[slot]);
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
+        const uint32_t wd[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+        const __half2 sa = *reinterpret_cast<const __half2*>(&s2[c].x);
+        const __half2 sb = *reinterpret_cast<const __half2*>(&s2[c].y);
+        const __half2 sg[4] = {__low2half2(sa), __high2half2(sa), __low2half2(sb), __high2half2(sb)};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t v[4];
+          p4::numbers_f16(wd[g], v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&v[k]), sg[g]);
+            v[k] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+          st_shared_v4(dst + (g >> 1) * kPanel + put[g & 1] + c * 1024, v[0], v[1], v[2], v[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.kv_full[slot]);
+    }
+    p4::cp_wait<0>();
+  } else {
+    regs_inc<kRegsSoft>();
+    // ------------------------------------------------------------ softmax / epilogue
+    const int i = warp >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tO = tmem + lane_field + 256 + i * 128;
+    const int grow = q0 + i * kBM + row;
+    const float back = stage_q<kBf16>(
+        sm.q[i], row, reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + min(grow, p.S_q - 1)) * kD),
+        grow < p.S_q);
+    const float sl2 = p.scale_log2 * back;
+    fence_proxy_async_smem();
+    mbar_arrive(&sm.q_full);
+
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int g = 0; g < n; ++g) {
+      const int buf = kNT == 2 ? i : g & 1;  // S and its barriers
+      const uint32_t tS = tmem + lane_field + buf * 128;
+      const bool got = mbar_wait(&sm.s_full[buf], (uint32_t)(kNT == 2 ? g : g >> 1) & 1u, abort, p.status,
+                                 ANIMA_ERR_TIMEOUT);
+      if (!(ok = __all_sync(0xffffffffu, got))) break;
+      tc_fence_after();
+      uint32_t r[4][32];
+      const int lim = len - (k0 + g) * kKeys;
+      const bool full = lim >= kKeys;
+      auto load_s = [&]() {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+        tmem_ld_wait();
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= lim) r[c][e] = __float_as_uint(-INFINITY);
+        }
+      };
+#define SV(e) __uint_as_float(r[(e) >> 5][(e) & 31])
+      auto row_max = [&]() {
+        float acc[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = fmaxf(SV(2 * k), SV(2 * k + 1));
+#pragma unroll
+        for (int e = 16; e < 128; e += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = max3f(acc[k], SV(e + 2 * k), SV(e + 2 * k + 1));
+        return max3f(max3f(acc[0], acc[1], acc[2]), max3f(acc[3], acc[4], acc[5]), fmaxf(acc[6], acc[7]));
+      };
+      uint64_t sum2[4];
+      uint32_t pk[2][32];
+      auto exp_pass = [&](float mu) {
+        const float nb = (mu == -INFINITY) ? 0.f : -mu;
+        const uint64_t scale2 = f2pack(sl2, sl2), base2 = f2pack(nb, nb);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum2[k] = 0ull;
+#pragma unroll
+        for (int pr = 0; pr < 64; ++pr) {
+          float x0, x1;
+          f2unpack(fma2(f2pack(SV(2 * pr), SV(2 * pr + 1)), scale2, base2), x0, x1);
+          x0 = ex2_approx(x0);
+          x1 = ex2_approx(x1);
+          sum2[pr & 3] = add2(sum2[pr & 3], f2pack(x0, x1));
+          pk[pr >> 5][pr & 31] = pack_f16x2(x0, x1);
+        }
+      };
+      auto row_sum = [&]() {
+        float sa, sb;
+        f2unpack(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sa, sb);
+        return sa + sb;
+      };
+      // As in the core kernel: P with the running max straight away; the row sum tells
+      // whether it has to be redone with a larger one.
+      load_s();
+      float m_use = m, alpha = 1.f, sum;
+      if (g == 0) {
+        m_use = row_max() * sl2;
+        alpha = 0.f;
+        exp_pass(m_use);
+        sum = row_sum();
+      } else {
+        exp_pass(m);
+        sum = row_sum();
+        const bool check = !(sum <= 256.f) || (m == -INFINITY && sum > 0.f);
+        if (__any_sync(0xffffffffu, check)) {
+          load_s();
+          const float m_tile = row_max() * sl2;
+          if (m == -INFINITY) {
+            m_use = m_tile;
+            alpha = 0.f;
+          } else if (m_tile > m + kRescaleThreshold) {
+            m_use = m_tile;
+            alpha = ex2_approx(m - m_tile);
+          }
+          exp_pass(m_use);
+          sum = row_sum();
+        }
+      }
+      tmem_st32(tS, pk[0]);
+      tmem_st32(tS + 32, pk[1]);
+#undef SV
+      l = l * alpha + sum;
+      if (__any_sync(0xffffffffu, g > 0 && alpha != 1.f)) {
+        if (kNT == 1) {  // the PV before this step may still run (s_full covers it with two tiles)
+          const bool idle = mbar_wait(&sm.pv_done, (uint32_t)(g - 1) & 1u, abort, p.status, ANIMA_ERR_TIMEOUT);
+          if (!(ok = __all_sync(0xffffffffu, idle))) break;
+          tc_fence_after();
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(tO + c * 32, o);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[buf]);
+      m = m_use;
+    }
+    if (ok && n > 0) {
+      const bool got = mbar_wait(&sm.o_full[i], 0, abort, p.status, ANIMA_ERR_TIMEOUT);
+      ok = __all_sync(0xffffffffu, got);
+      tc_fence_after();
+    }
+    if (ok) {
+      // The query tile's shared memory is free (its last QK^T is done): 4 KB of it per warp stage
+      // the output blocks.
+      float4* const stage = reinterpret_cast<float4*>(sm.q[i]) + quarter * 256;
+      const int r0 = grow - lane;  // the warp's first row
+      const int nvalid = p.S_q - r0;
+      const bool direct = p.part == nullptr;
+      const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;  // no key: zeros
+      const long long urow = i * kBM + quarter * 32;
+      float* const part = direct ? nullptr : p.part + ((long long)slice * p.units + unit) * part_floats(kRows);
+      char* const out_w = static_cast<char*>(p.out) +
+                          ((long long)b * p.ob + (long long)(bh % p.H) * p.oh + (long long)r0 * p.os) * 2;
+#pragma unroll 1
+      for (int c = 0; c < 4 && (direct || n > 0); ++c) {
+        float v[32];
+        if (n > 0) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        }
+        if (direct)
+          store_block<kBf16 ? ANIMA_DTYPE_BF16 : ANIMA_DTYPE_F16>(out_w, p.os * 2, nvalid, v, c, inv, stage, lane);
+        else
+          store_block<ANIMA_DTYPE_F32>(reinterpret_cast<char*>(part + urow * kD), kD * 4, nvalid, v, c, 1.f, stage, lane);
+      }
+      if (!direct) {
+        part[kRows * kD + urow + lane] = m;
+        part[kRows * kD + kRows + urow + lane] = l;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the slices of every query row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, in
+// slice order.  One warp per row, four columns per lane.  part: [slice][unit][part_floats(rows)].
+template <bool kBf16>
+__global__ void __launch_bounds__(256)
+    kv4_merge_kernel(const float* part, void* out, long long ob, long long oh, long long os, int H, int S_q,
+                     int nqb, int rows, int units, int nsplit, long long total) {
+  const int lane = threadIdx.x & 31;
+  const long long stride = (long long)units * part_floats(rows);
+  for (long long t = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < total;
+       t += ((long long)gridDim.x * blockDim.x) >> 5) {
+    const int bh = (int)(t / S_q), s = (int)(t - (long long)bh * S_q);
+    const int unit = bh * nqb + s / rows, r = s % rows;
+    const float* const base = part + (long long)unit * part_floats(rows);
+    const float* const mp = base + (long long)rows * kD + r;
+    float M = -INFINITY;
+    for (int k = 0; k < nsplit; ++k) M = fmaxf(M, mp[k * stride]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+    for (int k = 0; k < nsplit; ++k) {
+      const float mk = mp[k * stride];
+      const float f = mk == -INFINITY ? 0.f : ex2_approx(mk - M);
+      const float4 o = *reinterpret_cast<const float4*>(base + k * stride + (long long)r * kD + lane * 4);
+      if (mk == -INFINITY) continue;  // a slice without keys, whose O is not written
+      acc.x = fmaf(f, o.x, acc.x);
+      acc.y = fmaf(f, o.y, acc.y);
+      acc.z = fmaf(f, o.z, acc.z);
+      acc.w = fmaf(f, o.w, acc.w);
+      den = fmaf(f, mp[k * stride + rows], den);
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    uint32_t w0, w1;
+    if (kBf16) {
+      w0 = pack_bf16x2(acc.x * inv, acc.y * inv);
+      w1 = pack_bf16x2(acc.z * inv, acc.w * inv);
+    } else {
+      w0 = pack_f16x2(acc.x * inv, acc.y * inv);
+      w1 = pack_f16x2(acc.z * inv, acc.w * inv);
+    }
+    const long long at = (long long)(bh / H) * ob + (long long)(bh % H) * oh + (long long)s * os + lane * 4;
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w0, w1);
+  }
+}
+
+}  // namespace kv4t
+
+// How a call of many rows is cut: query tiles per unit, units, slices of the keys.
+Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
+  Kv4TilePlan t;
+  t.nt = S_q <= attn::kBM ? 1 : 2;
+  t.nqb = (S_q + t.nt * attn::kBM - 1) / (t.nt * attn::kBM);
+  t.units = (long long)bh * t.nqb;
+  const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
+  // as many slices as the SMs hold in one round, of two key tiles or more
+  t.nsplit = (int)std::max(1LL, std::min({sm_count / std::max(1LL, t.units), tiles / 2, 64LL}));
+  t.bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4t::part_floats(t.nt * attn::kBM)) * 4 : 0;
+  return t;
+}
+
+template <bool kBf16, int kNT>
+static int tile_t(const kv4t::Params& p, int grid, cudaStream_t st) {
+  auto kern = kv4t::kv4_tile_kernel<kBf16, kNT>;
+  static SmemAttr attr;
+  if (!attr.raise((const void*)kern, kv4t::kSmemBytes)) return ANIMA_ERR_CUDA;
+  kern<<<grid, kv4t::kThreads16, kv4t::kSmemBytes, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+}
+
+int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st) {
+  const bool bf = a->dtype == ANIMA_DTYPE_BF16;
+  if (t.units * t.nsplit > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
+  kv4t::Params p;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.kc = static_cast<const uint8_t*>(a->k_codes);
+  p.ks = static_cast<const uint8_t*>(a->k_scales);
+  p.vc = static_cast<const uint8_t*>(a->v_codes);
+  p.vs = static_cast<const uint8_t*>(a->v_scales);
+  p.valid = (a->flags & ANIMA_FLAG_MASK) ? a->kv_valid_len : nullptr;
+  p.out = a->out;
+  p.part = t.nsplit > 1 ? static_cast<float*>(a->workspace) : nullptr;
+  p.ob = a->out_stride[0];
+  p.oh = a->out_stride[1];
+  p.os = a->out_stride[2];
+  p.status = status;
+  p.H = a->H;
+  p.S_q = a->S_q;
+  p.S_kv = a->S_kv;
+  p.nqb = t.nqb;
+  p.units = (int)t.units;
+  p.nsplit = t.nsplit;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  const int grid = (int)t.units * t.nsplit;
+  const int rc = t.nt == 1 ? (bf ? tile_t<true, 1>(p, grid, st) : tile_t<false, 1>(p, grid, st))
+                           : (bf ? tile_t<true, 2>(p, grid, st) : tile_t<false, 2>(p, grid, st));
+  if (rc != ANIMA_OK || t.nsplit == 1) return rc;
+  const long long total = (long long)a->B * a->H * a->S_q;
+  const int mg = (int)std::min<long long>((total + 7) / 8, (long long)sm_count * 8);
+  auto merge = bf ? kv4t::kv4_merge_kernel<true> : kv4t::kv4_merge_kernel<false>;
+  merge<<<mg, 256, 0, st>>>(p.part, a->out, p.ob, p.oh, p.os, a->H, a->S_q, t.nqb, t.nt * attn::kBM, p.units,
+                            t.nsplit, total);
+  return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+}
+
+}  // namespace anima
