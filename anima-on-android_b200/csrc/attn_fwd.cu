@@ -526,6 +526,11 @@ static int make_head_map(CUtensorMap* map, const void* base, int op_dtype, int b
   return r == CUDA_SUCCESS ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 
+// The same for the other attention kernels.
+int attn_head_map(CUtensorMap* map, const void* base, int op_dtype, int bh, int rows) {
+  return make_head_map(map, base, op_dtype, bh, rows);
+}
+
 // Output [B, S_q, H, 128] addressed by element strides (ob, oh, os) as a TMA tile map for
 // the epilogue's 32 x 32 blocks (box: 32 columns x 32 tokens of one head), axes ordered by
 // stride: (D, H, S, B) when heads are closer than tokens (token-major output), else

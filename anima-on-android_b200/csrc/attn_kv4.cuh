@@ -6,6 +6,10 @@
 
 namespace anima {
 
+// Tensor map of a [bh][rows][128] 16-bit operand, boxes of 128 rows x 64 elements, 128-byte
+// swizzle (attn_fwd.cu).
+int attn_head_map(CUtensorMap* map, const void* base, int op_dtype, int bh, int rows);
+
 // A call of many query rows (attn_kv4_tile.cu).
 struct Kv4TilePlan {
   int nt;           // 128-row query tiles per unit

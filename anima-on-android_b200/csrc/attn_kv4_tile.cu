@@ -2,9 +2,12 @@
 // tensor cores: tcgen05 MMAs with TMEM accumulators, K and V unpacked into shared memory by the
 // CTA itself.  out = softmax(q K^T * scale) V per (batch, head), D = 128.
 //
-// Work unit = kNT 128-row query tiles of one (batch, head) against a slice of its keys, in 128-key
-// tiles.  A unit whose keys are cut into several slices writes fp32 partials (O, running max, running
-// sum), which kv4_merge_kernel joins in slice order, so results repeat bit for bit.
+// Work unit = kNT 128-row query tiles of one (batch, head); its keys may be cut into slices, and
+// (unit, slice) is a segment, streamed in 128-key tiles.  The grid is persistent: a CTA takes
+// segments c, c + G, ..., and moves from one to the next without draining (the next Q tile, K and V
+// are under way while the last P V and the output of the segment before run).  A unit cut into
+// slices writes fp32 partials (O, running max, running sum), which kv4_merge_kernel joins in slice
+// order, so results repeat bit for bit.
 //
 // Operands are fp16 whatever q's type.  K and V: n * s rounded once (most codes make it exact).
 // q: fp16 as it is; bf16 rows are first scaled by the power of two that brings their largest
@@ -12,13 +15,15 @@
 // eight bits down to 2^-31 of the row's largest.
 //
 // Warp roles (16 warps):
-//   warps 0-3    softmax of query tile 0: thread = query row = TMEM lane.  Stages its q row,
-//                then per key tile reads its S row, updates max / sum, writes P over S.
+//   warps 0-3    softmax of query tile 0: thread = query row = TMEM lane.  Per key tile reads its S
+//                row, updates max / sum, writes P over S; at the end stores O.  A bf16 Q
+//                tile is converted in place by its warpgroup before its first MMA.
 //   warps 4-7    softmax of query tile 1 (kNT = 2), or unpack (kNT = 1, where a key tile feeds
 //                half the MMA work and unpacking would bound it).
 //   warps 8-11   unpack: stream packed tiles through cp.async stages into 16-bit K / V tiles in the
 //                128-byte-swizzled layout of the MMA operands.
-//   warp 12      MMA issuer (one thread) + TMEM owner; warps 13-15 only fill its warpgroup.
+//   warp 12      MMA issuer (one thread) + TMEM owner.
+//   warp 13      TMA producer of the Q tiles; warps 14 and 15 only fill the warpgroup.
 // Tensor memory: S_0, S_1, O_0, O_1 of 128 columns; P_i overlays S_i.  With two query tiles their
 // MMAs alternate, so one tile's softmax runs beside the other's MMAs; with one, its key tiles
 // alternate between S_0 and S_1, and a tile's QK^T runs beside the softmax of the tile before it.
@@ -34,19 +39,17 @@ namespace kv4t {
 using namespace attn;  // kD, kBM, drain_wait, stage/store_block, pack2
 
 constexpr int kKeys = 128;                  // keys per tile
-constexpr int kSlots = 4;                   // unpacked K / V tiles
 constexpr int kRaw = 3;                     // packed tiles in flight
 constexpr int kPanel = 128 * 128;           // [128 rows][64 x 16-bit]
 constexpr int kTile = 2 * kPanel;
 constexpr int kRawBytes = kKeys * 64 + kKeys * 8;
-constexpr int kMmaWarp12 = 12;
+constexpr int kMmaWarp12 = 12, kQWarp13 = 13;
 constexpr int kThreads16 = 512;
 // 512 threads launch with 128 registers each: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
 constexpr uint32_t kRegsSoft = 192, kRegsUnpack = 72, kRegsMma = 56;
 static_assert(2 * kRegsSoft + kRegsUnpack + kRegsMma == 4 * 128, "register split");
 
 struct Params {
-  const uint16_t* q;
   const uint8_t* kc;
   const uint8_t* ks;
   const uint8_t* vc;
@@ -63,86 +66,111 @@ struct Params {
   float scale_log2;
 };
 
+template <int kNT>
 struct Smem {
-  uint8_t q[2][kTile];
+  static constexpr int kSlots = kNT == 2 ? 3 : 4;  // unpacked K / V tiles
+  uint8_t q[kNT][kTile];
   uint8_t kv[kSlots][kTile];
   uint8_t raw[kRaw][kRawBytes];
-  uint64_t q_full;
+  float4 stage[kNT * 4][256];  // per softmax warp: one 32 x 32 block on its way to global
+  uint64_t q_raw[2];           // Q tile as loaded
+  uint64_t q_conv[2];          // bf16: converted
+  uint64_t q_empty[2];
   uint64_t kv_full[kSlots];
   uint64_t kv_empty[kSlots];
   uint64_t s_full[2];
   uint64_t p_full[2];
   uint64_t o_full[2];
+  uint64_t o_empty[2];
   uint64_t pv_done;
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
 };
-constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
-static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+template <int kNT>
+constexpr size_t smem_bytes() {
+  return sizeof(Smem<kNT>) + 1024;
+}
+static_assert(smem_bytes<1>() <= 227 * 1024 && smem_bytes<2>() <= 227 * 1024, "shared memory budget");
+
+// A segment: key tiles [k0, k0 + n) of a unit.
+struct Seg {
+  int unit, slice, bh, b, q0, len, k0, n;
+};
+__device__ __forceinline__ Seg segment(const Params& p, int seg, int rows) {
+  Seg s;
+  s.slice = seg / p.units;
+  s.unit = seg - s.slice * p.units;
+  s.bh = s.unit / p.nqb;
+  s.q0 = (s.unit - s.bh * p.nqb) * rows;
+  s.b = s.bh / p.H;
+  s.len = p.valid ? min(max(__ldg(p.valid + s.b), 0), p.S_kv) : p.S_kv;
+  const int tiles = (s.len + kKeys - 1) / kKeys;
+  s.k0 = (int)((long long)tiles * s.slice / p.nsplit);
+  s.n = (int)((long long)tiles * (s.slice + 1) / p.nsplit) - s.k0;
+  return s;
+}
 
 // Floats of one slice's partial of a unit: O [rows][128], m [rows], l [rows].
 __host__ __device__ constexpr long long part_floats(int rows) { return (long long)rows * (kD + 2); }
 
-// A thread's query row (256 bytes) into its swizzled place of the Q tile as fp16.  Returns the factor
-// that undoes the row's scaling.
-template <bool kBf16>
-__device__ __forceinline__ float stage_q(uint8_t* tile, int row, const uint4* src, bool take) {
+// A thread's bf16 query row of a Q tile to fp16 in place, scaled; returns the factor that undoes it.
+__device__ __forceinline__ float convert_row(uint8_t* tile, int row) {
+  auto at = [&](int c) {
+    return reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+  };
   uint4 v[16];
 #pragma unroll
-  for (int c = 0; c < 16; ++c) v[c] = take ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
-  float back = 1.f;
-  if (kBf16) {
-    uint32_t top = 0;  // largest magnitude's bits (as bf16)
+  for (int c = 0; c < 16; ++c) v[c] = *at(c);
+  uint32_t top = 0;  // largest magnitude's bits
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+  for (int c = 0; c < 16; ++c) {
+    const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-    }
-    // exponent e of the largest: scale by 2^(14 - e), in two steps so that neither factor leaves
-    // fp32; zero, subnormal and non-finite rows are left as they are
-    const int ex = (int)(top >> 7);
-    const int shift = ex == 0 || ex == 255 ? 0 : 14 - (ex - 127);
-    const int s0 = shift / 2, s1 = shift - s0;
-    const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
-    back = __int_as_float((127 - s0) << 23);
-    back *= __int_as_float((127 - s1) << 23);
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k] = pack_f16x2(__uint_as_float(w[k] << 16) * f0 * f1, __uint_as_float(w[k] & 0xffff0000u) * f0 * f1);
-      v[c] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
   }
+  // With exponent e of the largest, scale by 2^(14 - e), in two steps so that neither factor leaves
+  // fp32; zero, subnormal and non-finite rows are left as they are.
+  const int ex = (int)(top >> 7);
+  const int shift = ex == 0 || ex == 255 ? 0 : 14 - (ex - 127);
+  const int s0 = shift / 2, s1 = shift - s0;
+  const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
 #pragma unroll
-  for (int c = 0; c < 16; ++c)
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[c];
-  return back;
+  for (int c = 0; c < 16; ++c) {
+    uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      w[k] = pack_f16x2(__uint_as_float(w[k] << 16) * f0 * f1, __uint_as_float(w[k] & 0xffff0000u) * f0 * f1);
+    *at(c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return __int_as_float((127 - s0) << 23) * __int_as_float((127 - s1) << 23);
 }
 
 template <bool kBf16, int kNT>
-__global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads16, 1)
+    kv4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + pad);
+  Smem<kNT>& sm = *reinterpret_cast<Smem<kNT>*>(smem_raw + pad);
   constexpr int kUnpackWarps = kNT == 2 ? 4 : 8;
   constexpr int kRows = kNT * kBM;
+  constexpr int kSlots = Smem<kNT>::kSlots;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   if (threadIdx.x == 0) {
-    mbar_init(&sm.q_full, kRows);
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], kUnpackWarps);
       mbar_init(&sm.kv_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_raw[i], 1);
+      mbar_init(&sm.q_conv[i], kBM);
+      mbar_init(&sm.q_empty[i], 1);
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], kBM);
       mbar_init(&sm.o_full[i], 1);
+      mbar_init(&sm.o_empty[i], kBM);
     }
     mbar_init(&sm.pv_done, 1);
     mbar_init(&sm.mma_done, 1);
@@ -157,18 +185,39 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-
-  const int slice = blockIdx.x / p.units, unit = blockIdx.x - slice * p.units;
-  const int bh = unit / p.nqb, q0 = (unit - bh * p.nqb) * kRows;
-  const int b = bh / p.H;
-  const int len = p.valid ? min(max(__ldg(p.valid + b), 0), p.S_kv) : p.S_kv;
-  const int ntiles = (len + kKeys - 1) / kKeys;
-  const int k0 = (int)((long long)ntiles * slice / p.nsplit);
-  const int n = (int)((long long)ntiles * (slice + 1) / p.nsplit) - k0;  // key tiles of this slice
+  const int segs = p.units * p.nsplit;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, abort, p.status, ANIMA_ERR_TIMEOUT);
+  };
+  // Every role walks the same segments; `a` counts those with keys, `gg` their key-tile steps.
 
   if (warp >= kMmaWarp12) {
     regs_dec<kRegsMma>();
-    if (warp == kMmaWarp12 && lane == 0 && n > 0) {
+    if (warp == kQWarp13 && lane == 0) {
+      // ---------------------------------------------------------- Q producer
+      tma_prefetch_desc(&tmap_q);
+      int a = 0;
+      bool ok = true;
+      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
+        const Seg s = segment(p, seg, kRows);
+        if (s.n <= 0) continue;
+        for (int i = 0; i < kNT && ok; ++i) {
+          if (a > 0 && !(ok = wait(&sm.q_empty[i], (uint32_t)(a - 1) & 1u))) break;
+          mbar_arrive_expect_tx(&sm.q_raw[i], kTile);
+          for (int pn = 0; pn < 2; ++pn)
+            tma_load_3d(sm.q[i] + pn * kPanel, &tmap_q, &sm.q_raw[i], pn * 64, s.q0 + i * kBM, s.bh);
+        }
+        if (ok) ++a;
+      }
+      // every copy this thread started lands before the CTA may exit
+      if (ok && a > 0)
+        for (int i = 0; i < kNT; ++i) drain_wait(&sm.q_raw[i], (uint32_t)(a - 1) & 1u);
+      if (!ok)  // an aborted round may have loaded tile 0 only
+        for (int i = 0; i < kNT; ++i) {
+          if (a > 0) drain_wait(&sm.q_raw[i], (uint32_t)(a - 1) & 1u);
+          if (i == 0) drain_wait(&sm.q_raw[0], (uint32_t)a & 1u);
+        }
+    } else if (warp == kMmaWarp12 && lane == 0) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_qk = make_idesc_f16(0u, kBM, kKeys, 0);
       constexpr uint32_t idesc_pv = make_idesc_f16(0u, kBM, kD, 1);
@@ -196,75 +245,91 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
         }
         umma_ts_x8(tmem + 256 + i * 128, a, bd, idesc_pv, acc ? 1u : 0u);
       };
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait(bar, parity, abort, p.status, ANIMA_ERR_TIMEOUT);
-      };
       auto slot_of = [](int item) { return item % kSlots; };
       auto par_of = [](int item) { return (uint32_t)(item / kSlots) & 1u; };
-      bool ok = wait(&sm.q_full, 0);
+      bool ok = true;
       auto key_tile = [&](int item) {
         ok = ok && wait(&sm.kv_full[slot_of(item)], par_of(item));
         tc_fence_after();
       };
-      if (kNT == 2) {
-        for (int g = 0; g <= n && ok; ++g) {
-          const int ik = 2 * g, iv = 2 * g - 1;  // K of step g, V of step g - 1
-          const uint32_t pp = (uint32_t)(g - 1) & 1u;
-          if (g > 0) key_tile(iv);
+      auto query_tile = [&](int i, int a) {
+        ok = ok && wait(kBf16 ? &sm.q_conv[i] : &sm.q_raw[i], (uint32_t)a & 1u);
+        tc_fence_after();
+      };
+      int a = 0, gg = 0;
+      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
+        const int n = segment(p, seg, kRows).n;
+        if (n <= 0) continue;
+        const uint32_t pa = (uint32_t)(a - 1) & 1u;
+        if (kNT == 2) {
+          for (int g = 0; g <= n && ok; ++g) {
+            const int ik = 2 * (gg + g), iv = ik - 1;  // K of this step, V of the one before
+            const uint32_t pp = (uint32_t)(gg + g - 1) & 1u;
+            if (g > 0) key_tile(iv);
 #pragma unroll
-          for (int i = 0; i < kNT; ++i) {
-            if (g > 0) {
-              if (!(ok = ok && wait(&sm.p_full[i], pp))) break;
-              tc_fence_after();
-              issue_pv(i, slot_of(iv), g > 1);
-              if (g == n) umma_commit(&sm.o_full[i]);
-              if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(iv)]);
+            for (int i = 0; i < kNT; ++i) {
+              if (g > 0) {
+                if (!(ok = ok && wait(&sm.p_full[i], pp))) break;
+                if (g == 1 && a > 0 && !(ok = wait(&sm.o_empty[i], pa))) break;
+                tc_fence_after();
+                issue_pv(i, slot_of(iv), g > 1);
+                if (g == n) umma_commit(&sm.o_full[i]);
+                if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(iv)]);
+              }
+              if (g < n) {
+                if (g == 0) query_tile(i, a);
+                if (i == 0) key_tile(ik);
+                if (!ok) break;
+                issue_qk(i, slot_of(ik));
+                umma_commit(&sm.s_full[i]);
+                if (g == n - 1) umma_commit(&sm.q_empty[i]);
+                if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(ik)]);
+              }
             }
-            if (g < n) {
-              if (i == 0) key_tile(ik);
-              if (!ok) break;
-              issue_qk(i, slot_of(ik));
-              umma_commit(&sm.s_full[i]);
-              if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(ik)]);
+          }
+        } else {
+          // S of step t in columns 128 (t % 2); Q is tile 0 and O columns 256 .. 383 throughout.
+          auto qk = [&](int t, bool last) {
+            key_tile(2 * t);
+            if (!ok) return;
+            const uint64_t kb = desc_plus(dk0, (uint32_t)slot_of(2 * t) * kTile);
+            uint64_t bd[8], aq[8];
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
+              aq[kk] = desc_plus(dq0, (kk >> 2) * kPanel + (kk & 3) * 32);
             }
-          }
-        }
-      } else {
-        // S of step g in columns 128 (g % 2); Q is tile 0 and O columns 256 .. 383 throughout.
-        auto qk = [&](int g) {
-          key_tile(2 * g);
-          if (!ok) return;
-          const uint64_t kb = desc_plus(dk0, (uint32_t)slot_of(2 * g) * kTile);
-          uint64_t bd[8], aq[8];
+            umma_ss_x8(tmem + (t & 1) * 128, aq, bd, idesc_qk, 0u);
+            umma_commit(&sm.s_full[t & 1]);
+            if (last) umma_commit(&sm.q_empty[0]);
+            umma_commit(&sm.kv_empty[slot_of(2 * t)]);
+          };
+          query_tile(0, a);
+          if (ok) qk(gg, n == 1);
+          for (int g = 0; g < n && ok; ++g) {
+            const int t = gg + g;
+            if (g + 1 < n) qk(t + 1, g + 2 == n);
+            if (!ok) break;
+            key_tile(2 * t + 1);
+            if (!(ok = ok && wait(&sm.p_full[t & 1], (uint32_t)(t >> 1) & 1u))) break;
+            if (g == 0 && a > 0 && !(ok = wait(&sm.o_empty[0], pa))) break;
+            tc_fence_after();
+            const uint64_t vb = desc_plus(dv0, (uint32_t)slot_of(2 * t + 1) * kTile);
+            uint64_t bd[8];
+            uint32_t ap[8];
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
-            aq[kk] = desc_plus(dq0, (kk >> 2) * kPanel + (kk & 3) * 32);
+            for (int kk = 0; kk < 8; ++kk) {
+              bd[kk] = desc_plus(vb, kk * 2048);
+              ap[kk] = tmem + (t & 1) * 128 + kk * 8;
+            }
+            umma_ts_x8(tmem + 256, ap, bd, idesc_pv, g > 0 ? 1u : 0u);
+            umma_commit(&sm.pv_done);
+            umma_commit(&sm.kv_empty[slot_of(2 * t + 1)]);
           }
-          umma_ss_x8(tmem + (g & 1) * 128, aq, bd, idesc_qk, 0u);
-          umma_commit(&sm.s_full[g & 1]);
-          umma_commit(&sm.kv_empty[slot_of(2 * g)]);
-        };
-        if (ok) qk(0);
-        for (int g = 0; g < n && ok; ++g) {
-          if (g + 1 < n) qk(g + 1);
-          if (!ok) break;
-          key_tile(2 * g + 1);
-          if (!(ok = ok && wait(&sm.p_full[g & 1], (uint32_t)(g >> 1) & 1u))) break;
-          tc_fence_after();
-          const uint64_t vb = desc_plus(dv0, (uint32_t)slot_of(2 * g + 1) * kTile);
-          uint64_t bd[8];
-          uint32_t a[8];
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            bd[kk] = desc_plus(vb, kk * 2048);
-            a[kk] = tmem + (g & 1) * 128 + kk * 8;
-          }
-          umma_ts_x8(tmem + 256, a, bd, idesc_pv, g > 0 ? 1u : 0u);
-          umma_commit(&sm.pv_done);
-          umma_commit(&sm.kv_empty[slot_of(2 * g + 1)]);
+          if (ok) umma_commit(&sm.o_full[0]);
         }
-        if (ok) umma_commit(&sm.o_full[0]);
+        gg += n;
+        ++a;
       }
       umma_commit(&sm.mma_done);
       drain_wait(&sm.mma_done, 0);
@@ -280,23 +345,29 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
     const int i = lane & 3, jr = (((lane >> 2) & 1) << 2) | (lane >> 3);
     constexpr int kGroups = 16 / kUnpackWarps;  // of eight rows, per item and warp
     const uint32_t raw0 = smem_u32(sm.raw[0]);
-    const long long row_base = (long long)bh * p.S_kv + (long long)k0 * kKeys;
-    const int items = 2 * n, r0 = w * kGroups * 8 + jr;
-    const uint8_t* const kc = p.kc + (row_base + r0) * 64 + i * 16;
-    const uint8_t* const vc = p.vc + (row_base + r0) * 64 + i * 16;
-    const uint8_t* const ks = p.ks + (row_base + r0) * 8;
-    const uint8_t* const vs = p.vs + (row_base + r0) * 8;
-    const int left0 = len - k0 * kKeys - r0;  // valid keys from this lane's first row on
-    int ld_slot = 0;
-    auto load = [&](int item) {
-      if (item < items) {
-        const int tile = item >> 1;
-        const uint8_t* const codes = ((item & 1) ? vc : kc) + (long long)tile * (kKeys * 64);
-        const uint8_t* const scales = ((item & 1) ? vs : ks) + (long long)tile * (kKeys * 8);
+    const int r0 = w * kGroups * 8 + jr;
+    // The loads run ahead of the conversion, across segments: their own walk.
+    int ld_seg = blockIdx.x - gridDim.x, ld_item = 0, ld_items = 0, ld_slot = 0, ld_left = 0;
+    long long ld_row = 0;
+    auto load = [&]() {
+      while (ld_item >= ld_items) {  // the next segment with keys
+        ld_seg += gridDim.x;
+        if (ld_seg >= segs) break;
+        const Seg s = segment(p, ld_seg, kRows);
+        ld_item = 0;
+        ld_items = 2 * s.n;
+        ld_row = (long long)s.bh * p.S_kv + (long long)s.k0 * kKeys + r0;
+        ld_left = s.len - s.k0 * kKeys;  // valid keys from the segment's first on
+      }
+      if (ld_seg < segs) {
+        const bool v = ld_item & 1;
+        const int left = ld_left - (ld_item >> 1) * kKeys;  // ... from this tile's first on
+        const long long row = ld_row + (long long)(ld_item >> 1) * kKeys;
+        const uint8_t* const codes = (v ? p.vc : p.kc) + row * 64 + i * 16;
+        const uint8_t* const scales = (v ? p.vs : p.ks) + row * 8;
         const uint32_t dst = raw0 + ld_slot * kRawBytes + r0 * 64 + i * 16;
         const uint32_t sdst = raw0 + ld_slot * kRawBytes + kKeys * 64 + r0 * 8;
-        const int left = left0 - tile * kKeys;
-        if ((tile + k0 + 1) * kKeys <= len) {
+        if (left >= kKeys) {
 #pragma unroll
           for (int c = 0; c < kGroups; ++c) {
             p4::cp16(dst + c * 512, codes + c * 512);
@@ -305,11 +376,12 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
         } else {  // keys past the length read as zeros
 #pragma unroll
           for (int c = 0; c < kGroups; ++c) {
-            const bool take = 8 * c < left;
+            const bool take = r0 + 8 * c < left;
             p4::cp16_if(dst + c * 512, take ? codes + c * 512 : p.kc, take);
             if (i == 0) p4::cp8_if(sdst + c * 64, take ? scales + c * 64 : p.ks, take);
           }
         }
+        ++ld_item;
       }
       p4::cp_commit();
       ld_slot = ld_slot + 1 == kRaw ? 0 : ld_slot + 1;
@@ -319,10 +391,11 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
 #pragma unroll
     for (int g = 0; g < 2; ++g) put[g] = r0 * 128 + (((4 * g + i) ^ (jr & 7)) << 4);
 #pragma unroll
-    for (int k = 0; k < kRaw - 1; ++k) load(k);
+    for (int k = 0; k < kRaw - 1; ++k) load();
     bool ok = true;
-    int raw = 0;
-    for (int item = 0; item < items; ++item) {
+    int raw = 0, item = 0;
+    for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x)
+    for (int todo = 2 * segment(p, seg, kRows).n; todo > 0; --todo, ++item) {
       const int slot = item % kSlots;
       p4::cp_wait<kRaw - 2>();
       __syncwarp();
@@ -336,9 +409,8 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
         s2[c] = p4::lds8(ssrc + c * 64);
       }
       raw = raw + 1 == kRaw ? 0 : raw + 1;
-      load(item + kRaw - 1);  // into the slot of the item before this one
-      const bool got = mbar_wait(&sm.kv_empty[slot], ((uint32_t)(item / kSlots) & 1u) ^ 1u, abort, p.status,
-                                 ANIMA_ERR_TIMEOUT);
+      load();  // into the slot of the item before this one
+      const bool got = wait(&sm.kv_empty[slot], ((uint32_t)(item / kSlots) & 1u) ^ 1u);
       if (!(ok = __all_sync(0xffffffffu, got))) break;
       const uint32_t dst = smem_u32(sm.kv[slot]);
 #pragma unroll
@@ -372,25 +444,43 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
     const int row = quarter * 32 + lane;
     const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
     const uint32_t tO = tmem + lane_field + 256 + i * 128;
-    const int grow = q0 + i * kBM + row;
-    const float back = stage_q<kBf16>(
-        sm.q[i], row, reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + min(grow, p.S_q - 1)) * kD),
-        grow < p.S_q);
-    const float sl2 = p.scale_log2 * back;
-    fence_proxy_async_smem();
-    mbar_arrive(&sm.q_full);
-
-    float m = -INFINITY, l = 0.f;
+    int a = 0, gg = 0;
     bool ok = true;
+    // The scale of this thread's row of segment round `round`; bf16: once its Q tile is loaded,
+    // converts the row.
+    auto take_q = [&](int round) {
+      if (!kBf16) return p.scale_log2;
+      const bool got = wait(&sm.q_raw[i], (uint32_t)round & 1u);
+      if (!(ok = __all_sync(0xffffffffu, got))) return 0.f;
+      const float back = convert_row(sm.q[i], row);
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.q_conv[i]);
+      return p.scale_log2 * back;
+    };
+    auto more = [&](int seg) {  // whether a segment with keys follows
+      for (seg += gridDim.x; seg < segs; seg += gridDim.x)
+        if (segment(p, seg, kRows).n > 0) return true;
+      return false;
+    };
+    float sl2 = 0.f;
+    bool have_q = false;
+    for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
+    const Seg s = segment(p, seg, kRows);
+    const int n = s.n, grow = s.q0 + i * kBM + row;
+    if (n > 0 && !have_q) {
+      sl2 = take_q(a);
+      if (!ok) break;
+    }
+    float m = -INFINITY, l = 0.f;
     for (int g = 0; g < n; ++g) {
-      const int buf = kNT == 2 ? i : g & 1;  // S and its barriers
+      const int t = gg + g;
+      const int buf = kNT == 2 ? i : t & 1;  // S and its barriers
       const uint32_t tS = tmem + lane_field + buf * 128;
-      const bool got = mbar_wait(&sm.s_full[buf], (uint32_t)(kNT == 2 ? g : g >> 1) & 1u, abort, p.status,
-                                 ANIMA_ERR_TIMEOUT);
+      const bool got = wait(&sm.s_full[buf], (uint32_t)(kNT == 2 ? t : t >> 1) & 1u);
       if (!(ok = __all_sync(0xffffffffu, got))) break;
       tc_fence_after();
       uint32_t r[4][32];
-      const int lim = len - (k0 + g) * kKeys;
+      const int lim = s.len - (s.k0 + g) * kKeys;
       const bool full = lim >= kKeys;
       auto load_s = [&]() {
 #pragma unroll
@@ -470,7 +560,7 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
       l = l * alpha + sum;
       if (__any_sync(0xffffffffu, g > 0 && alpha != 1.f)) {
         if (kNT == 1) {  // the PV before this step may still run (s_full covers it with two tiles)
-          const bool idle = mbar_wait(&sm.pv_done, (uint32_t)(g - 1) & 1u, abort, p.status, ANIMA_ERR_TIMEOUT);
+          const bool idle = wait(&sm.pv_done, (uint32_t)(t - 1) & 1u);
           if (!(ok = __all_sync(0xffffffffu, idle))) break;
           tc_fence_after();
         }
@@ -489,23 +579,25 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
       mbar_arrive(&sm.p_full[buf]);
       m = m_use;
     }
-    if (ok && n > 0) {
-      const bool got = mbar_wait(&sm.o_full[i], 0, abort, p.status, ANIMA_ERR_TIMEOUT);
-      ok = __all_sync(0xffffffffu, got);
+    if (!ok) break;
+    if (n > 0) {
+      // The next segment's Q tile, if any, has been loading since this one's last QK^T.
+      have_q = kBf16 && more(seg);
+      if (have_q) sl2 = take_q(a + 1);
+      const bool got = ok && wait(&sm.o_full[i], (uint32_t)a & 1u);
+      if (!(ok = __all_sync(0xffffffffu, got))) break;
       tc_fence_after();
     }
-    if (ok) {
-      // The query tile's shared memory is free (its last QK^T is done): 4 KB of it per warp stage
-      // the output blocks.
-      float4* const stage = reinterpret_cast<float4*>(sm.q[i]) + quarter * 256;
+    {
+      float4* const stage = sm.stage[warp];
       const int r0 = grow - lane;  // the warp's first row
       const int nvalid = p.S_q - r0;
       const bool direct = p.part == nullptr;
       const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;  // no key: zeros
       const long long urow = i * kBM + quarter * 32;
-      float* const part = direct ? nullptr : p.part + ((long long)slice * p.units + unit) * part_floats(kRows);
+      float* const part = direct ? nullptr : p.part + ((long long)s.slice * p.units + s.unit) * part_floats(kRows);
       char* const out_w = static_cast<char*>(p.out) +
-                          ((long long)b * p.ob + (long long)(bh % p.H) * p.oh + (long long)r0 * p.os) * 2;
+                          ((long long)s.b * p.ob + (long long)(s.bh % p.H) * p.oh + (long long)r0 * p.os) * 2;
 #pragma unroll 1
       for (int c = 0; c < 4 && (direct || n > 0); ++c) {
         float v[32];
@@ -528,6 +620,13 @@ __global__ void __launch_bounds__(kThreads16, 1) kv4_tile_kernel(const Params p)
         part[kRows * kD + urow + lane] = m;
         part[kRows * kD + kRows + urow + lane] = l;
       }
+    }
+    if (n > 0) {
+      tc_fence_before();
+      mbar_arrive(&sm.o_empty[i]);
+      gg += n;
+      ++a;
+    }
     }
   }
   tc_fence_before();
@@ -597,11 +696,12 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
 }
 
 template <bool kBf16, int kNT>
-static int tile_t(const kv4t::Params& p, int grid, cudaStream_t st) {
+static int tile_t(const CUtensorMap& mq, const kv4t::Params& p, int grid, cudaStream_t st) {
   auto kern = kv4t::kv4_tile_kernel<kBf16, kNT>;
+  constexpr size_t smem = kv4t::smem_bytes<kNT>();
   static SmemAttr attr;
-  if (!attr.raise((const void*)kern, kv4t::kSmemBytes)) return ANIMA_ERR_CUDA;
-  kern<<<grid, kv4t::kThreads16, kv4t::kSmemBytes, st>>>(p);
+  if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
+  kern<<<grid, kv4t::kThreads16, smem, st>>>(mq, p);
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 
@@ -609,7 +709,6 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   const bool bf = a->dtype == ANIMA_DTYPE_BF16;
   if (t.units * t.nsplit > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
   kv4t::Params p;
-  p.q = static_cast<const uint16_t*>(a->q);
   p.kc = static_cast<const uint8_t*>(a->k_codes);
   p.ks = static_cast<const uint8_t*>(a->k_scales);
   p.vc = static_cast<const uint8_t*>(a->v_codes);
@@ -628,9 +727,12 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   p.units = (int)t.units;
   p.nsplit = t.nsplit;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  const int grid = (int)t.units * t.nsplit;
-  const int rc = t.nt == 1 ? (bf ? tile_t<true, 1>(p, grid, st) : tile_t<false, 1>(p, grid, st))
-                           : (bf ? tile_t<true, 2>(p, grid, st) : tile_t<false, 2>(p, grid, st));
+  CUtensorMap mq;
+  int rc = attn_head_map(&mq, a->q, a->dtype, a->B * a->H, a->S_q);
+  if (rc != ANIMA_OK) return rc;
+  const int grid = (int)std::min<long long>(t.units * t.nsplit, sm_count);
+  rc = t.nt == 1 ? (bf ? tile_t<true, 1>(mq, p, grid, st) : tile_t<false, 1>(mq, p, grid, st))
+                 : (bf ? tile_t<true, 2>(mq, p, grid, st) : tile_t<false, 2>(mq, p, grid, st));
   if (rc != ANIMA_OK || t.nsplit == 1) return rc;
   const long long total = (long long)a->B * a->H * a->S_q;
   const int mg = (int)std::min<long long>((total + 7) / 8, (long long)sm_count * 8);
