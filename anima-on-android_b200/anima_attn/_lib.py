@@ -121,7 +121,7 @@ SIGNATURES = {
     # (the two structures by address: ctypes.byref of one, or its packed bytes)
     "anima_matvec4": ([_P, _P], ct.c_int),
     "anima_attn_kv4_fwd": ([_P, _P], ct.c_int),
-    "anima_attn_kv4_workspace_size": ([ct.c_int] * 4, ct.c_uint64),
+    "anima_attn_kv4_workspace_size": ([ct.c_int] * 5, ct.c_uint64),
     "anima_attn_device_info": ([ct.POINTER(ct.c_int), ct.POINTER(ct.c_int)], ct.c_int),
     "anima_attn_version": ([], ct.c_char_p),
 }

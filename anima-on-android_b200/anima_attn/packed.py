@@ -73,8 +73,8 @@ def _check_packed(p: Packed4, what: str) -> tuple:
 
 
 @lru_cache(maxsize=1024)
-def _kv4_workspace(dev: int, B: int, H: int, Sq: int, Skv: int) -> int:
-    return int(L.lib.anima_attn_kv4_workspace_size(B, H, Sq, Skv))
+def _kv4_workspace(dev: int, dtype: torch.dtype, B: int, H: int, Sq: int, Skv: int) -> int:
+    return int(L.lib.anima_attn_kv4_workspace_size(_TORCH_DT[dtype], B, H, Sq, Skv))
 
 
 def _row_strides(x: torch.Tensor) -> Optional[list]:
@@ -234,7 +234,7 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")
         flags = L.FLAG_MASK
-    nbytes = _kv4_workspace(q.get_device(), B, H, Sq, Skv)
+    nbytes = _kv4_workspace(q.get_device(), q.dtype, B, H, Sq, Skv)
     # Scratch of this call alone, from the caching allocator: freed on return, its block goes
     # to work enqueued later on this stream, and a captured graph keeps it in its own pool.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None

@@ -1,10 +1,11 @@
 // attn_kv4.cu -- attention over K and V held packed in 4 bits (format: packed4.cuh):
 // out = softmax(q K^T * scale) V per (batch, head), D = 128, key-padding lengths per sample.
 //
-// Few query rows (up to kRowsFew per head): kv4_rows_kernel reads the packed cache directly.
-// Many: the cache is unpacked once to 16 bits (expand_kernel) and the attention core of
-// attn_fwd.cu runs on it; each key tile is then read by every 256-row unit of its head, and
-// unpacking it again in each would cost issue slots that the softmax needs.
+// Three ways, chosen by rows_path and core_path below:
+//   little work: kv4_rows_kernel reads the packed cache directly, eight query rows at a time;
+//   more:        attn_kv4_tile.cu, on the tensor cores, unpacks K and V in the kernel;
+//   very many fp16 rows: the cache is unpacked once to 16 bits (expand_kernel) and the attention core
+//                of attn_fwd.cu runs on it, which spares each 256-row unit unpacking it again.
 //
 // kv4_rows_kernel.  One cluster per (batch, head, block of query rows); its CTAs and their
 // warps take 32-key blocks in turn, each warp with its own running maximum, sum and output, so
@@ -21,8 +22,9 @@
 //                 and small scales do not underflow, as they would in fp16.  movmatrix turns the
 //                 accumulator's layout of P^T into the operand's.
 // At the end the warps' outputs meet in shared memory, then the cluster's CTAs read one
-// another's over distributed shared memory, each writing its share of the output.  No
-// workspace, no atomics; the order of all sums is fixed.
+// another's over distributed shared memory, each writing its share of the output.  Where heads are
+// few and the cache long, several clusters share a unit's keys and write fp32 partials, which
+// kv4_merge_kernel joins.  No atomics; the order of all sums is fixed.
 #include <algorithm>
 
 #include "attn_kv4.cuh"
@@ -51,8 +53,12 @@ struct Params {
   const uint8_t* vs;
   const int* valid;
   void* out;
+  float* part;         // partials, or nullptr: write the output
   long long ob, oh, os;
-  int H, BH, S_q, S_kv;
+  int H, S_q, S_kv;
+  int nqb;             // units (blocks of query rows) per (batch, head)
+  int units;
+  int nsplit;          // clusters that share a unit's keys
   float scale_log2;
 };
 
@@ -76,55 +82,44 @@ __device__ __forceinline__ float ld_cluster(uint32_t a) {
   return v;
 }
 
-// Bytes of the merge area: per warp O [rows][128], m [rows], l [rows]; then the CTA's own.
-__host__ __device__ constexpr int part_floats(int rows) { return rows * kD + 2 * rows; }
-constexpr int rows_of(int nb) { return nb ? 8 * nb : 1; }
-template <int kW, int kNB>
-constexpr size_t smem_bytes(int stages) {
+template <int kW>
+constexpr size_t smem_bytes(int stages, int rows) {
   const size_t ring = (size_t)kW * stages * kStageBytes;
-  const size_t merge = (size_t)(kW + 1) * part_floats(rows_of(kNB)) * sizeof(float);
+  const size_t merge = (size_t)(kW + 1) * kv4_part_floats(rows) * sizeof(float);
   return ring > merge ? ring : merge;
 }
 
-// kBf16: type of q and out (else fp16); kW: warps; kNB: blocks of eight query rows; kNS: stages.
-// kNB = 0 is the form for a single row.  Its row fills all eight columns of Q, so that every
+// kBf16: type of q and out (else fp16); kOne: the form for a single row, else up to eight; kW:
+// warps; kNS: stages.  A single row fills all eight columns of Q, so that every
 // lane has the scores of its keys, and the columns of P are the row's four group-scaled forms, high
 // parts in columns 0 .. 3 and low parts in 4 .. 7: one operand, made once, serves all
 // eight dim tiles, and of a tile of group g columns g and 4 + g count.
-template <bool kBf16, int kW, int kNB_, int kNS>
+template <bool kBf16, bool kOne, int kW, int kNS>
 __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr bool kOne = kNB_ == 0;
-  constexpr int kNB = kOne ? 1 : kNB_;
-  constexpr int kRows = kOne ? 1 : 8 * kNB;
+  constexpr int kRows = kOne ? 1 : 8;
   constexpr int kStep = kOne ? 2 : 1;  // of the four accumulators, those that differ
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = lane >> 2, i = lane & 3;
   uint32_t ncta;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
   const int rank = (int)cluster_rank();
-  const int unit = blockIdx.x / ncta;
-  const int bh = unit % p.BH, row0 = unit / p.BH * kRows;
+  const int cluster = blockIdx.x / ncta;
+  const int slice = cluster / p.units, unit = cluster - slice * p.units;
+  const int bh = unit / p.nqb, row0 = (unit - bh * p.nqb) * kRows;
   const int b = bh / p.H;
   const int len = p.valid ? min(max(__ldg(p.valid + b), 0), p.S_kv) : p.S_kv;
   const int nblk = (len + kKeys - 1) / kKeys;
-  const int step = (int)ncta * kW;
+  const int step = (int)ncta * kW * p.nsplit;
 
   // Query rows as B fragments: word order and pairs match packed4's (group g, lane i).
-  uint32_t qf[kNB][4][4];
+  uint4 qf[4];
+  const int qrow = kOne ? 0 : row0 + j;
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-    const int r = kOne ? 0 : row0 + nb * 8 + j;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < p.S_q)
-        v = __ldg(reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + r) * kD + 32 * g + 8 * i));
-      qf[nb][g][0] = v.x;
-      qf[nb][g][1] = v.y;
-      qf[nb][g][2] = v.z;
-      qf[nb][g][3] = v.w;
-    }
+  for (int g = 0; g < 4; ++g) {
+    qf[g] = make_uint4(0u, 0u, 0u, 0u);
+    if (qrow < p.S_q)
+      qf[g] = __ldg(reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + qrow) * kD + 32 * g + 8 * i));
   }
 
   const uint32_t ring = smem_u32(smem) + warp * kNS * kStageBytes;
@@ -161,18 +156,15 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     }
   };
 
-  float o[kNB][8][4];  // O^T: tile 2 g + h of dims, rows j and j + 8; columns 2 i, 2 i + 1
+  float o[8][4];  // O^T: tile 2 g + h of dims, rows j and j + 8; columns 2 i, 2 i + 1
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb)
+  for (int t = 0; t < 8; ++t)
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[nb][t][c] = 0.f;
-  float m[kNB][2], l[kNB][2];  // of query rows 2 i, 2 i + 1; l: this lane's keys only
-#pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+    for (int c = 0; c < 4; ++c) o[t][c] = 0.f;
+  // of query rows 2 i, 2 i + 1; l: this lane's keys only
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  const int first = rank * kW + warp;
+  const int first = (slice * (int)ncta + rank) * kW + warp;
   int ahead = first;
 #pragma unroll
   for (int s = 0; s < kNS - 1; ++s) {
@@ -193,7 +185,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     const uint32_t st = ring + slot * kStageBytes;
     slot = slot + 1 == kNS ? 0 : slot + 1;
 
-    float sc[2][kNB][4];  // scores of keys 16 u + j (0, 1) and 16 u + j + 8 (2, 3)
+    float sc[2][4];  // scores of keys 16 u + j (0, 1) and 16 u + j + 8 (2, 3)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int k0 = 16 * u + j;
@@ -204,22 +196,17 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
       const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
       const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sc[u][nb][c] = 0.f;
+      for (int c = 0; c < 4; ++c) sc[u][c] = 0.f;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        uint32_t a[4], c[4];
-        p4::numbers<kBf16>(w0[g], a);
-        p4::numbers<kBf16>(w1[g], c);
+        uint32_t x[4], y[4];
+        p4::numbers<kBf16>(w0[g], x);
+        p4::numbers<kBf16>(w1[g], y);
+        float d[4];
+        p4::mma16816_zero<kBf16>(d, x[0], y[0], x[1], y[1], qf[g].x, qf[g].y);
+        p4::mma16816<kBf16>(d, x[2], y[2], x[3], y[3], qf[g].z, qf[g].w);
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          float d[4];
-          p4::mma16816_zero<kBf16>(d, a[0], c[0], a[1], c[1], qf[nb][g][0], qf[nb][g][1]);
-          p4::mma16816<kBf16>(d, a[2], c[2], a[3], c[3], qf[nb][g][2], qf[nb][g][3]);
-#pragma unroll
-          for (int c = 0; c < 4; c += kStep) sc[u][nb][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], sc[u][nb][c]);
-        }
+        for (int c = 0; c < 4; c += kStep) sc[u][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], sc[u][c]);
       }
     }
     // scores in log2 units; keys at or past len are masked
@@ -228,31 +215,27 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 4; c += kStep) {
-          const float v = sc[u][nb][c] * p.scale_log2;
-          sc[u][nb][c] = 16 * u + j + 8 * (c >> 1) < left ? v : -INFINITY;
-          over = over || sc[u][nb][c] > m[nb][c & 1] + kRescale;
-        }
+      for (int c = 0; c < 4; c += kStep) {
+        const float v = sc[u][c] * p.scale_log2;
+        sc[u][c] = 16 * u + j + 8 * (c >> 1) < left ? v : -INFINITY;
+        over = over || sc[u][c] > m[c & 1] + kRescale;
+      }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
+      for (int r = 0; r < (kOne ? 1 : 2); ++r) {
+        float x = fmaxf(fmaxf(sc[0][r], sc[0][r + 2]), fmaxf(sc[1][r], sc[1][r + 2]));
 #pragma unroll
-        for (int r = 0; r < (kOne ? 1 : 2); ++r) {
-          float x = fmaxf(fmaxf(sc[0][nb][r], sc[0][nb][r + 2]), fmaxf(sc[1][nb][r], sc[1][nb][r + 2]));
+        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+        const float mn = fmaxf(m[r], x);
+        const float alpha = m[r] == -INFINITY ? 0.f : ex2_approx(m[r] - mn);
+        m[r] = mn;
+        l[r] *= alpha;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          const float mn = fmaxf(m[nb][r], x);
-          const float alpha = m[nb][r] == -INFINITY ? 0.f : ex2_approx(m[nb][r] - mn);
-          m[nb][r] = mn;
-          l[nb][r] *= alpha;
+        for (int q = 0; q < 8; ++q)
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (kOne || (c & 1) == r) o[nb][q][c] *= alpha;
-        }
+          for (int c = 0; c < 4; ++c)
+            if (kOne || (c & 1) == r) o[q][c] *= alpha;
+      }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -269,14 +252,12 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
       const uint32_t w[4][4] = {{vw[0].x, vw[1].x, vw[2].x, vw[3].x}, {vw[0].y, vw[1].y, vw[2].y, vw[3].y},
                                 {vw[0].z, vw[1].z, vw[2].z, vw[3].z}, {vw[0].w, vw[1].w, vw[2].w, vw[3].w}};
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 4; c += kStep) {
-          const float mu = m[nb][c & 1];
-          const float e = ex2_approx(sc[u][nb][c] - (mu == -INFINITY ? 0.f : mu));
-          sc[u][nb][c] = e;
-          l[nb][c & 1] += e;
-        }
+      for (int c = 0; c < 4; c += kStep) {
+        const float mu = m[c & 1];
+        const float e = ex2_approx(sc[u][c] - (mu == -INFINITY ? 0.f : mu));
+        sc[u][c] = e;
+        l[c & 1] += e;
+      }
       const uint32_t half = (j & 1) ? 0x7632u : 0x5410u;
       float g0[4], g1[4];
       uint32_t one0 = 0, one1 = 0;  // the single row's operand
@@ -285,8 +266,8 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
         const uint32_t h0 = (i & 1) ? s0.y : s0.x, h1 = (i & 1) ? s1.y : s1.x;
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0));
         const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-        const float p0 = sc[u][0][0] * a.x, p1 = sc[u][0][0] * a.y;
-        const float p2 = sc[u][0][2] * c.x, p3 = sc[u][0][2] * c.y;
+        const float p0 = sc[u][0] * a.x, p1 = sc[u][0] * a.y;
+        const float p2 = sc[u][2] * c.x, p3 = sc[u][2] * c.y;
         one0 = pack_bf16x2(p0, p1);
         one1 = pack_bf16x2(p2, p3);
         const uint32_t l0 = pack_bf16x2(p0 - __uint_as_float(one0 << 16), p1 - __uint_as_float(one0 & 0xffff0000u));
@@ -305,21 +286,19 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
         p4::numbers_bf16(__byte_perm(w[g][0], w[g][1], half), x);
         p4::numbers_bf16(__byte_perm(w[g][2], w[g][3], half), y);
         if constexpr (kOne) {
-          p4::mma16816<true>(o[0][2 * g], x[0], x[1], y[0], y[1], one0, one1);
-          p4::mma16816<true>(o[0][2 * g + 1], x[2], x[3], y[2], y[3], one0, one1);
-        } else
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          const float p0 = sc[u][nb][0] * g0[g], p1 = sc[u][nb][1] * g0[g];
-          const float p2 = sc[u][nb][2] * g1[g], p3 = sc[u][nb][3] * g1[g];
+          p4::mma16816<true>(o[2 * g], x[0], x[1], y[0], y[1], one0, one1);
+          p4::mma16816<true>(o[2 * g + 1], x[2], x[3], y[2], y[3], one0, one1);
+        } else {
+          const float p0 = sc[u][0] * g0[g], p1 = sc[u][1] * g0[g];
+          const float p2 = sc[u][2] * g1[g], p3 = sc[u][3] * g1[g];
           const uint32_t h0 = pack_bf16x2(p0, p1), h1 = pack_bf16x2(p2, p3);
           const uint32_t l0 = pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xffff0000u));
           const uint32_t l1 = pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xffff0000u));
           const uint32_t b0 = transpose8(h0), b1 = transpose8(h1), e0 = transpose8(l0), e1 = transpose8(l1);
-          p4::mma16816<true>(o[nb][2 * g], x[0], x[1], y[0], y[1], b0, b1);
-          p4::mma16816<true>(o[nb][2 * g + 1], x[2], x[3], y[2], y[3], b0, b1);
-          p4::mma16816<true>(o[nb][2 * g], x[0], x[1], y[0], y[1], e0, e1);
-          p4::mma16816<true>(o[nb][2 * g + 1], x[2], x[3], y[2], y[3], e0, e1);
+          p4::mma16816<true>(o[2 * g], x[0], x[1], y[0], y[1], b0, b1);
+          p4::mma16816<true>(o[2 * g + 1], x[2], x[3], y[2], y[3], b0, b1);
+          p4::mma16816<true>(o[2 * g], x[0], x[1], y[0], y[1], e0, e1);
+          p4::mma16816<true>(o[2 * g + 1], x[2], x[3], y[2], y[3], e0, e1);
         }
       }
     }
@@ -328,51 +307,37 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   __syncthreads();  // the rings become the merge area
 
   // Per-warp results to shared memory: O [row][dim], m, l.
-  constexpr int kPart = part_floats(kRows);
+  constexpr int kPart = (int)kv4_part_floats(kRows);
   float* const parts = reinterpret_cast<float*>(smem);
   {
     float* const mine = parts + warp * kPart;
-    if constexpr (kOne) {
-      float x = l[0][0];
+#pragma unroll
+    for (int r = 0; r < (kOne ? 1 : 2); ++r) {
+      float x = l[r];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      if (lane == 0) {
-        mine[kD] = m[0][0];
-        mine[kD + 1] = x;
+      const int row = kOne ? 0 : 2 * i + r;
+      if (j == 0 && (!kOne || i == 0)) {
+        mine[kRows * kD + row] = m[r];
+        mine[kRows * kD + kRows + row] = x;
       }
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        // column g in lanes i = g / 2, column 4 + g two lanes on
-        const int g = q >> 1;
-        const float lo = o[0][q][g & 1] + __shfl_xor_sync(0xffffffffu, o[0][q][g & 1], 2);
-        const float hi = o[0][q][(g & 1) + 2] + __shfl_xor_sync(0xffffffffu, o[0][q][(g & 1) + 2], 2);
-        const int d0 = 32 * g + 8 * (j >> 1) + (j & 1) + 4 * (q & 1);
-        if (i == (g >> 1)) {
-          mine[d0] = lo;
-          mine[d0 + 2] = hi;
+        // tile q = 2 g + h: row j is nibble 2 h of the half word, row j + 8 nibble 2 h + 1
+        const int g = q >> 1, d0 = 32 * g + 8 * (j >> 1) + (j & 1) + 4 * (q & 1);
+        if constexpr (kOne) {  // column g is in lanes i = g / 2, column 4 + g two lanes on
+          const float lo = o[q][g & 1] + __shfl_xor_sync(0xffffffffu, o[q][g & 1], 2);
+          const float hi = o[q][(g & 1) + 2] + __shfl_xor_sync(0xffffffffu, o[q][(g & 1) + 2], 2);
+          if (i == (g >> 1)) {
+            mine[d0] = lo;
+            mine[d0 + 2] = hi;
+          }
+        } else {
+          mine[row * kD + d0] = o[q][r];
+          mine[row * kD + d0 + 2] = o[q][r + 2];
         }
       }
-    } else
-#pragma unroll
-    for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = l[nb][r];
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-        const int row = nb * 8 + 2 * i + r;
-        if (j == 0) {
-          mine[kRows * kD + row] = m[nb][r];
-          mine[kRows * kD + kRows + row] = x;
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          // tile q = 2 g + h: row j is nibble 2 h of the half word, row j + 8 nibble 2 h + 1
-          const int d0 = 32 * (q >> 1) + 8 * (j >> 1) + (j & 1) + 4 * (q & 1);
-          mine[row * kD + d0] = o[nb][q][r];
-          mine[row * kD + d0 + 2] = o[nb][q][r + 2];
-        }
-      }
+    }
   }
   __syncthreads();
   float* const own = parts + kW * kPart;
@@ -412,7 +377,14 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
       acc = fmaf(f, ld_cluster(base + e * 4), acc);
       sum = fmaf(f, ld_cluster(base + (kRows * kD + kRows + row) * 4), sum);
     }
-    if (row0 + row < p.S_q) {
+    if (p.part) {
+      float* const part = p.part + ((long long)slice * p.units + unit) * kPart;
+      part[e] = acc;
+      if (e % kD == 0) {
+        part[kRows * kD + row] = mx;
+        part[kRows * kD + kRows + row] = sum;
+      }
+    } else if (row0 + row < p.S_q) {
       const float v = sum == 0.f ? 0.f : acc / sum;  // no valid key: zeros
       const long long at = b * p.ob + (bh % p.H) * p.oh + (long long)(row0 + row) * p.os + e % kD;
       static_cast<uint16_t*>(p.out)[at] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
@@ -423,12 +395,12 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 }
 
 // ---------------------------------------------------------------- many rows: unpack once
-// Packed rows of K (blockIdx.y = 0) and V (1) to the attention core's 16-bit operands; rows at
+// Packed rows of K (blockIdx.y = 0) and V (1) to the attention core's fp16 operands; rows at
 // or past a sample's length are written as zeros, whatever the cache holds there.
-template <bool kBf16>
 __global__ void __launch_bounds__(256)
     expand_kernel(const uint4* kc, const uint2* ks, const uint4* vc, const uint2* vs, uint16_t* ko,
                   uint16_t* vo, const int* valid, int H, int S_kv, long long quads) {
+  grid_dependents_launch();  // the core sets up meanwhile; it waits for this grid before it reads
   const uint4* codes = blockIdx.y ? vc : kc;
   const uint2* scales = blockIdx.y ? vs : ks;
   uint16_t* out = blockIdx.y ? vo : ko;
@@ -457,7 +429,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&n[k]));
-        r[k] = kBf16 ? pack_bf16x2(v.x * sg[g], v.y * sg[g]) : pack_f16x2(v.x * sg[g], v.y * sg[g]);
+        r[k] = pack_f16x2(v.x * sg[g], v.y * sg[g]);
       }
       *reinterpret_cast<uint4*>(at + 32 * g) = make_uint4(r[0], r[1], r[2], r[3]);
     }
@@ -466,18 +438,56 @@ __global__ void __launch_bounds__(256)
 
 }  // namespace kv4
 
-// Query rows per head up to which the packed cache is read directly.
-constexpr int kRowsFew = 16;
-constexpr bool kUseTile = true;
+// Whether the packed cache is read directly.  Up to 16 rows always; beyond, the rows' passes over the
+// cache cost more than the tile kernel's start (some 6 us) once heads x rows x keys exceed 2^20.
+// Measured, us, this way against the tile kernel, heads x rows x keys: 4 x 256 x 512 9.7 / 14.8,
+// 32 x 64 x 512 12.5 / 13.4, 4 x 1024 x 512 19.3 / 17.4, 32 x 64 x 2048 28 / 18, 32 x 16 x 8192 27 / 35.
+static bool rows_path(long long bh, long long S_q, long long S_kv) {
+  return S_q <= 16 || bh * S_q * S_kv <= (1 << 20);
+}
+// Whether K and V are unpacked once for the attention core: fp16 calls of two rounds of 256-row units or
+// more (4096 x 512 at 32 heads 52 us against the tile kernel's 57, 16384 x 512 152 / 184; at one
+// round the two are even).  bf16 rows keep the tile kernel, whose fp16 operands are more exact.
+static bool core_path(const int dtype, long long bh, long long S_q, int sm_count) {
+  return dtype == ANIMA_DTYPE_F16 && bh * ((S_q + 255) / 256) >= 2LL * sm_count;
+}
 
-template <bool kBf16, int kW, int kNB, int kNS>
-static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
-  auto kern = kv4::kv4_rows_kernel<kBf16, kW, kNB, kNS>;
-  constexpr size_t smem = kv4::smem_bytes<kW, kNB>(kNS);
+// How a call on rows_path is cut.
+struct RowsPlan {
+  int rows, nqb;   // query rows per unit, units per (batch, head)
+  long long units;
+  int warps, ncta, nsplit;
+  size_t bytes;
+};
+static RowsPlan rows_plan(long long bh, int S_q, int S_kv, int sm_count) {
+  RowsPlan r;
+  r.rows = S_q > 1 ? 8 : 1;
+  r.nqb = (S_q + r.rows - 1) / r.rows;
+  r.units = bh * r.nqb;
+  // CTAs per cluster: as many as two to an SM have room for, while each of their warps has a block;
+  // eight warps where there are blocks for them.
+  const int nblk = (S_kv + kv4::kKeys - 1) / kv4::kKeys;
+  r.warps = nblk >= 128 ? 8 : 4;
+  const long long room = std::max(1LL, 2LL * sm_count / r.units);
+  r.ncta = (int)std::min<long long>(std::min<long long>((nblk + r.warps - 1) / r.warps, room), 8);
+  // Several clusters where one leaves each warp eight blocks or more and SMs idle, four blocks a
+  // warp at least.
+  r.nsplit = 1;
+  const int per_warp = nblk / (8 * r.warps);
+  if (r.ncta == 8 && per_warp >= 8) r.nsplit = (int)std::max(1LL, std::min<long long>(room / 8, per_warp / 4));
+  r.bytes = r.nsplit > 1 ? (size_t)r.nsplit * r.units * kv4_part_floats(r.rows) * sizeof(float) : 0;
+  return r;
+}
+
+template <bool kBf16, bool kOne, int kW>
+static int rows_t(const kv4::Params& p, int ncta, cudaStream_t st) {
+  constexpr int kStages = 3;
+  auto kern = kv4::kv4_rows_kernel<kBf16, kOne, kW, kStages>;
+  constexpr size_t smem = kv4::smem_bytes<kW>(kStages, kOne ? 1 : 8);
   static SmemAttr attr;
-  if (!attr.raise((const void*)kern, smem, true)) return ANIMA_ERR_CUDA;
+  if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * ncta));
+  cfg.gridDim = dim3((unsigned)(p.units * p.nsplit * ncta));
   cfg.blockDim = dim3(32 * kW);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -490,8 +500,6 @@ static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
     cudaGetLastError();
-    // a device that cannot place a cluster past the portable size takes one within it
-    if (ncta > 8) return rows_t<kBf16, kW, kNB, kNS>(p, units, 8, st);
     return ANIMA_ERR_CUDA;
   }
   return ANIMA_OK;
@@ -499,18 +507,22 @@ static int rows_t(const kv4::Params& p, int units, int ncta, cudaStream_t st) {
 
 static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }
 
-// Bytes of workspace: none for few rows.
-size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv, int sm_count) {
-  if (S_q <= kRowsFew) return 0;
-  if (kUseTile) return kv4_tile_plan(B * H, S_q, S_kv, sm_count).bytes;
-  return 2 * expanded_bytes((long long)B * H, S_kv);
+size_t attn_kv4_workspace_bytes(int dtype, int B, int H, int S_q, int S_kv, int sm_count) {
+  const long long bh = (long long)B * H;
+  if (rows_path(bh, S_q, S_kv)) return rows_plan(bh, S_q, S_kv, sm_count).bytes;
+  if (core_path(dtype, bh, S_q, sm_count)) return 2 * expanded_bytes(bh, S_kv);
+  return kv4_tile_plan((int)bh, S_q, S_kv, sm_count).bytes;
 }
 
 int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st) {
   const long long bh = (long long)a->B * a->H;
   const bool bf = a->dtype == ANIMA_DTYPE_BF16;
   const int* valid = (a->flags & ANIMA_FLAG_MASK) ? a->kv_valid_len : nullptr;
-  if (a->S_q <= kRowsFew) {
+  const size_t need = attn_kv4_workspace_bytes(a->dtype, a->B, a->H, a->S_q, a->S_kv, sm_count);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return ANIMA_ERR_NOMEM;
+  if (rows_path(bh, a->S_q, a->S_kv)) {
+    const RowsPlan r = rows_plan(bh, a->S_q, a->S_kv, sm_count);
+    if (r.units * r.nsplit * r.ncta > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
     kv4::Params p;
     p.q = static_cast<const uint16_t*>(a->q);
     p.kc = static_cast<const uint8_t*>(a->k_codes);
@@ -519,48 +531,35 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     p.vs = static_cast<const uint8_t*>(a->v_scales);
     p.valid = valid;
     p.out = a->out;
+    p.part = r.nsplit > 1 ? static_cast<float*>(a->workspace) : nullptr;
     p.ob = a->out_stride[0];
     p.oh = a->out_stride[1];
     p.os = a->out_stride[2];
     p.H = a->H;
-    p.BH = (int)bh;
     p.S_q = a->S_q;
     p.S_kv = a->S_kv;
+    p.nqb = r.nqb;
+    p.units = (int)r.units;
+    p.nsplit = r.nsplit;
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    const int nb = a->S_q > 8 ? 2 : a->S_q > 1 ? 1 : 0, rows = kv4::rows_of(nb);
-    const long long units = bh * ((a->S_q + rows - 1) / rows);
-    if (units * 16 > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
-    // CTAs per cluster: as many as the SMs hold at once, two to an SM, while each of their warps
-    // has a 32-key block or more; eight warps where there are blocks for them.
-    const int nblk = (a->S_kv + kv4::kKeys - 1) / kv4::kKeys;
-    const bool wide = nblk >= 128;
-    const int warps = wide ? 8 : 4;
-    const int by_work = (nblk + warps - 1) / warps;
-    const int by_room = (int)std::max(1LL, 2LL * sm_count / units);
-    const int ncta = std::min(std::min(by_work, by_room), 8);
-    const int u = (int)units;
-    if (wide) {
-      if (nb == 0) return bf ? rows_t<true, 8, 0, 3>(p, u, ncta, st) : rows_t<false, 8, 0, 3>(p, u, ncta, st);
-      if (nb == 1) return bf ? rows_t<true, 8, 1, 3>(p, u, ncta, st) : rows_t<false, 8, 1, 3>(p, u, ncta, st);
-      return bf ? rows_t<true, 8, 2, 3>(p, u, ncta, st) : rows_t<false, 8, 2, 3>(p, u, ncta, st);
-    }
-    if (nb == 0) return bf ? rows_t<true, 4, 0, 3>(p, u, ncta, st) : rows_t<false, 4, 0, 3>(p, u, ncta, st);
-    if (nb == 1) return bf ? rows_t<true, 4, 1, 3>(p, u, ncta, st) : rows_t<false, 4, 1, 3>(p, u, ncta, st);
-    return bf ? rows_t<true, 4, 2, 3>(p, u, ncta, st) : rows_t<false, 4, 2, 3>(p, u, ncta, st);
+    int rc;
+    if (r.warps == 8)
+      rc = r.rows == 1 ? (bf ? rows_t<true, true, 8>(p, r.ncta, st) : rows_t<false, true, 8>(p, r.ncta, st))
+                       : (bf ? rows_t<true, false, 8>(p, r.ncta, st) : rows_t<false, false, 8>(p, r.ncta, st));
+    else
+      rc = r.rows == 1 ? (bf ? rows_t<true, true, 4>(p, r.ncta, st) : rows_t<false, true, 4>(p, r.ncta, st))
+                       : (bf ? rows_t<true, false, 4>(p, r.ncta, st) : rows_t<false, false, 4>(p, r.ncta, st));
+    if (rc != ANIMA_OK || r.nsplit == 1) return rc;
+    return kv4_merge_launch(a, p.part, r.nqb, r.rows, p.units, r.nsplit, sm_count, st);
   }
-  if (kUseTile) {
-    const Kv4TilePlan t = kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count);
-    if (t.bytes > 0 && (!a->workspace || a->workspace_bytes < t.bytes)) return ANIMA_ERR_NOMEM;
-    return kv4_tile_launch(a, t, status, sm_count, st);
-  }
+  if (!core_path(a->dtype, bh, a->S_q, sm_count))
+    return kv4_tile_launch(a, kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count), status, sm_count, st);
   const size_t side = expanded_bytes(bh, a->S_kv);
-  if (!a->workspace || a->workspace_bytes < 2 * side) return ANIMA_ERR_NOMEM;
   uint16_t* const k16 = static_cast<uint16_t*>(a->workspace);
   uint16_t* const v16 = k16 + side / 2;
   const long long quads = bh * a->S_kv * 4;
   const dim3 grid((unsigned)std::min<long long>((quads + 255) / 256, (long long)sm_count * 8), 2);
-  auto kern = bf ? kv4::expand_kernel<true> : kv4::expand_kernel<false>;
-  kern<<<grid, 256, 0, st>>>(static_cast<const uint4*>(a->k_codes), static_cast<const uint2*>(a->k_scales),
+  kv4::expand_kernel<<<grid, 256, 0, st>>>(static_cast<const uint4*>(a->k_codes), static_cast<const uint2*>(a->k_scales),
                              static_cast<const uint4*>(a->v_codes), static_cast<const uint2*>(a->v_scales),
                              k16, v16, valid, a->H, a->S_kv, quads);
   if (cudaGetLastError() != cudaSuccess) return ANIMA_ERR_CUDA;

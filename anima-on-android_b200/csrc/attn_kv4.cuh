@@ -10,6 +10,10 @@ namespace anima {
 // swizzle (attn_fwd.cu).
 int attn_head_map(CUtensorMap* map, const void* base, int op_dtype, int bh, int rows);
 
+// Floats of a partial result of a unit: O [rows][128], m [rows], l [rows], and padding that keeps the
+// next partial 16-byte aligned.
+__host__ __device__ constexpr long long kv4_part_floats(int rows) { return ((long long)rows * 130 + 3) & ~3ll; }
+
 // A call of many query rows (attn_kv4_tile.cu).
 struct Kv4TilePlan {
   int nt;           // 128-row query tiles per unit
@@ -19,6 +23,9 @@ struct Kv4TilePlan {
   size_t bytes;     // workspace for the slices' partials
 };
 Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count);
+// Joins partials [slice][unit][kv4_part_floats(rows)] into a->out.
+int kv4_merge_launch(const AnimaAttnKv4Args* a, const float* part, int nqb, int rows, int units, int nsplit,
+                     int sm_count, cudaStream_t st);
 int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st);
 
 }  // namespace anima

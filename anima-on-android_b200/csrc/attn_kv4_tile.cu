@@ -39,7 +39,7 @@ namespace kv4t {
 using namespace attn;  // kD, kBM, drain_wait, stage/store_block, pack2
 
 constexpr int kKeys = 128;                  // keys per tile
-constexpr int kRaw = 3;                     // packed tiles in flight
+constexpr int kRaw = 5;                     // stages of packed tiles
 constexpr int kPanel = 128 * 128;           // [128 rows][64 x 16-bit]
 constexpr int kTile = 2 * kPanel;
 constexpr int kRawBytes = kKeys * 64 + kKeys * 8;
@@ -72,7 +72,7 @@ struct Smem {
   uint8_t q[kNT][kTile];
   uint8_t kv[kSlots][kTile];
   uint8_t raw[kRaw][kRawBytes];
-  float4 stage[kNT * 4][256];  // per softmax warp: one 32 x 32 block on its way to global
+  float4 stage[kNT * 4][128];  // per softmax warp: one 32 x 32 16-bit block on its way to global
   uint64_t q_raw[2];           // Q tile as loaded
   uint64_t q_conv[2];          // bf16: converted
   uint64_t q_empty[2];
@@ -110,9 +110,6 @@ __device__ __forceinline__ Seg segment(const Params& p, int seg, int rows) {
   s.n = (int)((long long)tiles * (s.slice + 1) / p.nsplit) - s.k0;
   return s;
 }
-
-// Floats of one slice's partial of a unit: O [rows][128], m [rows], l [rows].
-__host__ __device__ constexpr long long part_floats(int rows) { return (long long)rows * (kD + 2); }
 
 // A thread's bf16 query row of a Q tile to fp16 in place, scaled; returns the factor that undoes it.
 __device__ __forceinline__ float convert_row(uint8_t* tile, int row) {
@@ -595,7 +592,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       const bool direct = p.part == nullptr;
       const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;  // no key: zeros
       const long long urow = i * kBM + quarter * 32;
-      float* const part = direct ? nullptr : p.part + ((long long)s.slice * p.units + s.unit) * part_floats(kRows);
+      float* const part = direct ? nullptr : p.part + ((long long)s.slice * p.units + s.unit) * kv4_part_floats(kRows);
       char* const out_w = static_cast<char*>(p.out) +
                           ((long long)s.b * p.ob + (long long)(s.bh % p.H) * p.oh + (long long)r0 * p.os) * 2;
 #pragma unroll 1
@@ -614,7 +611,10 @@ __global__ void __launch_bounds__(kThreads16, 1)
         if (direct)
           store_block<kBf16 ? ANIMA_DTYPE_BF16 : ANIMA_DTYPE_F16>(out_w, p.os * 2, nvalid, v, c, inv, stage, lane);
         else
-          store_block<ANIMA_DTYPE_F32>(reinterpret_cast<char*>(part + urow * kD), kD * 4, nvalid, v, c, 1.f, stage, lane);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(part + (urow + lane) * kD + c * 32 + 4 * e) =
+                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
       }
       if (!direct) {
         part[kRows * kD + urow + lane] = m;
@@ -638,18 +638,19 @@ __global__ void __launch_bounds__(kThreads16, 1)
 }
 
 // Joins the slices of every query row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, in
-// slice order.  One warp per row, four columns per lane.  part: [slice][unit][part_floats(rows)].
+// slice order.  One warp per row, four columns per lane.  part: [slice][unit][kv4_part_floats(rows)].
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
     kv4_merge_kernel(const float* part, void* out, long long ob, long long oh, long long os, int H, int S_q,
                      int nqb, int rows, int units, int nsplit, long long total) {
   const int lane = threadIdx.x & 31;
-  const long long stride = (long long)units * part_floats(rows);
+  grid_dependency_wait();  // launched while the slices' kernel drains
+  const long long stride = (long long)units * kv4_part_floats(rows);
   for (long long t = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < total;
        t += ((long long)gridDim.x * blockDim.x) >> 5) {
     const int bh = (int)(t / S_q), s = (int)(t - (long long)bh * S_q);
     const int unit = bh * nqb + s / rows, r = s % rows;
-    const float* const base = part + (long long)unit * part_floats(rows);
+    const float* const base = part + (long long)unit * kv4_part_floats(rows);
     const float* const mp = base + (long long)rows * kD + r;
     float M = -INFINITY;
     for (int k = 0; k < nsplit; ++k) M = fmaxf(M, mp[k * stride]);
@@ -689,9 +690,11 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
   t.nqb = (S_q + t.nt * attn::kBM - 1) / (t.nt * attn::kBM);
   t.units = (long long)bh * t.nqb;
   const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
-  // as many slices as the SMs hold in one round, of two key tiles or more
-  t.nsplit = (int)std::max(1LL, std::min({sm_count / std::max(1LL, t.units), tiles / 2, 64LL}));
-  t.bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4t::part_floats(t.nt * attn::kBM)) * 4 : 0;
+  // As many slices as the SMs hold in one round, if that shortens the longest chain of key tiles by
+  // three or more (the merge costs about two).
+  t.nsplit = (int)std::max(1LL, std::min({sm_count / std::max(1LL, t.units), tiles, 64LL}));
+  if (tiles - (tiles + t.nsplit - 1) / t.nsplit < 3) t.nsplit = 1;
+  t.bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4_part_floats(t.nt * attn::kBM)) * 4 : 0;
   return t;
 }
 
@@ -703,6 +706,28 @@ static int tile_t(const CUtensorMap& mq, const kv4t::Params& p, int grid, cudaSt
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
   kern<<<grid, kv4t::kThreads16, smem, st>>>(mq, p);
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+}
+
+int kv4_merge_launch(const AnimaAttnKv4Args* a, const float* part, int nqb, int rows, int units, int nsplit,
+                     int sm_count, cudaStream_t st) {
+  const long long total = (long long)a->B * a->H * a->S_q;
+  auto merge = a->dtype == ANIMA_DTYPE_BF16 ? kv4t::kv4_merge_kernel<true> : kv4t::kv4_merge_kernel<false>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<long long>((total + 7) / 8, (long long)sm_count * 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, merge, part, a->out, (long long)a->out_stride[0], (long long)a->out_stride[1],
+                         (long long)a->out_stride[2], a->H, a->S_q, nqb, rows, units, nsplit, total) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return ANIMA_ERR_CUDA;
+  }
+  return ANIMA_OK;
 }
 
 int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st) {
@@ -734,12 +759,7 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   rc = t.nt == 1 ? (bf ? tile_t<true, 1>(mq, p, grid, st) : tile_t<false, 1>(mq, p, grid, st))
                  : (bf ? tile_t<true, 2>(mq, p, grid, st) : tile_t<false, 2>(mq, p, grid, st));
   if (rc != ANIMA_OK || t.nsplit == 1) return rc;
-  const long long total = (long long)a->B * a->H * a->S_q;
-  const int mg = (int)std::min<long long>((total + 7) / 8, (long long)sm_count * 8);
-  auto merge = bf ? kv4t::kv4_merge_kernel<true> : kv4t::kv4_merge_kernel<false>;
-  merge<<<mg, 256, 0, st>>>(p.part, a->out, p.ob, p.oh, p.os, a->H, a->S_q, t.nqb, t.nt * attn::kBM, p.units,
-                            t.nsplit, total);
-  return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+  return kv4_merge_launch(a, p.part, t.nqb, t.nt * attn::kBM, p.units, t.nsplit, sm_count, st);
 }
 
 }  // namespace anima

@@ -381,7 +381,7 @@ typedef struct AnimaAttnKv4Args {
 } AnimaAttnKv4Args;
 
 int anima_attn_kv4_fwd(const AnimaAttnKv4Args* args, void* stream);
-uint64_t anima_attn_kv4_workspace_size(int B, int H, int S_q, int S_kv);
+uint64_t anima_attn_kv4_workspace_size(int dtype, int B, int H, int S_q, int S_kv);
 
 /* Self-test of the bounded-wait path (no reference counterpart): launches one block
  * whose mbarrier wait can never complete and gives up after timeout_us microseconds

@@ -515,6 +515,48 @@ def test_attention_long_and_wide(Sq, Skv, B, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Sq,Skv,lens", [(1, 20011, [5, 0]), (3, 20011, [20011, 700]), (200, 5000, [0, 130]),
+                                         (200, 5000, [5000, 1]), (100, 5000, [4999, 257])])
+def test_attention_masked_slices(Sq, Skv, lens):
+    """Keys cut into slices, of which masks leave some without a key."""
+    check_attention(2, 1, Sq, Skv, F16, lens=lens)
+    check_attention(2, 1, Sq, Skv, BF16, lens=lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,H,Sq,Skv,lens", [(2, 16, 2307, 133, None), (3, 13, 2049, 130, [0, 130, 40]), (5, 40, 100, 300, [300, 0, 1, 0, 128])])
+def test_attention_many_units(dtype, B, H, Sq, Skv, lens):
+    """More units than SMs: the persistent grid of the tile kernel, and the unpacked core for fp16."""
+    check_attention(B, H, Sq, Skv, dtype, lens=lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [64, 300])
+def test_attention_rows_of_any_size(Sq):
+    """bf16 query rows whose magnitudes differ by far, a zero row, and a row past fp16's range."""
+    g = torch.Generator().manual_seed(12)
+    q = torch.randn(2, Sq, 128, generator=g)
+    q[0, 1] *= 1e-30
+    q[0, 2] *= 1e6
+    q[0, 3] = 0
+    q[1, 5, 7] = 1e8
+    q[1, 6, :64] *= 1e-6
+    q = q.to(BF16).cuda()
+    k, kv = random_packed((2, 4200, 128), 1)  # beyond the direct form's work for both Sq
+    v, vv = random_packed((2, 4200, 128), 2)
+    got = anima_attn.attention_core_kv4(q, k, v, 1, 2)
+    out, pv, top = attention_ref(q.double().cpu().numpy(), kv, vv, 1, 2, None, 1 / math.sqrt(128))
+    tol = attention_bound(out, pv, top, F16, False) + np.abs(out) * half_step(BF16)
+    # Where a row's scores are so large that their own bound passes 1, the largest keys may trade
+    # places: those rows are only checked to be an average of values.
+    far = (half_step(F16) * top > 1).squeeze(-1)
+    err = np.abs(got.double().cpu().numpy() - out)
+    assert (err[~far] <= tol[~far]).all(), float((err / tol)[~far].max())
+    assert np.abs(got.float().cpu().numpy()[far]).max() <= np.abs(vv).max() * 1.01 and far.sum() == 2
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("Sq", [1, 100])
 def test_attention_sharp_and_flat(Sq):
     """Scores spread over hundreds (one key takes all) and nearly alike."""
