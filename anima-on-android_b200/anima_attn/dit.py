@@ -210,12 +210,17 @@ class AnimaDiT:
     one-element all-reduce orders the ranks, instead of an NCCL all-gather.  The buffers are
     allocated by a collective call on the first step (every rank, before graph capture);
     ``close()`` releases the peer mappings (every rank, before the process group goes).
+    ``adaln_bits``: 16, or 4 to hold the blocks' adaLN-LoRA modulation weights packed (CUDA;
+    4.5 bits a value: 352 MB of the full model become 99 MB).  They are read whole once per
+    step by one row per sample, so their products (matvec4) are bound by that read.
     """
 
     def __init__(self, cfg: DiTConfig, weights: Dict[str, torch.Tensor], rank: int = 0,
                  world: int = 1, group=None, attn_fn: Optional[AttnFn] = None,
                  shard: str = "tokens", fused_qkv: bool = True, peer_gather: bool = True,
-                 peer_a2a: bool = True):
+                 peer_a2a: bool = True, adaln_bits: int = 16):
+        if adaln_bits not in (16, 4):
+            raise ValueError("adaln_bits must be 16 or 4")
         if cfg.heads % world:
             raise ValueError("heads must divide evenly over ranks")
         if shard not in ("tokens", "heads"):
@@ -272,6 +277,13 @@ class AnimaDiT:
             for i, (n1, n2) in enumerate(mnames):
                 self.w[n1], self.w[n2] = w1[i * lr:(i + 1) * lr], w2[i]
             self._mod_w = (w1, w2)
+        if adaln_bits == 4:
+            if self._mod_w is None:
+                raise ValueError("adaln_bits=4 needs every block's modulation weights on CUDA")
+            from .packed import quantize4
+            self._mod_w = tuple(quantize4(t) for t in self._mod_w)
+            for n1, n2 in mnames:  # the views of the 16-bit stacks, which go with them
+                del self.w[n1], self.w[n2]
         from .ops import attention as _lib_attention
         if attn_fn is None:
             attn_fn = _lib_attention
@@ -339,9 +351,18 @@ class AnimaDiT:
     def _all_mods(self, emb, lora):
         """Every block's adaLN-LoRA modulation at once, [blocks * 3, B, 3 * hidden] fp32 in
         (block, sub-block) order: the same operand rounding as _mods (16-bit SiLU(emb) and
-        hidden layer, fp32 accumulation), one GEMM and one batched GEMM."""
+        hidden layer, fp32 accumulation), one GEMM and one batched GEMM.  Packed weights
+        (adaln_bits=4): two matvec4 calls, SiLU and the addend in them, the hidden layer in
+        fp32."""
         w1, w2 = self._mod_w
-        dt, B = w1.dtype, emb.shape[0]
+        B = emb.shape[0]
+        if isinstance(w1, tuple):
+            from .packed import matvec4
+            with _region("gemm"):
+                h = matvec4(emb.reshape(B, -1).float(), w1, silu=True)
+                x = h.view(B, w2.shape[0], -1).transpose(0, 1)  # [84, B, Lr]
+                return matvec4(x, w2, add=lora.reshape(B, -1).float())
+        dt = w1.dtype
         with _region("gemm"):
             h = torch.mm(F.silu(emb).reshape(B, -1).to(dt), w1.t(), out_dtype=torch.float32)
             h = h.view(B, w2.shape[0], -1).transpose(0, 1).to(dt)  # [84, B, Lr]
@@ -566,7 +587,7 @@ class AnimaDiT:
         entry = None
         if ctx is not None and self._fused(x):
             entry = ctx if isinstance(ctx, dict) else self._context_entry(p, ctx, True)
-        if self._fused(x) and (ctx is None or "kh" in entry):
+        if self._fused(x) and (ctx is None or "kh" in entry or "k4" in entry):
             from .ops import attention_core, qkv_projection
             x16 = x.to(dt).contiguous()
             qw = self._norm32(p + ".q_norm.weight")
@@ -578,7 +599,12 @@ class AnimaDiT:
                 else:
                     qh, _, _ = qkv_projection(x16, self.w[p + ".q_proj.weight"], hl, 1, 0, qw,
                                               None, None, cfg.eps, True, False)
-                    kh, vh = entry["kh"], entry["vh"]
+                    kh, vh = entry.get("kh"), entry.get("vh")
+            if ctx is not None and "k4" in entry:  # packed K/V (context_cache(kv_bits=4))
+                from .packed import attention_core_kv4
+                with _region("attention"):
+                    o = attention_core_kv4(qh, entry["k4"], entry["v4"], B, hl)
+                return self._gather_oproj(o, self.w[p + ".output_proj.weight"])
             if self.peer_gather and x.is_cuda:
                 g = self._gather_buffers(B, S, x.device)
                 i = 0 if ctx is None else 1  # self- and cross-attention alternate buffers
@@ -613,11 +639,11 @@ class AnimaDiT:
             with _region("attention"):
                 return self.attn_fn(q, k, v, qw, kw, freqs, eps=cfg.eps, out_dtype=dt, op_dtype=dt)
         entry = ctx if isinstance(ctx, dict) else self._context_entry(p, ctx)
-        if "kh" in entry:  # operands already in the attention core's layout (GPU)
+        if "kh" in entry or "k4" in entry:  # operands in the attention core's layout (GPU)
             from .ops import attention_cached_kv
+            kh, vh = (entry["k4"], entry["v4"]) if "k4" in entry else (entry["kh"], entry["vh"])
             with _region("attention"):
-                return attention_cached_kv(q, entry["kh"], entry["vh"], qw, eps=cfg.eps,
-                                           out_dtype=dt)
+                return attention_cached_kv(q, kh, vh, qw, eps=cfg.eps, out_dtype=dt)
         with _region("attention"):
             return self.attn_fn(q, entry["k"], entry["v"], qw, kw, None, eps=cfg.eps,
                                 out_dtype=dt, op_dtype=dt)
@@ -647,7 +673,8 @@ class AnimaDiT:
             entry = {"kh": kh, "vh": vh}
         return entry
 
-    def context_cache(self, ctx_cond: torch.Tensor, ctx_uncond: torch.Tensor) -> Dict[str, dict]:
+    def context_cache(self, ctx_cond: torch.Tensor, ctx_uncond: torch.Tensor,
+                      kv_bits: int = 16) -> Dict[str, dict]:
         """Cross-attention K/V of every block for the CFG pair's contexts (stacked [uncond,
         cond], the order euler_cfg_step uses).  The text context is the same in every step of
         a sampling run (anima_rt/scripts/sampling.py:127), while the reference projects and
@@ -656,8 +683,17 @@ class AnimaDiT:
         from .ops import attention as _lib_attention
         ctx = torch.cat([ctx_uncond, ctx_cond], dim=0).float()
         keep = ctx.is_cuda and self.attn_fn is _lib_attention
-        return {f"blocks.{b}.cross_attn": self._context_entry(f"blocks.{b}.cross_attn", ctx, keep)
-                for b in range(self.cfg.blocks)}
+        if kv_bits not in (16, 4) or (kv_bits == 4 and not keep):
+            raise ValueError("kv_bits must be 16, or 4 with the library attention on CUDA")
+        cache = {}
+        for b in range(self.cfg.blocks):
+            p = f"blocks.{b}.cross_attn"
+            entry = self._context_entry(p, ctx, keep)
+            if kv_bits == 4:
+                from .packed import quantize4
+                entry = {"k4": quantize4(entry["kh"]), "v4": quantize4(entry["vh"])}
+            cache[p] = entry
+        return cache
 
     def _block(self, b: int, x, pending, emb, lora, ctx, freqs):
         """One block on the whole residual stream [B, L, D]; pending as in _block_rows."""

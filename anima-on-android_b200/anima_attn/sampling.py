@@ -39,19 +39,22 @@ def seeded_noise(seed: int, H: int, W: int, channels: int = 16) -> np.ndarray:
 class EulerCFGSampler:
     """EulerSampler.sample for an AnimaDiT: latent [1, C, H, W] and both contexts [1, N,
     ctx_dim] on the model's device.  ``cfg_scale`` is fixed per sampler (as in a captured
-    graph).  On N ranks every rank builds and runs its sampler in the same order (the
+    graph).  ``kv_bits`` 4 keeps the context's K/V packed (AnimaDiT.context_cache).  On N ranks
+    every rank builds and runs its sampler in the same order (the
     collectives are captured), and drops it before the process group is destroyed."""
 
     def __init__(self, model, ctx_cond: torch.Tensor, ctx_uncond: torch.Tensor, cfg_scale: float,
                  latent_shape, graph: bool = True, cache_context: bool = True,
-                 warmup: int = 2):
-        self.model, self.cfg_scale = model, float(cfg_scale)
+                 warmup: int = 2, kv_bits: int = 16):
+        if kv_bits != 16 and not cache_context:
+            raise ValueError("kv_bits applies to the cached context")
+        self.model, self.cfg_scale, self.kv_bits = model, float(cfg_scale), kv_bits
         dev = ctx_cond.device
         self.cc, self.cu = ctx_cond.clone(), ctx_uncond.clone()
         self.x = torch.zeros(latent_shape, device=dev, dtype=torch.float32)
         self.sig = torch.zeros(1, device=dev, dtype=torch.float32)
         self.sig_next = torch.zeros(1, device=dev, dtype=torch.float32)
-        self.cache = model.context_cache(self.cc, self.cu) if cache_context else None
+        self.cache = model.context_cache(self.cc, self.cu, kv_bits) if cache_context else None
         self.graph = self.ctx_graph = None
         if graph:
             if not self.x.is_cuda:
@@ -74,7 +77,7 @@ class EulerCFGSampler:
                     self._fill_cache()
 
     def _fill_cache(self):
-        fresh = self.model.context_cache(self.cc, self.cu)
+        fresh = self.model.context_cache(self.cc, self.cu, self.kv_bits)
         for key, entry in fresh.items():
             for name, t in entry.items():
                 self.cache[key][name].copy_(t)
@@ -111,10 +114,11 @@ class EulerCFGSampler:
 def run_ksampler(model, ctx_cond: torch.Tensor, ctx_uncond: torch.Tensor, H: int, W: int,
                  steps: int = 3, cfg: float = 5.0, seed: int = 6666, denoise: float = 1.0,
                  shift: float = 3.0, graph: bool = True,
-                 sampler: Optional[EulerCFGSampler] = None) -> torch.Tensor:
+                 sampler: Optional[EulerCFGSampler] = None, kv_bits: int = 16) -> torch.Tensor:
     """run_ksampler (sampling.py:183-209) with the z_image schedule and the Euler sampler:
     seeded noise, the sigma schedule, then the loop.  Returns [1, 16, H, W] fp32."""
     dev = ctx_cond.device
     noise = torch.from_numpy(seeded_noise(seed, H, W)).to(dev)
-    s = sampler or EulerCFGSampler(model, ctx_cond, ctx_uncond, cfg, noise.shape, graph=graph)
+    s = sampler or EulerCFGSampler(model, ctx_cond, ctx_uncond, cfg, noise.shape, graph=graph,
+                                   kv_bits=kv_bits)
     return s.sample(noise, z_image_sigmas(steps, denoise, shift)).clone()
