@@ -112,13 +112,20 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
         _check_packed(out, "out")
         if out.codes.shape != lead + (K // 2,):
             raise ValueError("out must be packed with x's shape")
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return out
-    axes = _row_strides(x)
-    if x.stride(-1) != 1 or axes is None or any(s % 8 for _, s in axes) or x.data_ptr() % 16:
-        raise ValueError("x needs a contiguous last axis, row strides that are multiples of 8 and at "
-                         "most three of them, and 16-byte alignment")
-    (n0, s0), (n1, s1), (n2, s2) = axes
+    n0 = n1 = 1
+    s0 = s1 = 0
+    if x.is_contiguous():
+        n2, s2 = n // K, K
+    else:
+        axes = _row_strides(x)
+        if x.stride(-1) != 1 or axes is None or any(s % 8 for _, s in axes):
+            raise ValueError("x needs a contiguous last axis and at most three row strides, all multiples of 8")
+        (n0, s0), (n1, s1), (n2, s2) = axes
+    if x.data_ptr() % 16:
+        raise ValueError("x must be 16-byte aligned")
     L.check(L.lib.anima_quantize4(x.data_ptr(), _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K,
                                   out.codes.data_ptr(), out.scales.data_ptr(), stream),
             "anima_quantize4")
