@@ -179,19 +179,26 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------- matrix-vector products
 // y[e, m, n] = sum_k f(x[e, m, k]) W[e, n, k] + add[e, m, n], f the identity or SiLU.
 //
-// Sixteen rows of W are the A operand of m16n8k16 and the rows x its eight columns, so up to
-// eight columns cost what one does.  The products are of whole numbers n (packed4.cuh) and 16-bit
-// x, exact; a group's partial sum is taken from a zeroed accumulator and multiplied by the group's
-// scale in fp32.  fp32 rows (and SiLU's results) become three bf16 columns each, x = x0 + x1 + x2
-// with x1 and x2 the rounded remainders: 24 bits together, so nothing of x is lost, and the three
-// column sums are added at the end.
+// Sixteen rows of W are the A operand of an MMA and the rows x its columns, so eight columns
+// cost what one does, and every product is of whole numbers and exact (packed4.cuh); a group's sum
+// is multiplied by the group's scale in fp32.
+//
+// 16-bit rows (kF16, kBf16) are a column each of m16n8k16, codes unpacked to n in their type.
+//
+// fp32 rows and SiLU's results (kDigits) are four columns each of the whole-number MMA m16n8k32.  Per
+// group of 32, x is scaled by the power of two that takes the largest below 2^30, rounded to a whole
+// number and written in four signed base-256 digits, so nothing above 2^-31 of the group's largest
+// magnitude is lost, more than an fp32 sum keeps.  A word's codes are its bytes' halves, c = n + 8, three
+// instructions for eight where bf16 takes eleven; the 8 goes into the accumulator's start value, -8
+// sum(digits), together with the 1.5 * 2^23 that makes the whole sum an fp32's low bits.  (As three
+// bf16 columns a row, 84 x 6144 x 256 with two rows took 24 us, bound by unpacking.)
 //
 // A CTA of 8 warps works on one matrix, on a run of tiles of 16 rows of W; `split` warps share a
 // tile, taking its 128-value blocks in turn, and their sums meet in shared memory in a fixed
 // order.  A warp streams its blocks (1 KB of codes, 128 bytes of scales) through a private ring
 // of cp.async stages that runs on across tiles; each lane fetches the codes that it will read
-// itself.  The columns are staged in shared memory once, rows 64 bytes past a multiple of 256 so
-// that the quads of two columns fill the 128 bytes of a wavefront.
+// itself.  The columns are staged in shared memory once, with a row stride that spreads the columns
+// that a wavefront reads over all banks.
 struct Mv4Params {
   const void* x;
   const uint8_t* codes;
@@ -201,8 +208,8 @@ struct Mv4Params {
   long long xe, xm, ae, am, oe, om;
   int N, K, M;
   int parts;             // CTAs per matrix
-  int groups;            // tile groups of one matrix (8 / split tiles each)
-  int split;             // warps per tile
+  int g_each, g_more;    // tile groups (8 / split tiles) of a CTA; the first g_more have one more
+  int log_split;         // log2 of the warps per tile
   int silu, x_dtype, out_dtype;
 };
 
@@ -216,25 +223,111 @@ __device__ __forceinline__ float load_x(const Mv4Params& p, long long at) {
                                        : __half2float(__ushort_as_half(u));
 }
 
-// kParts: columns per row of x (3: bf16 parts of an fp32 value, which take columns 4 m .. 4 m + 2,
-// so that a row's sum needs one exchange between neighbour lanes; 1: the 16-bit value itself);
-// kNB: blocks of eight columns; kStages: ring stages (4; 3 for rows so long that their columns
-// need the room).  Columns without a row repeat another one's data: columns do not mix.
-template <bool kBf16, int kParts, int kNB, int kStages>
+enum { kF16 = 0, kBf16 = 1, kDigits = 2 };
+
+// Bytes between staged columns, and of all staged data.
+template <int kMode>
+__host__ __device__ constexpr int mv4_stride(int K) {
+  return kMode == kDigits ? K + 32 : 2 * K + 64;
+}
+template <int kMode>
+__host__ __device__ constexpr size_t mv4_staged(int M, int K, int nb) {
+  return kMode == kDigits ? (size_t)4 * M * mv4_stride<kMode>(K) + (size_t)(K / 32) * nb * 72
+                          : (size_t)M * mv4_stride<kMode>(K);
+}
+
+// Eight values of x, SiLU applied if asked for.
+__device__ __forceinline__ void load_x8(const Mv4Params& p, long long at, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = load_x(p, at + k);
+  if (p.silu)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = __fdividef(v[k], 1.0f + expf(-v[k]));
+}
+
+// Stages the rows of x as digits.  A lane takes 8 values; the four lanes of a group share its
+// exponent.  cols: digit q of value e at [4 m + q][32 g + 8 i + place of e], in the order in which the
+// code words' halves come (values 0 4 1 5, then 2 6 3 7).  start[g][pair of columns]: the start values of
+// a lane's four accumulators; xscale[g][m]: the group's scale 2^(E - 6), E with largest magnitude
+// below 2^E.
+__device__ __forceinline__ void stage_digits(const Mv4Params& p, int e, int nb, uint8_t* cols, uint4* start,
+                                             float* xscale) {
+  const int stride = mv4_stride<kDigits>(p.K), runs = p.K / 8;
+  for (int c = threadIdx.x; c < p.M * runs; c += kMvThreads) {
+    const uint32_t mask = __activemask();  // K / 8 is a multiple of 16: a group's lanes stay together
+    const int m = c / runs, r = c - m * runs;
+    float v[8];
+    load_x8(p, (long long)e * p.xe + (long long)m * p.xm + 8 * r, v);
+    uint32_t top = 0;
+    int odd = 0;  // values that are infinite, or 2 for a NaN
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t b = __float_as_uint(v[k]) & 0x7fffffffu;
+      top = max(top, b);
+      odd += b == 0x7f800000u ? 1 : b > 0x7f800000u ? 2 : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      top = max(top, __shfl_xor_sync(mask, top, o));
+      odd += __shfl_xor_sync(mask, odd, o);
+    }
+    const int E = max((int)(top >> 23), 1) - 126;
+    uint32_t t[8];
+    float scale;
+    if (odd == 0) {
+      const int s0 = (30 - E) / 2, s1 = 30 - E - s0;  // in two steps: neither leaves fp32
+      const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)  // the signed digits as bytes: add 128 to the lower three, then flip
+        t[k] = ((uint32_t)__float2int_rn(v[k] * f0 * f1) + 0x00808080u) ^ 0x00808080u;
+      scale = E - 6 >= -126 ? __int_as_float((E - 6 + 127) << 23) : __int_as_float(1 << (E - 6 + 149));
+    } else {
+      // one infinity makes its products infinite or NaN and hides the rest; anything else is NaN
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        t[k] = isinf(v[k]) ? (v[k] > 0.f ? 0x01010101u : 0xffffffffu) : 0u;
+      scale = odd == 1 ? INFINITY : NAN;
+    }
+    uint32_t sum[4];
+    const int g = r >> 2, i = r & 3;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // digit q is byte 3 - q
+      const uint32_t sel = (uint32_t)(3 - q) | (uint32_t)(7 - q) << 4;
+      const uint32_t lo = __byte_perm(__byte_perm(t[0], t[4], sel), __byte_perm(t[1], t[5], sel), 0x5410);
+      const uint32_t hi = __byte_perm(__byte_perm(t[2], t[6], sel), __byte_perm(t[3], t[7], sel), 0x5410);
+      *reinterpret_cast<uint2*>(cols + (size_t)(4 * m + q) * stride + 32 * g + 8 * i) = make_uint2(lo, hi);
+      int s = __dp4a((int)lo, 0x01010101, __dp4a((int)hi, 0x01010101, 0));
+      s += __shfl_xor_sync(mask, s, 1);
+      s += __shfl_xor_sync(mask, s, 2);
+      sum[q] = 0x4b400000u - 8u * (uint32_t)s;
+    }
+    if (i < 2)  // pair 2 m: digits 0 and 1; pair 2 m + 1: digits 2 and 3
+      start[g * 4 * nb + 2 * m + i] = i ? make_uint4(sum[2], sum[3], sum[2], sum[3]) : make_uint4(sum[0], sum[1], sum[0], sum[1]);
+    if (i == 2) xscale[g * 2 * nb + m] = scale;
+  }
+}
+
+// kNB: blocks of eight columns (two fp32 rows or eight 16-bit ones); kStages: ring stages (4; 2 for rows
+// so long that their columns need the room).  Columns without a row repeat another one's data:
+// columns do not mix.
+template <int kMode, int kNB, int kStages>
 __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kOuts = kParts == 3 ? 1 : 4;  // results of a lane per block of columns
+  constexpr bool kDig = kMode == kDigits;
+  constexpr int kOuts = kDig ? 1 : 4;  // results of a lane per block of columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = lane >> 2, i = lane & 3;
-  const int stride = p.K + 32;  // elements between staged columns
+  const int stride = mv4_stride<kMode>(p.K);
   const uint32_t ring = smem_u32(smem) + warp * kStages * kMvStage;
   float* const red = reinterpret_cast<float*>(smem + 8 * kStages * kMvStage);
-  uint16_t* const xs = reinterpret_cast<uint16_t*>(red + 8 * 32 * kNB * kOuts);
-  const int s = warp % p.split, t = warp / p.split, tiles = 8 / p.split;
+  uint8_t* const cols = reinterpret_cast<uint8_t*>(red + 8 * 32 * kNB * kOuts);
+  uint4* const start = reinterpret_cast<uint4*>(cols + (size_t)4 * p.M * stride);  // kDigits
+  float* const xscale = reinterpret_cast<float*>(start + (p.K / 32) * 4 * kNB);
+  const int split = 1 << p.log_split;
+  const int s = warp & (split - 1), t = warp >> p.log_split, tiles = 8 >> p.log_split;
   const int blocks = p.K / p4::kBlock;
   const int e = blockIdx.x / p.parts, part = blockIdx.x - e * p.parts;
-  const int g_lo = (int)((long long)p.groups * part / p.parts);
-  const int g_hi = (int)((long long)p.groups * (part + 1) / p.parts);
+  const int g_lo = part * p.g_each + min(part, p.g_more), g_hi = g_lo + p.g_each + (part < p.g_more ? 1 : 0);
 
   // The block sequence of this warp: (group, block) with block = s, s + split, ...  A lane
   // fetches its 16 bytes of rows j and j + 8, lanes i = 0, 1 their scales.  Rows past the
@@ -245,12 +338,12 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
   int ld_g = g_lo, ld_blk = s;
   uint32_t ld_at = ring;
   const int tile_rows = 16 * tiles;  // from a warp's tile to its next
-  const long long c_next = (long long)tile_rows * (p.K / 2) - (long long)((blocks - s - 1) / p.split + 1) * p.split * 64;
-  const long long s_next = (long long)tile_rows * (p.K / 16) - (long long)((blocks - s - 1) / p.split + 1) * p.split * 8;
+  const int rounds = ((blocks - s - 1) >> p.log_split) + 1;
+  const long long c_next = (long long)tile_rows * (p.K / 2) - (long long)rounds * split * 64;
+  const long long s_next = (long long)tile_rows * (p.K / 16) - (long long)rounds * split * 8;
   int ld_n = (g_lo * tiles + t) * 16;  // first row of the tile being fetched
   auto tile_start = [&]() {
-    const int n = ld_n + j;
-    const int n0 = min(n, p.N - 1), n1 = min(n + 8, p.N - 1);
+    const int n0 = min(ld_n + j, p.N - 1), n1 = min(ld_n + j + 8, p.N - 1);
     c0 = codes + (long long)n0 * (p.K / 2) + s * 64;
     c1 = codes + (long long)n1 * (p.K / 2) + s * 64;
     sp = scales + (long long)(i == 0 ? n0 : n1) * (p.K / 16) + s * 8;
@@ -260,10 +353,10 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
       p4::cp16(ld_at + lane * 16, c0);
       p4::cp16(ld_at + 512 + lane * 16, c1);
       if (i < 2) p4::cp8(ld_at + 1024 + (i * 8 + j) * 8, sp);
-      c0 += p.split * 64;
-      c1 += p.split * 64;
-      sp += p.split * 8;
-      ld_blk += p.split;
+      c0 += split * 64;
+      c1 += split * 64;
+      sp += split * 8;
+      ld_blk += split;
       if (ld_blk >= blocks) {
         ld_blk = s;
         ++ld_g;
@@ -284,42 +377,29 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
 #pragma unroll
   for (int k = 0; k < kStages - 1; ++k) fetch();
 
-  for (int m = 0; m < p.M; ++m) {
-    const long long from = (long long)e * p.xe + (long long)m * p.xm;
-    uint16_t* const to = xs + m * kParts * stride;
+  if constexpr (kDig) {
+    stage_digits(p, e, kNB, cols, start, xscale);
+  } else {  // 16-bit rows as they are
+    for (int m = 0; m < p.M; ++m) {
+      const uint16_t* const x = static_cast<const uint16_t*>(p.x) + (long long)e * p.xe + (long long)m * p.xm;
+      uint16_t* const to = reinterpret_cast<uint16_t*>(cols + (size_t)m * stride);
 #pragma unroll 4
-    for (int k = 2 * threadIdx.x; k < p.K; k += 2 * kMvThreads) {
-      float v0 = load_x(p, from + k), v1 = load_x(p, from + k + 1);
-      if (p.silu) {
-        v0 = __fdividef(v0, 1.0f + expf(-v0));
-        v1 = __fdividef(v1, 1.0f + expf(-v1));
-      }
-      if (kParts == 1) {
-        *reinterpret_cast<uint32_t*>(to + k) = kBf16 ? pack_bf16x2(v0, v1) : pack_f16x2(v0, v1);
-      } else {
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) {
-          const uint32_t b = pack_bf16x2(v0, v1);
-          *reinterpret_cast<uint32_t*>(to + q * stride + k) = b;
-          const float f0 = __uint_as_float(b << 16), f1 = __uint_as_float(b & 0xffff0000u);
-          v0 = isinf(f0) ? 0.f : v0 - f0;
-          v1 = isinf(f1) ? 0.f : v1 - f1;
-        }
-      }
+      for (int k = threadIdx.x; k < p.K; k += kMvThreads) to[k] = __ldg(x + k);
     }
   }
   uint32_t xa[kNB];  // this lane's column of x, at its eight values of a group
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
-    const int col = kParts == 3 ? min(nb * 2 + (j >> 2), p.M - 1) * 3 + min(j & 3, 2) : min(nb * 8 + j, p.M - 1);
-    xa[nb] = smem_u32(xs + col * stride + 8 * i);
+    const int col = kDig ? 4 * min(nb * 2 + (j >> 2), p.M - 1) + (j & 3) : min(nb * 8 + j, p.M - 1);
+    xa[nb] = smem_u32(cols) + col * stride + (kDig ? 8 : 16) * i;
   }
+  const uint32_t sa = smem_u32(start) + 16 * i, fa = smem_u32(xscale) + 4 * (i >> 1);
   __syncthreads();
 
   // Result r of this lane for column block nb is row `row + out_row(r)`, row m = out_m(nb, r) of x.
-  auto out_row = [&](int r) { return kParts == 3 ? 0 : 8 * (r >> 1); };
-  auto out_m = [&](int nb, int r) { return kParts == 3 ? nb * 2 + (i >> 1) : nb * 8 + 2 * i + (r & 1); };
-  int row = (g_lo * tiles + t) * 16 + j + (kParts == 3 ? 8 * (i & 1) : 0);
+  auto out_row = [&](int r) { return kDig ? 0 : 8 * (r >> 1); };
+  auto out_m = [&](int nb, int r) { return kDig ? nb * 2 + (i >> 1) : nb * 8 + 2 * i + (r & 1); };
+  int row = (g_lo * tiles + t) * 16 + j + (kDig ? 8 * (i & 1) : 0);
   long long out_at[kNB], add_at[kNB];
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
@@ -343,7 +423,10 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
     for (int b = 0; b < kNB; ++b)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[b][c] = 0.f;
-    for (int blk = s; blk < blocks; blk += p.split) {
+    uint64_t acc2[kNB][2];  // kDigits: the same as pairs
+#pragma unroll
+    for (int b = 0; b < kNB; ++b) acc2[b][0] = acc2[b][1] = 0ull;
+    for (int blk = s; blk < blocks; blk += split) {
       p4::cp_wait<kStages - 2>();
       __syncwarp();
       fetch();  // into the slot read in the last round
@@ -355,27 +438,48 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
       const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        uint32_t a[4], b[4];
-        p4::numbers<kBf16>(w0[g], a);
-        p4::numbers<kBf16>(w1[g], b);
+        if constexpr (kDig) {
+          constexpr uint32_t kHalf = 0x0f0f0f0fu;
+          const uint32_t a0 = w0[g] & kHalf, a2 = (w0[g] >> 4) & kHalf;
+          const uint32_t a1 = w1[g] & kHalf, a3 = (w1[g] >> 4) & kHalf;
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          const uint4 xv = p4::lds16(xa[nb] + blk * (2 * p4::kBlock) + 64 * g);
-          float d[4];
-          p4::mma16816_zero<kBf16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
-          p4::mma16816<kBf16>(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
-          acc[nb][0] = fmaf(g0[g], d[0], acc[nb][0]);
-          acc[nb][1] = fmaf(g0[g], d[1], acc[nb][1]);
-          acc[nb][2] = fmaf(g1[g], d[2], acc[nb][2]);
-          acc[nb][3] = fmaf(g1[g], d[3], acc[nb][3]);
+          for (int nb = 0; nb < kNB; ++nb) {
+            const uint2 xv = p4::lds8(xa[nb] + blk * p4::kBlock + 32 * g);
+            const uint4 c4 = p4::lds16(sa + ((blk * 4 + g) * kNB + nb) * 64);
+            const float sx = p4::lds4(fa + ((blk * 4 + g) * kNB + nb) * 8);
+            int d[4];
+            p4::mma16832(d, a0, a1, a2, a3, xv.x, xv.y, c4);
+            const float s0 = g0[g] * sx, s1 = g1[g] * sx;
+            const uint64_t off = f2pack(-12582912.f, -12582912.f);
+            const uint64_t v0 = add2(f2pack(__int_as_float(d[0]), __int_as_float(d[1])), off);
+            const uint64_t v1 = add2(f2pack(__int_as_float(d[2]), __int_as_float(d[3])), off);
+            acc2[nb][0] = fma2(f2pack(s0, s0), v0, acc2[nb][0]);
+            acc2[nb][1] = fma2(f2pack(s1, s1), v1, acc2[nb][1]);
+          }
+        } else {
+          uint32_t a[4], b[4];
+          p4::numbers<kMode == kBf16>(w0[g], a);
+          p4::numbers<kMode == kBf16>(w1[g], b);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) {
+            const uint4 xv = p4::lds16(xa[nb] + blk * (2 * p4::kBlock) + 64 * g);
+            float d[4];
+            p4::mma16816_zero<kMode == kBf16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+            p4::mma16816<kMode == kBf16>(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[nb][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], acc[nb][c]);
+          }
         }
       }
     }
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
-      if (kParts == 3) {
-        float v0 = acc[nb][0] + ((i & 1) ? 0.f : acc[nb][1]);
-        float v1 = acc[nb][2] + ((i & 1) ? 0.f : acc[nb][3]);
+      if constexpr (kDig) {  // digits 2 (i % 2) and the next of rows j and j + 8, then the other lane's
+        const float f = (i & 1) ? 1.52587890625e-05f : 1.0f;  // 2^-16
+        f2unpack(acc2[nb][0], acc[nb][0], acc[nb][1]);
+        f2unpack(acc2[nb][1], acc[nb][2], acc[nb][3]);
+        float v0 = fmaf(acc[nb][1], 0.00390625f, acc[nb][0]) * f;
+        float v1 = fmaf(acc[nb][3], 0.00390625f, acc[nb][2]) * f;
         v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
         v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
         y[nb][0] += (i & 1) ? v1 : v0;
@@ -384,14 +488,14 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
         for (int r = 0; r < kOuts; ++r) y[nb][r] += acc[nb][r];
       }
     }
-    if (p.split > 1) {  // the warps of a tile are neighbours: the first adds the others' results
+    if (split > 1) {  // the warps of a tile are neighbours: the first adds the others' results
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
         for (int r = 0; r < kOuts; ++r) red[((warp * kNB + nb) * kOuts + r) * 32 + lane] = y[nb][r];
       __syncthreads();
       if (s == 0)
-        for (int q = 1; q < p.split; ++q)
+        for (int q = 1; q < split; ++q)
 #pragma unroll
           for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
@@ -413,7 +517,7 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
                                                    : __half_as_ushort(__float2half_rn(v));
         }
     }
-    if (p.split > 1) __syncthreads();  // the sums are read before the next tile's are written
+    if (split > 1) __syncthreads();  // the sums are read before the next tile's are written
     row += tile_rows;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
@@ -473,10 +577,10 @@ constexpr size_t mv4_fixed_smem(int nb, int outs, int stages) {
   return 8 * stages * kMvStage + 8 * 32 * nb * outs * sizeof(float);
 }
 
-template <bool kBf16, int kParts, int kNB, int kStages>
+template <int kMode, int kNB, int kStages>
 static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
-  auto kern = matvec4_kernel<kBf16, kParts, kNB, kStages>;
-  const size_t smem = mv4_fixed_smem(kNB, kParts == 3 ? 1 : 4, kStages) + (size_t)p.M * kParts * (p.K + 32) * 2;
+  auto kern = matvec4_kernel<kMode, kNB, kStages>;
+  const size_t smem = mv4_fixed_smem(kNB, kMode == kDigits ? 1 : 4, kStages) + mv4_staged<kMode>(p.M, p.K, kNB);
   if (smem > kMaxSmem) return ANIMA_ERR_SHAPE;
   static SmemAttr attr;
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
@@ -486,16 +590,18 @@ static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
   const int per_sm = std::max(1, std::min(3, (int)(kMaxSmem / (smem + 1024))));
   const long long slots = (long long)per_sm * sm_count;
   long long best = 0;
-  for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+  for (int lg = 0; lg <= 3 && (1 << lg) <= blocks; ++lg) {
+    const int split = 1 << lg;
     const long long groups = ((long long)ntiles * split + 7) / 8;
     const long long parts = std::min(groups, std::max(1LL, slots / E));
     const long long waves = (E * parts + slots - 1) / slots;
     const long long cost = waves * ((groups + parts - 1) / parts) * ((blocks + split - 1) / split + 1);
-    if (split == 1 || cost < best) {
+    if (lg == 0 || cost < best) {
       best = cost;
-      p.split = split;
-      p.groups = (int)groups;
+      p.log_split = lg;
       p.parts = (int)parts;
+      p.g_each = (int)(groups / parts);
+      p.g_more = (int)(groups % parts);
     }
   }
   if ((long long)E * p.parts > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
@@ -505,19 +611,21 @@ static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
 
 // Rows of x of one launch: eight fp32 rows or sixteen 16-bit ones; fewer where their columns
 // would not fit shared memory, and a shorter ring where not even one would.
-static int mv4_rows(int K, int parts, int* stages) {
-  const size_t row = (size_t)parts * (K + 32) * 2;
+static int mv4_rows(int K, bool digits, int* stages) {
   *stages = 4;
-  const int fit = (int)((kMaxSmem - mv4_fixed_smem(2, 4, 4)) / row);
-  if (fit >= 1) return std::min(parts == 3 ? 8 : 16, fit);
-  *stages = 3;
-  return kMaxSmem - mv4_fixed_smem(1, 4, 3) >= row ? 1 : 0;
+  for (int m = digits ? 8 : 16; m > 0; --m) {
+    const size_t staged = digits ? mv4_staged<kDigits>(m, K, m <= 2 ? 1 : m <= 4 ? 2 : 4) : mv4_staged<kF16>(m, K, 1);
+    if (staged + mv4_fixed_smem(digits ? 4 : 2, digits ? 1 : 4, 4) <= kMaxSmem) return m;
+  }
+  *stages = 2;
+  const size_t staged = digits ? mv4_staged<kDigits>(1, K, 1) : mv4_staged<kF16>(1, K, 1);
+  return staged + mv4_fixed_smem(1, digits ? 1 : 4, 2) <= kMaxSmem ? 1 : 0;
 }
 
 int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
-  const int parts = a->x_dtype == ANIMA_DTYPE_F32 || a->silu ? 3 : 1;
+  const bool digits = a->x_dtype == ANIMA_DTYPE_F32 || a->silu;
   int stages;
-  const int rows = mv4_rows(a->K, parts, &stages);
+  const int rows = mv4_rows(a->K, digits, &stages);
   if (rows < 1) return ANIMA_ERR_SHAPE;
   Mv4Params p;
   p.codes = static_cast<const uint8_t*>(a->codes);
@@ -539,21 +647,20 @@ int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
     p.x = static_cast<const char*>(a->x) + m0 * p.xm * xs;
     p.out = static_cast<char*>(a->out) + m0 * p.om * os;
     p.add = a->add ? static_cast<const float*>(a->add) + m0 * p.am : nullptr;
-    const int nb = parts == 3 ? (p.M + 1) / 2 : (p.M + 7) / 8;
-    const bool bf = parts == 3 || a->x_dtype == ANIMA_DTYPE_BF16;
+    const bool bf = a->x_dtype == ANIMA_DTYPE_BF16, one = p.M <= 8;
     int rc;
-    if (stages == 3)
-      rc = parts == 3 ? mv4_t<true, 3, 1, 3>(p, a->E, sm_count, st)
-           : bf       ? mv4_t<true, 1, 1, 3>(p, a->E, sm_count, st)
-                      : mv4_t<false, 1, 1, 3>(p, a->E, sm_count, st);
-    else if (parts == 3)
-      rc = nb == 1   ? mv4_t<true, 3, 1, 4>(p, a->E, sm_count, st)
-           : nb == 2 ? mv4_t<true, 3, 2, 4>(p, a->E, sm_count, st)
-                     : mv4_t<true, 3, 4, 4>(p, a->E, sm_count, st);
+    if (stages == 2)
+      rc = digits ? mv4_t<kDigits, 1, 2>(p, a->E, sm_count, st)
+           : bf   ? mv4_t<kBf16, 1, 2>(p, a->E, sm_count, st)
+                  : mv4_t<kF16, 1, 2>(p, a->E, sm_count, st);
+    else if (digits)
+      rc = p.M <= 2   ? mv4_t<kDigits, 1, 4>(p, a->E, sm_count, st)
+           : p.M <= 4 ? mv4_t<kDigits, 2, 4>(p, a->E, sm_count, st)
+                      : mv4_t<kDigits, 4, 4>(p, a->E, sm_count, st);
     else if (bf)
-      rc = nb == 1 ? mv4_t<true, 1, 1, 4>(p, a->E, sm_count, st) : mv4_t<true, 1, 2, 4>(p, a->E, sm_count, st);
+      rc = one ? mv4_t<kBf16, 1, 4>(p, a->E, sm_count, st) : mv4_t<kBf16, 2, 4>(p, a->E, sm_count, st);
     else
-      rc = nb == 1 ? mv4_t<false, 1, 1, 4>(p, a->E, sm_count, st) : mv4_t<false, 1, 2, 4>(p, a->E, sm_count, st);
+      rc = one ? mv4_t<kF16, 1, 4>(p, a->E, sm_count, st) : mv4_t<kF16, 2, 4>(p, a->E, sm_count, st);
     if (rc != ANIMA_OK) return rc;
   }
   return ANIMA_OK;

@@ -105,6 +105,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ float lds4(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint2 lds8(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
@@ -146,6 +151,17 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32
         "{%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// D = A B + C, m16n8k32 on whole numbers: A unsigned and B signed bytes.  Lane 4 j + i holds k = 4 i .. + 3 and 16 + 4 i .. + 3 of A rows j (a0, a2) and j + 8 (a1,
+// a3) and of B column j; D as in m16n8k16.
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1, const uint4& c) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
 }
 
 }  // namespace p4

@@ -309,13 +309,15 @@ def test_quantize_strided_views():
 def matvec_bound(ax, aw, K, y, out_dtype, silu):
     """Rounding bound of one result, with S = sum |x| |w|.  Products are exact.  A group's 32 are
     summed by the tensor core (one truncation, a step of fp32, per product and addition: 64), then
-    K/32 scaled sums, at most 8 warps and 3 parts, the addend and the scale's product are
-    rounded: K/32 + 16 half steps, taken as steps.  The two parts that follow a bf16 one are
-    below 2^-8 of it, so S covers them with 1 %.  SiLU adds 8 steps on x (expf 2, sum, quotient, and
-    the argument's)."""
+    K/32 scaled sums, at most 8 warps and 4 digits, the addend and the scale's product are
+    rounded: K/32 + 16 half steps, taken as steps.  fp32 rows enter as whole numbers of 2^(E - 30) per
+    group of 32, 2^E at most twice the group's largest magnitude: half of that per value.  SiLU
+    adds 8 steps on x (expf 2, sum, quotient, and the argument's)."""
     step = 2.0 ** -23
     S = ax @ np.swapaxes(aw, -1, -2)
-    return 1.01 * S * step * (64 + K / 32 + 16 + (8 if silu else 0)) + np.abs(y) * half_step(out_dtype) + 1e-37 + \
+    top = np.repeat(ax.reshape(ax.shape[:-1] + (K // 32, 32)).max(-1), 32, -1)
+    T = top @ np.swapaxes(aw, -1, -2)
+    return 1.01 * S * step * (64 + K / 32 + 16 + (8 if silu else 0)) + T * 2.0 ** -30 + np.abs(y) * half_step(out_dtype) + 1e-37 + \
         (6e-8 if out_dtype == F16 else 0.0)  # fp16 subnormals
 
 
@@ -376,9 +378,25 @@ def test_matvec_many_rows_of_w():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("std", [1e-30, 1e30])
+@pytest.mark.parametrize("std", [1e-38, 1e-30, 1e30, 2e36])
 def test_matvec_keeps_the_range_of_fp32(std):
     check_matvec(1, 2, 64, 256, F32, std=std)
+
+
+@pytest.mark.gpu
+def test_matvec_magnitudes_far_apart():
+    """Groups of 1e-20, 1 and 1e20 side by side, and within a group values 2^20 apart."""
+    w, wv = random_packed((40, 384), 8)
+    x = torch.randn(3, 384, generator=torch.Generator().manual_seed(9))
+    x[:, :128] *= 1e-20
+    x[0, 256:] *= 1e20
+    x[1, 128:] = 0
+    x[2, ::3] *= 2.0 ** -20
+    x[2, 5] = -2.0 ** -149
+    y = anima_attn.matvec4(x.cuda(), w).double().cpu().numpy()
+    xv = x.double().numpy()
+    want = xv @ wv.T
+    assert (np.abs(y - want) <= matvec_bound(np.abs(xv), np.abs(wv), 384, want, F32, False)).all()
 
 
 @pytest.mark.gpu
