@@ -30,6 +30,8 @@ _HALF = (torch.float16, torch.bfloat16)
 _MATVEC_ARGS = struct.Struct("@Pi2qPPP2qPi2qiiiii0q")
 _ATTN_ARGS = struct.Struct("@PPPPPiP3qiiiiifIPPQ")
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current = getattr(torch._C, "_cuda_getDevice", None)
+_U8, _F16 = torch.uint8, torch.float16
 
 
 class Packed4(NamedTuple):
@@ -48,28 +50,27 @@ class Packed4(NamedTuple):
         return self
 
 
-def _here(*ts) -> int:
+def _here(t, *ts) -> int:
     """The current stream of the current device, on which every tensor must be."""
-    if not ts[0].is_cuda:
+    dev = t.get_device()  # -1 on the CPU
+    if dev < 0 or dev != _current():
         raise ValueError("anima_attn ops take CUDA tensors on the current device")
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
+    for u in ts:
+        if u is not None and u.get_device() != dev:
             raise ValueError("anima_attn ops take CUDA tensors on the current device")
     return _raw_stream(dev)
 
 
-def _check_packed(p: Packed4, what: str) -> tuple:
-    """Shape [..., K] of a packed tensor, after checking that its two arrays belong together."""
+def _check_packed(p: Packed4, what: str) -> torch.Size:
+    """The codes' shape [..., K/2], after checking that codes and scales belong together."""
     c, s = p
-    if c.dtype is not torch.uint8 or s.dtype is not torch.float16 or not c.is_contiguous() or not s.is_contiguous():
+    if c.dtype is not _U8 or s.dtype is not _F16 or not c.is_contiguous() or not s.is_contiguous():
         raise ValueError(f"{what}: packed codes are contiguous uint8, scales contiguous float16")
-    *lead, half = c.shape
-    *slead, groups = s.shape
-    if half == 0 or half % 64 or groups * 16 != half or lead != slead:
+    cs, ss = c.shape, s.shape
+    half = cs[-1]
+    if half == 0 or half % 64 or ss[-1] * 16 != half or cs[:-1] != ss[:-1]:
         raise ValueError(f"{what}: codes [..., K/2] and scales [..., K/32], K a multiple of 128")
-    lead.append(2 * half)
-    return lead
+    return cs
 
 
 @lru_cache(maxsize=1024)
@@ -105,8 +106,7 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
         raise ValueError("the last axis must be a positive multiple of 128")
     K, lead = x.shape[-1], x.shape[:-1]
     if out is None:
-        out = Packed4(torch.empty(lead + (K // 2,), device=x.device, dtype=torch.uint8),
-                      torch.empty(lead + (K // 32,), device=x.device, dtype=torch.float16))
+        out = Packed4(x.new_empty(lead + (K // 2,), dtype=_U8), x.new_empty(lead + (K // 32,), dtype=_F16))
     else:
         _here(*out)
         _check_packed(out, "out")
@@ -126,9 +126,10 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
         (n0, s0), (n1, s1), (n2, s2) = axes
     if x.data_ptr() % 16:
         raise ValueError("x must be 16-byte aligned")
-    L.check(L.lib.anima_quantize4(x.data_ptr(), _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K,
-                                  out.codes.data_ptr(), out.scales.data_ptr(), stream),
-            "anima_quantize4")
+    rc = L.lib.anima_quantize4(x.data_ptr(), _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K,
+                               out.codes.data_ptr(), out.scales.data_ptr(), stream)
+    if rc:
+        L.check(rc, "anima_quantize4")
     return out
 
 
@@ -136,14 +137,15 @@ def dequantize4(p: Packed4, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values [..., K] that a packed tensor stands for: exact in float32, rounded once in
     float16 and bfloat16."""
     stream = _here(*p)
-    shape = _check_packed(p, "p")
+    cs = _check_packed(p, "p")
     if dtype not in _TORCH_DT:
         raise ValueError("dtype must be float32, float16 or bfloat16")
-    y = torch.empty(shape, device=p.codes.device, dtype=dtype)
-    K = shape[-1]
-    L.check(L.lib.anima_dequantize4(p.codes.data_ptr(), p.scales.data_ptr(), y.data_ptr(),
-                                    _TORCH_DT[dtype], y.numel() // K, K, stream),
-            "anima_dequantize4")
+    K = 2 * cs[-1]
+    y = p.scales.new_empty(cs[:-1] + (K,), dtype=dtype)
+    rc = L.lib.anima_dequantize4(p.codes.data_ptr(), p.scales.data_ptr(), y.data_ptr(),
+                                 _TORCH_DT[dtype], y.numel() // K, K, stream)
+    if rc:
+        L.check(rc, "anima_dequantize4")
     return y
 
 
@@ -160,7 +162,7 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     pass over W."""
     stream = _here(x, add, out, *w)
     ws = _check_packed(w, "w")
-    K = ws[-1]
+    K = 2 * ws[-1]
     if x.dtype not in _TORCH_DT:
         raise ValueError("x must be float32, float16 or bfloat16")
     if len(ws) == 2 and x.dim() in (1, 2):
@@ -179,7 +181,7 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     if out is None:
         if out_dtype not in _TORCH_DT:
             raise ValueError("out_dtype must be float32, float16 or bfloat16")
-        out = torch.empty(shape, device=x.device, dtype=out_dtype)
+        out = x.new_empty(shape, dtype=out_dtype)
     elif out.shape != shape or out.dtype not in _TORCH_DT or (N > 1 and out.stride(-1) != 1):
         raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous")
     ostr = out.stride()
@@ -196,7 +198,9 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     a = _MATVEC_ARGS.pack(x.data_ptr(), _TORCH_DT[x.dtype], xe, xm, w.codes.data_ptr(),
                           w.scales.data_ptr(), aptr, ae, am, out.data_ptr(), _TORCH_DT[out.dtype],
                           oe, om, E, M, N, K, 1 if silu else 0)
-    L.check(L.lib.anima_matvec4(a, stream), "anima_matvec4")
+    rc = L.lib.anima_matvec4(a, stream)
+    if rc:
+        L.check(rc, "anima_matvec4")
     return out
 
 
@@ -220,14 +224,14 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     if BH != B * H or D != 128 or BH == 0 or Sq == 0:
         raise ValueError("q must be [B*H, S_q, 128] with at least one row")
     ks = _check_packed(k, "k")
-    if ks != _check_packed(v, "v") or len(ks) != 3 or ks[0] != BH or ks[1] == 0 or ks[2] != D:
+    if ks != _check_packed(v, "v") or len(ks) != 3 or ks[0] != BH or ks[1] == 0 or ks[2] != 64:
         raise ValueError("k and v must be packed [B*H, S_kv, 128] with at least one key")
     Skv = ks[1]
     if out_layout not in ("bshd", "bhsd"):
         raise ValueError("out_layout must be 'bshd' or 'bhsd'")
     shape = (B, Sq, H, D) if out_layout == "bshd" else (B, H, Sq, D)
     if out is None:
-        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("out must have q's type, the layout's shape and a contiguous head dimension")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
@@ -237,17 +241,20 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     strides = (st[0], st[2], st[1]) if out_layout == "bshd" else (st[0], st[1], st[2])
     flags, vl = 0, None
     if kv_valid_len is not None:
-        vl = kv_valid_len.to(dtype=torch.int32).contiguous()
+        vl = kv_valid_len if kv_valid_len.dtype is torch.int32 else kv_valid_len.to(torch.int32)
+        vl = vl.contiguous()
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")
         flags = L.FLAG_MASK
     nbytes = _kv4_workspace(q.get_device(), q.dtype, B, H, Sq, Skv)
     # Scratch of this call alone, from the caching allocator: freed on return, its block goes
     # to work enqueued later on this stream, and a captured graph keeps it in its own pool.
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ws = q.new_empty(nbytes, dtype=_U8) if nbytes else None
     a = _ATTN_ARGS.pack(q.data_ptr(), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
                         v.scales.data_ptr(), _TORCH_DT[q.dtype], out.data_ptr(), *strides, B, H, Sq, Skv,
                         D, scale, flags, 0 if vl is None else vl.data_ptr(),
                         0 if ws is None else ws.data_ptr(), nbytes)
-    L.check(L.lib.anima_attn_kv4_fwd(a, stream), "anima_attn_kv4_fwd")
+    rc = L.lib.anima_attn_kv4_fwd(a, stream)
+    if rc:
+        L.check(rc, "anima_attn_kv4_fwd")
     return out
