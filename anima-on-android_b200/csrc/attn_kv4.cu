@@ -439,11 +439,12 @@ __global__ void __launch_bounds__(256)
 }  // namespace kv4
 
 // Whether the packed cache is read directly.  Up to 16 rows always; beyond, the rows' passes over the
-// cache cost more than the tile kernel's start (some 6 us) once heads x rows x keys exceed 2^20.
-// Measured, us, this way against the tile kernel, heads x rows x keys: 4 x 256 x 512 9.7 / 14.8,
-// 32 x 64 x 512 12.5 / 13.4, 4 x 1024 x 512 19.3 / 17.4, 32 x 64 x 2048 28 / 18, 32 x 16 x 8192 27 / 35.
+// cache (and, below 256 keys, their starts) cost more than the tile kernel's start (some 6 us) once
+// heads x rows x keys exceed 2^20.  Measured, us, this way against the tile kernel, heads x rows x
+// keys: 4 x 256 x 512 9.7 / 14.8, 32 x 64 x 512 12.5 / 13.4, 4 x 1024 x 512 19.3 / 17.4, 32 x 64 x
+// 2048 28 / 18, 32 x 16 x 8192 27 / 35, 32 x 128 x 130 12.3 / 10.2, 4 x 1024 x 130 12.5 / 12.7.
 static bool rows_path(long long bh, long long S_q, long long S_kv) {
-  return S_q <= 16 || bh * S_q * S_kv <= (1 << 20);
+  return S_q <= 16 || bh * S_q * std::max(S_kv, 256LL) <= (1 << 20);
 }
 // Whether K and V are unpacked once for the attention core: fp16 calls of two rounds of 256-row units or
 // more (4096 x 512 at 32 heads 52 us against the tile kernel's 57, 16384 x 512 152 / 184; at one

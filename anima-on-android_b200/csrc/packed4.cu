@@ -211,6 +211,7 @@ struct Mv4Params {
   int g_each, g_more;    // tile groups (8 / split tiles) of a CTA; the first g_more have one more
   int log_split;         // log2 of the warps per tile
   int silu, x_dtype, out_dtype;
+  int x_aligned;         // every row of x starts on 16 bytes
 };
 
 constexpr int kMvThreads = 256;
@@ -238,8 +239,14 @@ __host__ __device__ constexpr size_t mv4_staged(int M, int K, int nb) {
 
 // Eight values of x, SiLU applied if asked for.
 __device__ __forceinline__ void load_x8(const Mv4Params& p, long long at, float (&v)[8]) {
+  if (p.x_dtype == ANIMA_DTYPE_F32 && p.x_aligned) {
+    const float4* x = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at);
+    const float4 a = __ldg(x), b = __ldg(x + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = load_x(p, at + k);
+    for (int k = 0; k < 8; ++k) v[k] = load_x(p, at + k);
+  }
   if (p.silu)
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = __fdividef(v[k], 1.0f + expf(-v[k]));
@@ -259,22 +266,14 @@ __device__ __forceinline__ void stage_digits(const Mv4Params& p, int e, int nb, 
     float v[8];
     load_x8(p, (long long)e * p.xe + (long long)m * p.xm + 8 * r, v);
     uint32_t top = 0;
-    int odd = 0;  // values that are infinite, or 2 for a NaN
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t b = __float_as_uint(v[k]) & 0x7fffffffu;
-      top = max(top, b);
-      odd += b == 0x7f800000u ? 1 : b > 0x7f800000u ? 2 : 0;
-    }
+    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      top = max(top, __shfl_xor_sync(mask, top, o));
-      odd += __shfl_xor_sync(mask, odd, o);
-    }
+    for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
     const int E = max((int)(top >> 23), 1) - 126;
     uint32_t t[8];
     float scale;
-    if (odd == 0) {
+    if (top < 0x7f800000u) {
       const int s0 = (30 - E) / 2, s1 = 30 - E - s0;  // in two steps: neither leaves fp32
       const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
 #pragma unroll
@@ -283,6 +282,12 @@ __device__ __forceinline__ void stage_digits(const Mv4Params& p, int e, int nb, 
       scale = E - 6 >= -126 ? __int_as_float((E - 6 + 127) << 23) : __int_as_float(1 << (E - 6 + 149));
     } else {
       // one infinity makes its products infinite or NaN and hides the rest; anything else is NaN
+      int odd = 0;  // infinities of the group, two for a NaN
+#pragma unroll
+      for (int k = 0; k < 8; ++k) odd += isnan(v[k]) ? 2 : isinf(v[k]) ? 1 : 0;
+      const uint32_t group = 0xfu << (threadIdx.x & 28);  // its four lanes come here together
+      odd += __shfl_xor_sync(group, odd, 1);
+      odd += __shfl_xor_sync(group, odd, 2);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         t[k] = isinf(v[k]) ? (v[k] > 0.f ? 0x01010101u : 0xffffffffu) : 0u;
@@ -380,11 +385,21 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
   if constexpr (kDig) {
     stage_digits(p, e, kNB, cols, start, xscale);
   } else {  // 16-bit rows as they are
-    for (int m = 0; m < p.M; ++m) {
-      const uint16_t* const x = static_cast<const uint16_t*>(p.x) + (long long)e * p.xe + (long long)m * p.xm;
-      uint16_t* const to = reinterpret_cast<uint16_t*>(cols + (size_t)m * stride);
+    const uint16_t* const x = static_cast<const uint16_t*>(p.x) + (long long)e * p.xe;
+    if (p.x_aligned) {
+      const int runs = p.K / 8;
+      for (int c = threadIdx.x; c < p.M * runs; c += kMvThreads) {
+        const int m = c / runs, r = c - m * runs;
+        p4::cp16(smem_u32(cols) + m * stride + 16 * r, x + (long long)m * p.xm + 8 * r);
+      }
+      p4::cp_commit();
+      p4::cp_wait<0>();
+    } else {
+      for (int m = 0; m < p.M; ++m) {
+        uint16_t* const to = reinterpret_cast<uint16_t*>(cols + (size_t)m * stride);
 #pragma unroll 4
-      for (int k = threadIdx.x; k < p.K; k += kMvThreads) to[k] = __ldg(x + k);
+        for (int k = threadIdx.x; k < p.K; k += kMvThreads) to[k] = __ldg(x + (long long)m * p.xm + k);
+      }
     }
   }
   uint32_t xa[kNB];  // this lane's column of x, at its eight values of a group
@@ -642,6 +657,7 @@ int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
   p.x_dtype = a->x_dtype;
   p.out_dtype = a->out_dtype;
   const int xs = a->x_dtype == ANIMA_DTYPE_F32 ? 4 : 2, os = a->out_dtype == ANIMA_DTYPE_F32 ? 4 : 2;
+  p.x_aligned = ((reinterpret_cast<uintptr_t>(a->x) | (uintptr_t)(xs * p.xe) | (uintptr_t)(xs * p.xm)) & 15u) == 0;
   for (int m0 = 0; m0 < a->M; m0 += rows) {
     p.M = std::min(rows, a->M - m0);
     p.x = static_cast<const char*>(a->x) + m0 * p.xm * xs;

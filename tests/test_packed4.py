@@ -422,6 +422,20 @@ def test_matvec_views_and_shapes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("xdt", [F16, BF16, F32])
+def test_matvec_unaligned_rows(xdt):
+    """Rows of x that start on any element, and a row repeated by a zero stride."""
+    g = torch.Generator().manual_seed(10)
+    w, wv = random_packed((50, 256), 11)
+    buf = torch.randn(3, 259, generator=g).to(xdt).cuda()
+    for x in (buf[:, 1:257], buf[:, 3:], buf[1:2, 1:257].expand(4, 256)):
+        y = anima_attn.matvec4(x, w).double().cpu().numpy()
+        xv = x.double().cpu().numpy()
+        want = xv @ wv.T
+        assert (np.abs(y - want) <= matvec_bound(np.abs(xv), np.abs(wv), 256, want, F32, False)).all()
+
+
+@pytest.mark.gpu
 def test_matvec_not_finite():
     """A NaN scale reaches its row of W only, a NaN or infinite x its row of x only."""
     w, wv = random_packed((32, 256), 7)
@@ -543,7 +557,8 @@ def test_attention_masked_slices(Sq, Skv, lens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("B,H,Sq,Skv,lens", [(2, 16, 2307, 133, None), (3, 13, 2049, 130, [0, 130, 40]), (5, 40, 100, 300, [300, 0, 1, 0, 128])])
+@pytest.mark.parametrize("B,H,Sq,Skv,lens", [(2, 16, 2307, 133, None), (3, 13, 2049, 130, [0, 130, 40]), (5, 40, 100, 300, [300, 0, 1, 0, 128]),
+                                             (4, 2, 2186, 6, [6, 4, 2, 0]), (2, 4, 3812, 2, None)])
 def test_attention_many_units(dtype, B, H, Sq, Skv, lens):
     """More units than SMs: the persistent grid of the tile kernel, and the unpacked core for fp16."""
     check_attention(B, H, Sq, Skv, dtype, lens=lens)
