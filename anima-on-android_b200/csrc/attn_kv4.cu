@@ -70,6 +70,11 @@ using p4::cp_commit;
 using p4::cp_wait;
 using p4::lds16;
 using p4::lds8;
+template <bool kBf16>
+__device__ __forceinline__ float2 widen(uint32_t w) {
+  if (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
 // Transposes an 8 x 8 matrix of 16-bit values held two to a lane (row lane / 4).
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -90,10 +95,15 @@ constexpr size_t smem_bytes(int stages, int rows) {
 }
 
 // kBf16: type of q and out (else fp16); kOne: the form for a single row, else up to eight; kW:
-// warps; kNS: stages.  A single row fills all eight columns of Q, so that every
-// lane has the scores of its keys, and the columns of P are the row's four group-scaled forms, high
-// parts in columns 0 .. 3 and low parts in 4 .. 7: one operand, made once, serves all
-// eight dim tiles, and of a tile of group g columns g and 4 + g count.
+// warps; kNS: stages.
+//
+// A single row has the eight columns to itself.  For S^T its q is scaled by a power of two to whole
+// numbers below 2^30 and written in four signed base-256 digits, the columns (twice over), and the MMA
+// is the one of whole numbers (m16n8k32) on c = n + 8: three instructions unpack eight codes where
+// fp16 takes nine and bf16 eleven, and the sums are exact (1 x 65536, 32 heads: 66 -> 60 us).  For O^T
+// the columns of P are the row's four group-scaled forms, high parts in columns 0 .. 3 and low parts in
+// 4 .. 7: one operand, made once, serves all eight dim tiles, and of a tile of group g
+// columns g and 4 + g count.
 template <bool kBf16, bool kOne, int kW, int kNS>
 __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -120,6 +130,49 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     qf[g] = make_uint4(0u, 0u, 0u, 0u);
     if (qrow < p.S_q)
       qf[g] = __ldg(reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + qrow) * kD + 32 * g + 8 * i));
+  }
+  float sl2 = p.scale_log2;
+  uint2 qd[4];       // kOne: digit j % 4 of this lane's eight values of group g, in the codes' order
+  uint64_t base[4];  // and what its two columns' sums start from, 1.5 * 2^23 + 8 sum(digits)
+  if constexpr (kOne) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t w[4] = {qf[g].x, qf[g].y, qf[g].z, qf[g].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = widen<kBf16>(w[k]);
+        top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+      }
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int E = max((int)(top >> 23), 1) - 126;  // |q| < 2^E
+    const int e0 = (30 - E) / 2, e1 = 30 - E - e0;  // in two steps: neither factor leaves fp32
+    const float f0 = __int_as_float((e0 + 127) << 23), f1 = __int_as_float((e1 + 127) << 23);
+    const int s0 = (E - 6) / 2, s1 = E - 6 - s0;
+    sl2 = top >= 0x7f800000u ? NAN
+                             : sl2 * __int_as_float((s0 + 127) << 23) * __int_as_float((s1 + 127) << 23);
+    const uint32_t sel = (uint32_t)(3 - (j & 3)) | (uint32_t)(7 - (j & 3)) << 4;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t w[4] = {qf[g].x, qf[g].y, qf[g].z, qf[g].w};
+      uint32_t t[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = widen<kBf16>(w[k]);
+        t[2 * k] = ((uint32_t)__float2int_rn(v.x * f0 * f1) + 0x00808080u) ^ 0x00808080u;
+        t[2 * k + 1] = ((uint32_t)__float2int_rn(v.y * f0 * f1) + 0x00808080u) ^ 0x00808080u;
+      }
+      qd[g].x = __byte_perm(__byte_perm(t[0], t[4], sel), __byte_perm(t[1], t[5], sel), 0x5410);
+      qd[g].y = __byte_perm(__byte_perm(t[2], t[6], sel), __byte_perm(t[3], t[7], sel), 0x5410);
+      int x = __dp4a((int)qd[g].x, 0x01010101, __dp4a((int)qd[g].y, 0x01010101, 0));
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      const float x0 = (float)(12582912 + 8 * __shfl_sync(0xffffffffu, x, 8 * i));
+      const float x1 = (float)(12582912 + 8 * __shfl_sync(0xffffffffu, x, 8 * i + 4));
+      base[g] = f2pack(-x0, -x1);
+    }
   }
 
   const uint32_t ring = smem_u32(smem) + warp * kNS * kStageBytes;
@@ -197,16 +250,38 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
       const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
       for (int c = 0; c < 4; ++c) sc[u][c] = 0.f;
+      if constexpr (kOne) {
+        constexpr uint32_t kHalf = 0x0f0f0f0fu, kStart = 0x4b400000u;
+        uint64_t s0 = 0ull, s1 = 0ull;  // of keys k0 and k0 + 8: columns 2 i, 2 i + 1
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t x[4], y[4];
-        p4::numbers<kBf16>(w0[g], x);
-        p4::numbers<kBf16>(w1[g], y);
-        float d[4];
-        p4::mma16816_zero<kBf16>(d, x[0], y[0], x[1], y[1], qf[g].x, qf[g].y);
-        p4::mma16816<kBf16>(d, x[2], y[2], x[3], y[3], qf[g].z, qf[g].w);
+        for (int g = 0; g < 4; ++g) {
+          int d[4];
+          p4::mma16832(d, w0[g] & kHalf, w1[g] & kHalf, (w0[g] >> 4) & kHalf, (w1[g] >> 4) & kHalf, qd[g].x,
+                       qd[g].y, make_uint4(kStart, kStart, kStart, kStart));
+          s0 = fma2(f2pack(g0[g], g0[g]), add2(f2pack(__int_as_float(d[0]), __int_as_float(d[1])), base[g]), s0);
+          s1 = fma2(f2pack(g1[g], g1[g]), add2(f2pack(__int_as_float(d[2]), __int_as_float(d[3])), base[g]), s1);
+        }
+        // the digits 2 (i % 2) and the next together, then the other lane's two
+        const float f = (i & 1) ? 1.52587890625e-05f : 1.0f;  // 2^-16
+        float a, b;
+        f2unpack(s0, a, b);
+        a = fmaf(b, 0.00390625f, a) * f;
+        sc[u][0] = a + __shfl_xor_sync(0xffffffffu, a, 1);
+        f2unpack(s1, a, b);
+        a = fmaf(b, 0.00390625f, a) * f;
+        sc[u][2] = a + __shfl_xor_sync(0xffffffffu, a, 1);
+      } else {
 #pragma unroll
-        for (int c = 0; c < 4; c += kStep) sc[u][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], sc[u][c]);
+        for (int g = 0; g < 4; ++g) {
+          uint32_t x[4], y[4];
+          p4::numbers<kBf16>(w0[g], x);
+          p4::numbers<kBf16>(w1[g], y);
+          float d[4];
+          p4::mma16816_zero<kBf16>(d, x[0], y[0], x[1], y[1], qf[g].x, qf[g].y);
+          p4::mma16816<kBf16>(d, x[2], y[2], x[3], y[3], qf[g].z, qf[g].w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[u][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], sc[u][c]);
+        }
       }
     }
     // scores in log2 units; keys at or past len are masked
@@ -216,7 +291,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int c = 0; c < 4; c += kStep) {
-        const float v = sc[u][c] * p.scale_log2;
+        const float v = sc[u][c] * sl2;
         sc[u][c] = 16 * u + j + 8 * (c >> 1) < left ? v : -INFINITY;
         over = over || sc[u][c] > m[c & 1] + kRescale;
       }
