@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   uint32_t ncta;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
   const int rank = (int)cluster_rank();
+  grid_dependency_wait();  // launched while the kernel before it drains
   const int cluster = blockIdx.x / ncta;
   const int slice = cluster / p.units, unit = cluster - slice * p.units;
   const int bh = unit / p.nqb, row0 = (unit - bh * p.nqb) * kRows;
@@ -476,6 +477,7 @@ __global__ void __launch_bounds__(256)
     expand_kernel(const uint4* kc, const uint2* ks, const uint4* vc, const uint2* vs, uint16_t* ko,
                   uint16_t* vo, const int* valid, int H, int S_kv, long long quads) {
   grid_dependents_launch();  // the core sets up meanwhile; it waits for this grid before it reads
+  grid_dependency_wait();
   const uint4* codes = blockIdx.y ? vc : kc;
   const uint2* scales = blockIdx.y ? vs : ks;
   uint16_t* out = blockIdx.y ? vo : ko;
@@ -562,23 +564,7 @@ static int rows_t(const kv4::Params& p, int ncta, cudaStream_t st) {
   constexpr size_t smem = kv4::smem_bytes<kW>(kStages, kOne ? 1 : 8);
   static SmemAttr attr;
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.units * p.nsplit * ncta));
-  cfg.blockDim = dim3(32 * kW);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ncta;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
-    cudaGetLastError();
-    return ANIMA_ERR_CUDA;
-  }
-  return ANIMA_OK;
+  return launch_clusters(kern, p.units * p.nsplit * ncta, ncta, 32 * kW, smem, st, p);
 }
 
 static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }

@@ -183,6 +183,9 @@ __global__ void __launch_bounds__(kThreads16, 1)
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   const int segs = p.units * p.nsplit;
+  // Launched as a programmatic dependent of the kernel before it on the stream: the set-up above
+  // overlaps that kernel's end, and no global memory is touched before it has completed.
+  grid_dependency_wait();
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(bar, parity, abort, p.status, ANIMA_ERR_TIMEOUT);
   };
@@ -690,10 +693,20 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
   t.nqb = (S_q + t.nt * attn::kBM - 1) / (t.nt * attn::kBM);
   t.units = (long long)bh * t.nqb;
   const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
-  // As many slices as the SMs hold in one round, if that shortens the longest chain of key tiles by
-  // three or more (the merge costs about two).
-  t.nsplit = (int)std::max(1LL, std::min({sm_count / std::max(1LL, t.units), tiles, 64LL}));
-  if (tiles - (tiles + t.nsplit - 1) / t.nsplit < 3) t.nsplit = 1;
+  // Slices: at most as many as the SMs hold in one round; the number with the least of the longest
+  // chain of key tiles, some 2 us each, plus, if more than one, the merge, which is two tiles and one
+  // more per 16384 rows of partials (32 units of 256 rows: 4 tiles whole 16.7 us, in 2 slices 20.3, in
+  // 4 19.3; 16 units, 16 tiles: 42.7 whole, 23.8 in 4, 21.0 in 8).
+  const long long most = std::min({sm_count / std::max(1LL, t.units), tiles, 64LL});
+  t.nsplit = 1;
+  double best = (double)tiles;
+  for (int k = 2; k <= most; ++k) {
+    const double cost = (double)((tiles + k - 1) / k) + 2.0 + (double)k * t.units * t.nt * attn::kBM / 16384.0;
+    if (cost < best) {
+      best = cost;
+      t.nsplit = k;
+    }
+  }
   t.bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4_part_floats(t.nt * attn::kBM)) * 4 : 0;
   return t;
 }
@@ -704,30 +717,17 @@ static int tile_t(const CUtensorMap& mq, const kv4t::Params& p, int grid, cudaSt
   constexpr size_t smem = kv4t::smem_bytes<kNT>();
   static SmemAttr attr;
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
-  kern<<<grid, kv4t::kThreads16, smem, st>>>(mq, p);
-  return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+  return launch_dependent(kern, grid, kv4t::kThreads16, smem, st, mq, p);
 }
 
 int kv4_merge_launch(const AnimaAttnKv4Args* a, const float* part, int nqb, int rows, int units, int nsplit,
                      int sm_count, cudaStream_t st) {
   const long long total = (long long)a->B * a->H * a->S_q;
   auto merge = a->dtype == ANIMA_DTYPE_BF16 ? kv4t::kv4_merge_kernel<true> : kv4t::kv4_merge_kernel<false>;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<long long>((total + 7) / 8, (long long)sm_count * 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, merge, part, a->out, (long long)a->out_stride[0], (long long)a->out_stride[1],
-                         (long long)a->out_stride[2], a->H, a->S_q, nqb, rows, units, nsplit, total) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return ANIMA_ERR_CUDA;
-  }
-  return ANIMA_OK;
+  const int grid = (int)std::min<long long>((total + 7) / 8, (long long)sm_count * 8);
+  return launch_dependent(merge, grid, 256, 0, st, part, a->out, (long long)a->out_stride[0],
+                          (long long)a->out_stride[1], (long long)a->out_stride[2], a->H, a->S_q, nqb, rows,
+                          units, nsplit, total);
 }
 
 int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st) {

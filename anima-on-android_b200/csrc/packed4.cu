@@ -318,6 +318,7 @@ __device__ __forceinline__ void stage_digits(const Mv4Params& p, int e, int nb, 
 template <int kMode, int kNB, int kStages>
 __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  grid_dependency_wait();  // launched while the kernel before it drains
   constexpr bool kDig = kMode == kDigits;
   constexpr int kOuts = kDig ? 1 : 4;  // results of a lane per block of columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -620,8 +621,7 @@ static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
     }
   }
   if ((long long)E * p.parts > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
-  kern<<<E * p.parts, kMvThreads, smem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
+  return launch_dependent(kern, E * p.parts, kMvThreads, smem, st, p);
 }
 
 // Rows of x of one launch: eight fp32 rows or sixteen 16-bit ones; fewer where their columns

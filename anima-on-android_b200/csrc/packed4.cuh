@@ -14,6 +14,7 @@
 // 2 p, 2 p + 1, so masking with 0x000f000f leaves a pair in consecutive order.
 #pragma once
 #include <atomic>
+#include <utility>
 
 #include "common.cuh"
 
@@ -165,6 +166,38 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
 }
 
 }  // namespace p4
+
+// Launches a kernel as a programmatic dependent of the one before it on the stream, optionally in
+// clusters: its blocks may start while that one drains.  Every block of the kernel has to run
+// grid_dependency_wait() before it touches global memory.
+template <typename... Params, typename... Args>
+static int launch_clusters(void (*kern)(Params...), int grid, int cluster, int threads, size_t smem, cudaStream_t st,
+                           Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kern, Params(std::forward<Args>(args))...) != cudaSuccess) {
+    cudaGetLastError();
+    return ANIMA_ERR_CUDA;
+  }
+  return ANIMA_OK;
+}
+template <typename... Params, typename... Args>
+static int launch_dependent(void (*kern)(Params...), int grid, int threads, size_t smem, cudaStream_t st,
+                            Args&&... args) {
+  return launch_clusters(kern, grid, 0, threads, smem, st, std::forward<Args>(args)...);
+}
 
 // Largest dynamic shared memory asked for a kernel so far, per device: the attribute is set when
 // a launch needs more, not at every launch.
