@@ -27,6 +27,12 @@
 // Tensor memory: S_0, S_1, O_0, O_1 of 128 columns; P_i overlays S_i.  With two query tiles their
 // MMAs alternate, so one tile's softmax runs beside the other's MMAs; with one, its key tiles
 // alternate between S_0 and S_1, and a tile's QK^T runs beside the softmax of the tile before it.
+//
+// What bounds it is the chain of the core kernel: softmax (an exponential a score), hand-off, MMAs.  A
+// step of two query tiles takes some 4,300 cycles against 2,050 of MMAs (traced); without any unpacking
+// it took 8 % less, without any exponential 2 %.  256 rows against 32768 keys, 32 heads: 160 us, 860
+// TFLOP/s of fp16 products; 64 rows 103 us.  Three or four K / V slots and two to four packed tiles in
+// flight measured alike; fewer registers for the softmax (184) cost 10 %.
 #include <algorithm>
 
 #include "attn_kv4.cuh"

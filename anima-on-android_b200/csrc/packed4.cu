@@ -20,8 +20,8 @@ namespace anima {
 // e_s the exponent of s), while products with an approximate 1 / s are off by less than 2^-19.  So
 // with t = saturate(x / (16 s) + 17/32 + 2^-18), the sum t (16 - 2^-14) + 2^23 - 1/2 rounds to
 // 2^23 + n + 8: at a border the bias leaves between 2^-18 and 2^-14 above it, and t = 1 gives 15.
-// (With a clamp on both sides, tests of every value and a true reciprocal this took 106 us for 132 M
-// values, bound by instructions; the floor is 52.)
+// 132 M bf16 values take 71 us (4.8 TB/s; 52 at the copy rate), bound by the integer pipe.  With tests
+// of every value, clamps on both sides and a true reciprocal they took 106.
 struct Quant4Params {
   const void* x;
   uint32_t* codes;
@@ -30,7 +30,6 @@ struct Quant4Params {
   long long s0, s1, s2;       // element strides of a, b, c
   long long units;            // rows * K / 8
   int upr;                    // units per row, K / 8
-  int contiguous;             // rows are K elements apart: unit u starts at 8 u
 };
 
 template <bool kBf16>
@@ -38,7 +37,7 @@ __device__ __forceinline__ float2 widen2(uint32_t w) {
   if (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-// Pairwise maximum; NaN wins.
+// Pairwise maximum and minimum; NaN wins.
 template <bool kBf16>
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -48,15 +47,25 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+template <bool kBf16>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (kBf16)
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
+template <bool kContiguous>
 __device__ __forceinline__ const uint4* unit_ptr(const Quant4Params& p, long long u) {
   const uint16_t* x = static_cast<const uint16_t*>(p.x);
-  if (p.contiguous) return reinterpret_cast<const uint4*>(x + 8 * u);
+  if (kContiguous) return reinterpret_cast<const uint4*>(x + 8 * u);
   const long long row = u / p.upr;
   const long long c = row % p.n2, ab = row / p.n2;
   return reinterpret_cast<const uint4*>(x + (ab / p.n1) * p.s0 + (ab % p.n1) * p.s1 + c * p.s2 +
@@ -68,7 +77,7 @@ __device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u
   constexpr uint32_t kSign = 0x80008000u;
   const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
   const uint32_t hi2 = max2<kBf16>(max2<kBf16>(v.x, v.y), max2<kBf16>(v.z, v.w));
-  const uint32_t lo2 = max2<kBf16>(max2<kBf16>(v.x ^ kSign, v.y ^ kSign), max2<kBf16>(v.z ^ kSign, v.w ^ kSign));
+  const uint32_t lo2 = min2<kBf16>(min2<kBf16>(v.x, v.y), min2<kBf16>(v.z, v.w)) ^ kSign;
   // (max x, max -x) of the eight values, then of the group
   uint32_t m = max2<kBf16>(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
   m = max2<kBf16>(m, __shfl_xor_sync(mask, m, 1));
@@ -106,16 +115,16 @@ __device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u
   if ((u & 3) == 0) p.scales[u >> 2] = s;
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kContiguous>
 __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
   // units is a multiple of 16, so the lanes of a group leave the loop together
   const long long step = (long long)gridDim.x * blockDim.x;
   for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < p.units; u += 2 * step) {
     const uint32_t mask = __activemask();
     const bool two = u + step < p.units;
-    const uint4 v0 = __ldg(unit_ptr(p, u));
+    const uint4 v0 = __ldg(unit_ptr<kContiguous>(p, u));
     uint4 v1 = make_uint4(0u, 0u, 0u, 0u);
-    if (two) v1 = __ldg(unit_ptr(p, u + step));
+    if (two) v1 = __ldg(unit_ptr<kContiguous>(p, u + step));
     quantize_unit<kBf16>(p, u, v0, mask);
     if (two) quantize_unit<kBf16>(p, u + step, v1, __activemask());
   }
@@ -123,8 +132,8 @@ __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
 
 // ---------------------------------------------------------------- unpacking
 // One lane per run of 8 values, in value order, so a warp's stores are one contiguous run (with
-// a lane per 16 bytes of codes, each store touched eight 64-byte pieces: 110 us against 57 for
-// 132 M values to bf16).  Value run v of a block (v = 4 g + i) is word 4 i + g of its codes.  n * s
+// a lane per 16 bytes of codes, each store touched eight 64-byte pieces: 110 us against 65 for
+// 132 M values to bf16, 5.2 TB/s).  Value run v of a block (v = 4 g + i) is word 4 i + g of its codes.  n * s
 // is exact in fp32 and rounded once.
 template <int kDt>
 __device__ __forceinline__ void store8(void* y, long long at, uint32_t w, float s) {
@@ -190,8 +199,13 @@ __global__ void __launch_bounds__(256)
 // number and written in four signed base-256 digits, so nothing above 2^-31 of the group's largest
 // magnitude is lost, more than an fp32 sum keeps.  A word's codes are its bytes' halves, c = n + 8, three
 // instructions for eight where bf16 takes eleven; the 8 goes into the accumulator's start value, -8
-// sum(digits), together with the 1.5 * 2^23 that makes the whole sum an fp32's low bits.  (As three
-// bf16 columns a row, 84 x 6144 x 256 with two rows took 24 us, bound by unpacking.)
+// sum(digits), together with the 1.5 * 2^23 that makes the whole sum an fp32's low bits.
+//
+// 84 matrices of 6144 x 256 with two fp32 rows take 19.6 us (4.0 TB/s of codes, scales and results; 12 at
+// the copy rate): 194 instructions a block of 16 x 128 weights at 0.65 a cycle and scheduler, of which
+// the tile's ends are a fifth with two blocks a row, and about 3 us of start, when x is staged.
+// As three bf16 columns a row, codes unpacked to bf16, they took 24.  One 6144 x 2048 matrix and row
+// takes 5.1 us, one 21504 x 2048 with SiLU and two rows 10.8.
 //
 // A CTA of 8 warps works on one matrix, on a run of tiles of 16 rows of W; `split` warps share a
 // tile, taking its 128-value blocks in turn, and their sums meet in shared memory in a fixed
@@ -564,12 +578,13 @@ int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long 
   p.s2 = s2;
   p.upr = K / 8;
   p.units = n0 * n1 * n2 * p.upr;
-  p.contiguous = (n2 == 1 || s2 == K) && (n1 == 1 || s1 == n2 * K) && (n0 == 1 || s0 == n1 * n2 * K);
+  // rows K elements apart: unit u starts at 8 u
+  const bool contiguous = (n2 == 1 || s2 == K) && (n1 == 1 || s1 == n2 * K) && (n0 == 1 || s0 == n1 * n2 * K);
   const int grid = stream_grid(p.units, 512, sm_count, 8);
   if (dtype == ANIMA_DTYPE_BF16)
-    quantize4_kernel<true><<<grid, 256, 0, st>>>(p);
+    (contiguous ? quantize4_kernel<true, true> : quantize4_kernel<true, false>)<<<grid, 256, 0, st>>>(p);
   else
-    quantize4_kernel<false><<<grid, 256, 0, st>>>(p);
+    (contiguous ? quantize4_kernel<false, true> : quantize4_kernel<false, false>)<<<grid, 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 

@@ -206,16 +206,11 @@ struct SmemAttr {
   SmemAttr() {
     for (auto& m : most) m.store(0);
   }
-  bool raise(const void* kern, size_t bytes, bool large_clusters = false) {
+  bool raise(const void* kern, size_t bytes) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
     if (bytes <= most[dev].load(std::memory_order_acquire)) return true;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-      cudaGetLastError();
-      return false;
-    }
-    if (large_clusters &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
       cudaGetLastError();
       return false;
     }
