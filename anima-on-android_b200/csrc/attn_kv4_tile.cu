@@ -666,15 +666,16 @@ __global__ void __launch_bounds__(256)
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float den = 0.f;
     for (int k = 0; k < nsplit; ++k) {
-      const float mk = mp[k * stride];
+      const float mk = mp[k * stride], lk = mp[k * stride + rows];
+      if (lk == 0.f) continue;  // a slice without keys, whose O may not be written
+      // only NaN scores leave the maximum at its start: their NaN sums come through
       const float f = mk == -INFINITY ? 0.f : ex2_approx(mk - M);
       const float4 o = *reinterpret_cast<const float4*>(base + k * stride + (long long)r * kD + lane * 4);
-      if (mk == -INFINITY) continue;  // a slice without keys, whose O is not written
       acc.x = fmaf(f, o.x, acc.x);
       acc.y = fmaf(f, o.y, acc.y);
       acc.z = fmaf(f, o.z, acc.z);
       acc.w = fmaf(f, o.w, acc.w);
-      den = fmaf(f, mp[k * stride + rows], den);
+      den = fmaf(f, lk, den);
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
     uint32_t w0, w1;

@@ -628,6 +628,81 @@ def test_attention_repeats_bit_for_bit(Sq):
         assert torch.equal(anima_attn.attention_core_kv4(q, k, v, 2, 2), first)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Sq,Skv,dtype", [(1, 2, 1, 60, F16), (1, 2, 5, 60, BF16), (1, 1, 1, 20011, BF16), (1, 1, 4, 20011, F16),
+                                              (1, 2, 40, 5000, F16), (1, 2, 200, 5000, BF16), (1, 4, 2000, 200, BF16),
+                                              (2, 16, 2400, 130, F16)])
+def test_attention_nan_reaches_its_rows_only(B, H, Sq, Skv, dtype):
+    """A NaN query value reaches its row; a NaN scale of a key or a value reaches its head (a value's: its
+    group's dims); nothing else changes.  Direct, in slices, by tiles and through the core."""
+    g = torch.Generator().manual_seed(13)
+    q = torch.randn(B * H, Sq, 128, generator=g).to(dtype).cuda()
+    k, v = (Packed4(*(t.expand(B * H, -1, -1).contiguous() for t in random_packed((1, Skv, 128), s)[0])) for s in (1, 2))
+    clean = anima_attn.attention_core_kv4(q, k, v, B, H)
+    assert clean.isfinite().all()
+    last = B * H - 1
+    q2 = q.clone()
+    q2[last, Sq - 1, 77] = float("nan")
+    got = anima_attn.attention_core_kv4(q2, k, v, B, H)
+    assert got[-1, -1, -1].isnan().all()
+    got[-1, -1, -1] = clean[-1, -1, -1]
+    assert torch.equal(got, clean)
+    for which in (0, 1):
+        bad = Packed4((k, v)[which].codes, (k, v)[which].scales.clone())
+        bad.scales[last, Skv // 2, 1] = float("nan")
+        got = anima_attn.attention_core_kv4(q, bad if which == 0 else k, bad if which == 1 else v, B, H)
+        hit = got[-1, :, -1] if which == 0 else got[-1, :, -1, 32:64]
+        assert hit.isnan().all()
+        (got[-1, :, -1] if which == 0 else got[-1, :, -1, 32:64]).copy_(clean[-1, :, -1] if which == 0 else clean[-1, :, -1, 32:64])
+        assert torch.equal(got, clean)
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 3, 20])
+def test_attention_offsets_past_32_bits(Sq):
+    H, Skv = 72, 480000  # 2.2 GB of codes each for K and V
+    g = torch.Generator(device="cuda").manual_seed(14)
+
+    def cache():
+        return Packed4(torch.randint(0, 256, (H, Skv, 64), dtype=torch.uint8, device="cuda", generator=g),
+                       (torch.rand(H, Skv, 4, device="cuda", generator=g) * 0.2 + 0.1).half())
+    k, v = cache(), cache()
+    q = torch.randn(H, Sq, 128, device="cuda", generator=g).half()
+    got = anima_attn.attention_core_kv4(q, k, v, 1, H)
+    for h in (0, H - 1):
+        kv, vv = (anima_attn.dequantize4(Packed4(t.codes[h:h + 1], t.scales[h:h + 1]), F32)[0].double() for t in (k, v))
+        p = torch.softmax(q[h].double() @ kv.T / math.sqrt(128), -1)
+        err, size = (got[0, :, h].double() - p @ vv).abs(), p @ vv.abs()
+        assert (err <= 2.0 ** -11 * (p @ vv).abs() + 2.0 ** -9 * size + 6e-8).all()  # far inside a misread
+
+
+@pytest.mark.gpu
+def test_matvec_and_packing_offsets_past_32_bits():
+    E, N, K = 3, 100000, 16384  # 2.4 GB of codes
+    g = torch.Generator(device="cuda").manual_seed(15)
+    w = Packed4(torch.randint(0, 256, (E, N, K // 2), dtype=torch.uint8, device="cuda", generator=g),
+                (torch.rand(E, N, K // 32, device="cuda", generator=g) * 0.01).half())
+    x = torch.randn(E, 1, K, device="cuda", generator=g)
+    y = anima_attn.matvec4(x, w)
+    for e, n in ((0, 0), (E - 1, N - 40)):
+        wv = anima_attn.dequantize4(Packed4(w.codes[e, n:n + 40], w.scales[e, n:n + 40]), F32).double()
+        want = (wv @ x[e, 0].double()).cpu().numpy()
+        tol = matvec_bound(x[e].abs().double().cpu().numpy(), wv.abs().cpu().numpy(), K, want, F32, False)[0]
+        assert (np.abs(y[e, 0, n:n + 40].double().cpu().numpy() - want) <= tol).all()
+    del w, y
+    rows = (1 << 31) // 128 + 37  # more than 2^31 values
+    big = torch.empty(rows, 128, dtype=F16, device="cuda")
+    big[:] = torch.randn(1, 128, device="cuda", generator=g).half()
+    tail = torch.randn(64, 128, device="cuda", generator=g).half()
+    big[-64:] = tail
+    p = anima_attn.quantize4(big)
+    want = anima_attn.quantize4(tail)
+    assert torch.equal(p.codes[-64:], want.codes) and torch.equal(p.scales[-64:], want.scales)
+    back = anima_attn.dequantize4(p)
+    assert torch.equal(back[-64:], anima_attn.dequantize4(want)) and torch.equal(back[:1], back[rows // 2:rows // 2 + 1])
+
+
 # ------------------------------------------------------------------ as they are used
 @pytest.mark.gpu
 def test_streams_and_graphs():
