@@ -67,7 +67,7 @@ def _check_packed(p: Packed4, what: str) -> torch.Size:
     if c.dtype is not _U8 or s.dtype is not _F16 or not c.is_contiguous() or not s.is_contiguous():
         raise ValueError(f"{what}: packed codes are contiguous uint8, scales contiguous float16")
     cs, ss = c.shape, s.shape
-    half = cs[-1]
+    half = cs[-1] if cs and ss else 0
     if half == 0 or half % 64 or ss[-1] * 16 != half or cs[:-1] != ss[:-1]:
         raise ValueError(f"{what}: codes [..., K/2] and scales [..., K/32], K a multiple of 128")
     return cs
@@ -76,6 +76,11 @@ def _check_packed(p: Packed4, what: str) -> torch.Size:
 @lru_cache(maxsize=1024)
 def _kv4_workspace(dev: int, dtype: torch.dtype, B: int, H: int, Sq: int, Skv: int) -> int:
     return int(L.lib.anima_attn_kv4_workspace_size(_TORCH_DT[dtype], B, H, Sq, Skv))
+
+
+def _repeats(t: torch.Tensor) -> bool:
+    """Whether an axis of a tensor to be written repeats the same memory (an expanded view)."""
+    return 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride()))
 
 
 def _row_strides(x: torch.Tensor) -> Optional[list]:
@@ -157,9 +162,10 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     w [N, K] with x [M, K] or [K]; or a stack w [E, N, K] with x [E, M, K].  x is float32,
     float16 or bfloat16 with a contiguous last axis (other strides are free); ``add`` is float32
     and broadcasts to the result [.., M, N] over its leading axes; the result has ``out``'s or
-    ``out_dtype``'s type.  Sums are fp32 over exact products and fp32 x keeps its 24 bits, so
-    the result is an fp32 one rounded once.  8 float32 rows or 16 16-bit ones share a
-    pass over W."""
+    ``out_dtype``'s type; ``out`` may be ``add`` itself, and overlaps no other operand.  Sums are
+    fp32 over exact products, and of float32 x only what is below 2^-31 of its group's largest
+    is lost, so the result is an fp32 one rounded once.  8 float32 rows or 16 16-bit ones
+    share a pass over W."""
     stream = _here(x, add, out, *w)
     ws = _check_packed(w, "w")
     K = 2 * ws[-1]
@@ -182,8 +188,8 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
         if out_dtype not in _TORCH_DT:
             raise ValueError("out_dtype must be float32, float16 or bfloat16")
         out = x.new_empty(shape, dtype=out_dtype)
-    elif out.shape != shape or out.dtype not in _TORCH_DT or (N > 1 and out.stride(-1) != 1):
-        raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous")
+    elif out.shape != shape or out.dtype not in _TORCH_DT or (N > 1 and out.stride(-1) != 1) or _repeats(out):
+        raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous, none repeated")
     ostr = out.stride()
     oe, om = ((0, 0) if len(shape) == 1 else (0, ostr[0])) if len(ws) == 2 else (ostr[0], ostr[1])
     aptr = ae = am = 0
@@ -214,9 +220,9 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     S_q, 128].  ``kv_valid_len`` int32 [B]: keys at or past it do not count, whatever the
     cache holds there; a sample without any has zero rows.
 
-    Few query rows read the packed cache directly, with fp32 accuracy up to the output's rounding;
-    more rows unpack K and V once into 16-bit scratch of this call and run the attention
-    core (anima_attn_kv4_fwd)."""
+    ``out`` overlaps no operand.  Few query rows have fp32 accuracy up to the output's rounding;
+    many run on fp16 operands (unpacked K and V, probabilities), whose products are summed in
+    fp32 (anima_attn_kv4_fwd)."""
     stream = _here(q, kv_valid_len, out, *k, *v)
     if q.dim() != 3 or q.dtype not in _HALF or not q.is_contiguous():
         raise ValueError("q must be [B*H, S_q, 128], contiguous, float16 or bfloat16")
@@ -232,8 +238,8 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     shape = (B, Sq, H, D) if out_layout == "bshd" else (B, H, Sq, D)
     if out is None:
         out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
-        raise ValueError("out must have q's type, the layout's shape and a contiguous head dimension")
+    elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1 or _repeats(out):
+        raise ValueError("out must have q's type, the layout's shape, a contiguous head dimension and no repeated axis")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")

@@ -1096,6 +1096,8 @@ static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintp
 static bool any_dtype(int d) {
   return d == ANIMA_DTYPE_F32 || d == ANIMA_DTYPE_F16 || d == ANIMA_DTYPE_BF16;
 }
+// Counts of rows that the kernels step past by a tile or a round in 32 bits.
+constexpr int kMaxRows4 = 1 << 30;
 // Rows of K values within 2^46 values, so that no offset of a call passes 64 bits.
 static bool rows_fit(long long a, long long b, long long c, int K) {
   const double n = (double)a * (double)b * (double)c * (double)K;
@@ -1138,7 +1140,7 @@ int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype,
 int anima_matvec4(const AnimaMatvec4Args* a, void* stream) {
   if (!a || !any_dtype(a->x_dtype) || !any_dtype(a->out_dtype)) return ANIMA_ERR_ARG;
   if (a->E < 0 || a->M < 0 || a->N < 0 || a->K <= 0 || a->K % 128 || a->K > ANIMA_MATVEC4_MAX_K ||
-      !rows_fit(a->E, a->N, 1, a->K))
+      a->N > kMaxRows4 || !rows_fit(a->E, a->N, 1, a->K))
     return ANIMA_ERR_SHAPE;
   if (a->E == 0 || a->M == 0 || a->N == 0) return ANIMA_OK;
   if (!a->x || !a->codes || !a->scales || !a->out || !al16(a->codes) || !aligned(a->scales, 8))
@@ -1165,7 +1167,7 @@ int anima_attn_kv4_fwd(const AnimaAttnKv4Args* a, void* stream) {
       !aligned(a->k_scales, 8) || !aligned(a->v_scales, 8) || !aligned(a->workspace, 256))
     return ANIMA_ERR_ARG;
   if (a->D != 128 || a->B <= 0 || a->H <= 0 || a->S_q <= 0 || a->S_kv <= 0 ||
-      (long long)a->B * a->H > 0x7fffffffLL || !rows_fit((long long)a->B * a->H, a->S_kv, 1, 128) ||
+      a->S_q > kMaxRows4 || a->S_kv > kMaxRows4 || (long long)a->B * a->H > 0x7fffffffLL || !rows_fit((long long)a->B * a->H, a->S_kv, 1, 128) ||
       !rows_fit((long long)a->B * a->H, a->S_q, 1, 128))
     return ANIMA_ERR_SHAPE;
   int rc = ANIMA_OK;
@@ -1178,7 +1180,9 @@ int anima_attn_kv4_fwd(const AnimaAttnKv4Args* a, void* stream) {
 uint64_t anima_attn_kv4_workspace_size(int dtype, int B, int H, int S_q, int S_kv) {
   int rc = ANIMA_OK;
   DeviceState* d = current_device(&rc);
-  if (!d || B <= 0 || H <= 0 || S_q <= 0 || S_kv <= 0 || (long long)B * H > 0x7fffffffLL) return 0;
+  if (!d || B <= 0 || H <= 0 || S_q <= 0 || S_kv <= 0 || S_q > kMaxRows4 || S_kv > kMaxRows4 ||
+      (long long)B * H > 0x7fffffffLL)
+    return 0;
   return attn_kv4_workspace_bytes(dtype, B, H, S_q, S_kv, d->sm_count);
 }
 

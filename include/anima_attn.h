@@ -330,10 +330,12 @@ int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype,
  *   out[e, m, n] = sum_k f(x[e, m, k]) W[e, n, k] + add[e, m, n],  f = SiLU if silu, else x.
  * W: packed rows [E, N] of K values.  x, add (fp32, or NULL) and out are addressed by element
  * strides {e, m} (0 repeats), their last axis contiguous; x and out F32, F16 or BF16.  The
- * products are exact, sums are fp32; fp32 rows (and SiLU of any) enter as three bf16 parts
- * (magnitudes up to 3.38e38), so the result has fp32 accuracy before its one rounding.
- * Up to 8 fp32 or 16 16-bit rows share one pass over W; more rows take further passes.  K up
- * to ANIMA_MATVEC4_MAX_K.  E, M or N = 0 does nothing.  Asynchronous on `stream`.
+ * products are exact, sums are fp32; fp32 rows (and SiLU of any) enter as whole numbers below
+ * 2^30, one scale per group of 32 (values below 2^-31 of the group's largest count as 0), so the
+ * result has fp32 accuracy before its one rounding.  One infinity in a group of x gives what
+ * it should, several give NaN.  Up to 8 fp32 or 16 16-bit rows share one pass over W; more rows
+ * take further passes.  K up to ANIMA_MATVEC4_MAX_K, N up to 2^30.  E, M or N = 0 does nothing.
+ * out may be add at the same strides, else it overlaps no operand.  Asynchronous on `stream`.
  */
 #define ANIMA_MATVEC4_MAX_K 32768
 typedef struct AnimaMatvec4Args {
@@ -356,12 +358,14 @@ int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
 /*
  * Attention over packed K and V: anima_attn_fwd with k/v [B*H, S_kv] packed rows of D = 128.
  * q [B*H, S_q, 128] contiguous and out (strides {b, h, s} as in anima_attn_fwd, multiples of
- * 8) are of dtype (F16 or BF16); scale is positive.  flags: ANIMA_FLAG_MASK with kv_valid_len (keys at or past it
- * are not read or do not count, whatever is stored there; none left gives zero rows).
- * Calls of few query rows read the packed rows directly and have fp32 accuracy up to the output's
- * rounding; others unpack K and V into `workspace` (anima_attn_kv4_workspace_size bytes,
- * 256-byte aligned, contents irrelevant; 0 for few rows) and run the attention core on them.
- * Calls that share a workspace must be ordered.  Asynchronous on `stream`.
+ * 8) are of dtype (F16 or BF16), out overlapping no operand; scale is positive; S_q and S_kv go
+ * up to 2^30.  flags: ANIMA_FLAG_MASK with kv_valid_len (keys at or past it are not read or do
+ * not count, whatever is stored there; none left gives zero rows).
+ * Little work reads the packed rows directly and has fp32 accuracy up to the output's rounding.
+ * More runs on the tensor cores with fp16 operands (K and V, which are to be in fp16's range as
+ * anima_quantize4 leaves them, and the probabilities); very many fp16 rows unpack K and V first.
+ * `workspace`: anima_attn_kv4_workspace_size bytes (0 for some calls), 256-byte aligned, contents
+ * irrelevant; calls that share one must be ordered.  Asynchronous on `stream`.
  */
 typedef struct AnimaAttnKv4Args {
   const void* q;

@@ -119,7 +119,7 @@ def _mv(**kw):
 @pytest.mark.parametrize("kw,want", [
     (dict(x_dtype=5), L.ERR_ARG), (dict(out_dtype=-1), L.ERR_ARG), (dict(K=192), L.ERR_SHAPE),
     (dict(K=0), L.ERR_SHAPE), (dict(K=32768 + 128), L.ERR_SHAPE), (dict(M=-1), L.ERR_SHAPE),
-    (dict(E=1 << 30, N=1 << 30), L.ERR_SHAPE), (dict(x=None), L.ERR_ARG), (dict(out=None), L.ERR_ARG),
+    (dict(E=1 << 30, N=1 << 30), L.ERR_SHAPE), (dict(N=(1 << 31) - 5), L.ERR_SHAPE), (dict(x=None), L.ERR_ARG), (dict(out=None), L.ERR_ARG),
     (dict(codes=A + 4), L.ERR_ARG), (dict(scales=A + 2), L.ERR_ARG), (dict(add=A + 2), L.ERR_ARG),
     (dict(x=A + 2), L.ERR_ARG), (dict(N=0, x=None), L.OK), (dict(M=0), L.OK), (dict(E=0), L.OK)])
 def test_matvec_refusals(kw, want):
@@ -145,7 +145,8 @@ def _attn(**kw):
     (dict(scale=math.nan), L.ERR_ARG), (dict(flags=L.FLAG_CAUSAL), L.ERR_ARG), (dict(out_stride=(128, 128, 4)), L.ERR_ARG),
     (dict(out_stride=(-128, 128, 128)), L.ERR_ARG), (dict(q=A + 8), L.ERR_ARG), (dict(out=A + 8), L.ERR_ARG),
     (dict(k_codes=A + 8), L.ERR_ARG), (dict(k_scales=A + 4), L.ERR_ARG), (dict(workspace=A + 64), L.ERR_ARG),
-    (dict(B=1 << 20, H=1 << 20), L.ERR_SHAPE)])
+    (dict(B=1 << 20, H=1 << 20), L.ERR_SHAPE), (dict(S_q=(1 << 31) - 1), L.ERR_SHAPE),
+    (dict(S_kv=(1 << 30) + 1), L.ERR_SHAPE)])
 def test_attention_refusals(kw, want):
     assert _attn(**kw) == want
     assert L.lib.anima_attn_kv4_fwd(None, None) == L.ERR_ARG
@@ -196,12 +197,17 @@ def test_python_refusals(any_device):
         anima_attn.dequantize4(Packed4(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(3, 4, dtype=F16)))
     with bad:
         anima_attn.dequantize4(Packed4(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 4, dtype=F16)))
+    with bad:
+        anima_attn.dequantize4(Packed4(torch.zeros((), dtype=torch.uint8), torch.zeros((), dtype=F16)))
+    with bad:
+        anima_attn.dequantize4(Packed4(torch.zeros(64, dtype=torch.uint8), torch.zeros((), dtype=F16)))
     w, ws = _pk(32, 256), _pk(3, 32, 256)
     for x, p, kw in ((torch.zeros(2, 128), w, {}), (torch.zeros(2, 2, 256), w, {}), (torch.zeros(2, 256), ws, {}),
                      (torch.zeros(2, 2, 256), ws, {}), (torch.zeros(2, 256, dtype=torch.float64), w, {}),
                      (torch.zeros(256, 2).t(), w, {}), (torch.zeros(2, 256), w, {"out_dtype": torch.float64}),
                      (torch.zeros(2, 256), w, {"out": torch.zeros(2, 31)}),
                      (torch.zeros(2, 256), w, {"out": torch.zeros(32, 2).t()}),
+                     (torch.zeros(2, 256), w, {"out": torch.zeros(32).expand(2, 32)}),
                      (torch.zeros(2, 256), w, {"add": torch.zeros(3, 32)}),
                      (torch.zeros(2, 256), w, {"add": torch.zeros(2, 1)}),
                      (torch.zeros(2, 256), w, {"add": torch.zeros(32, dtype=F16)})):
@@ -212,6 +218,7 @@ def test_python_refusals(any_device):
                   ((q, k, _pk(4, 6, 128), 2, 2), {}), ((q, _pk(4, 0, 128), _pk(4, 0, 128), 2, 2), {}),
                   ((q.transpose(0, 1), k, k, 2, 2), {}), ((q, k, k, 2, 2), {"out_layout": "sbhd"}),
                   ((q, k, k, 2, 2), {"out": torch.zeros(2, 3, 2, 128)}),
+                  ((q, k, k, 2, 2), {"out": torch.zeros(2, 1, 2, 128, dtype=F16).expand(2, 3, 2, 128)}),
                   ((q, k, k, 2, 2), {"kv_valid_len": torch.zeros(3)}),
                   ((q, k, k, 2, 2), {"scale": 0.0}), ((q, k, k, 2, 2), {"scale": -0.3}),
                   ((q, k, k, 2, 2), {"scale": math.nan})):
