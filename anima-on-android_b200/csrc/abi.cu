@@ -74,7 +74,7 @@ int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long 
                      long long s0, long long s1, long long s2, int K, void* codes, void* scales,
                      int sm_count, cudaStream_t st);
 int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype, long long rows,
-                       int K, int sm_count, cudaStream_t st);
+                       int K, cudaStream_t st);
 int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st);
 int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st);
 size_t attn_kv4_workspace_bytes(int dtype, int B, int H, int S_q, int S_kv, int sm_count);
@@ -1132,7 +1132,7 @@ int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype,
   int rc = ANIMA_OK;
   DeviceState* d = current_device(&rc);
   if (!d) return rc;
-  return done4(dequantize4_launch(codes, scales, y, dtype, rows, K, d->sm_count,
+  return done4(dequantize4_launch(codes, scales, y, dtype, rows, K,
                                   static_cast<cudaStream_t>(stream)),
                "anima_dequantize4");
 }

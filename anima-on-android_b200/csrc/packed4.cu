@@ -20,8 +20,8 @@ namespace anima {
 // e_s the exponent of s), while products with an approximate 1 / s are off by less than 2^-19.  So
 // with t = saturate(x / (16 s) + 17/32 + 2^-18), the sum t (16 - 2^-14) + 2^23 - 1/2 rounds to
 // 2^23 + n + 8: at a border the bias leaves between 2^-18 and 2^-14 above it, and t = 1 gives 15.
-// 132 M bf16 values take 71 us (4.8 TB/s; 52 at the copy rate), bound by the integer pipe.  With tests
-// of every value, clamps on both sides and a true reciprocal they took 106.
+// 132 M bf16 values take 61 us (5.6 TB/s; 52 at the copy rate), bound by the integer pipe.  With tests
+// of every value, clamps on both sides and a true reciprocal they took 106 (at 71 otherwise).
 struct Quant4Params {
   const void* x;
   uint32_t* codes;
@@ -118,22 +118,23 @@ __device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u
 template <bool kBf16, bool kContiguous>
 __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
   // units is a multiple of 16, so the lanes of a group leave the loop together
-  const long long step = (long long)gridDim.x * blockDim.x;
-  for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < p.units; u += 2 * step) {
+  constexpr int kStep = 256;  // a block takes runs of 512 units (rounds spread over the grid: 65 us against 61)
+  const long long first = (long long)blockIdx.x * (2 * kStep) + threadIdx.x;
+  for (long long u = first; u < p.units; u += (long long)gridDim.x * (2 * kStep)) {
     const uint32_t mask = __activemask();
-    const bool two = u + step < p.units;
+    const bool two = u + kStep < p.units;
     const uint4 v0 = __ldg(unit_ptr<kContiguous>(p, u));
     uint4 v1 = make_uint4(0u, 0u, 0u, 0u);
-    if (two) v1 = __ldg(unit_ptr<kContiguous>(p, u + step));
+    if (two) v1 = __ldg(unit_ptr<kContiguous>(p, u + kStep));
     quantize_unit<kBf16>(p, u, v0, mask);
-    if (two) quantize_unit<kBf16>(p, u + step, v1, __activemask());
+    if (two) quantize_unit<kBf16>(p, u + kStep, v1, __activemask());
   }
 }
 
 // ---------------------------------------------------------------- unpacking
 // One lane per run of 8 values, in value order, so a warp's stores are one contiguous run (with
 // a lane per 16 bytes of codes, each store touched eight 64-byte pieces: 110 us against 65 for
-// 132 M values to bf16, 5.2 TB/s).  Value run v of a block (v = 4 g + i) is word 4 i + g of its codes.  n * s
+// 132 M values to bf16; now 56, 6.0 TB/s).  Value run v of a block (v = 4 g + i) is word 4 i + g of its codes.  n * s
 // is exact in fp32 and rounded once.
 template <int kDt>
 __device__ __forceinline__ void store8(void* y, long long at, uint32_t w, float s) {
@@ -160,13 +161,18 @@ __device__ __forceinline__ void store8(void* y, long long at, uint32_t w, float 
   }
 }
 
+// Runs per lane and round, loaded before any is converted (132 M values: bf16 in 56 us with four, 58 with
+// two, 80 with one; fp32 in 139 with four, 128 with two).
+__host__ __device__ constexpr int deq_runs(int dtype) { return dtype == ANIMA_DTYPE_F32 ? 2 : 4; }
+
 template <int kDt>
 __global__ void __launch_bounds__(256)
     dequantize4_kernel(const uint32_t* __restrict__ codes, const __half* __restrict__ scales, void* y,
                        long long words) {
-  constexpr int kU = 4;  // runs per lane and round, loaded before any is converted
-  const long long step = (long long)gridDim.x * blockDim.x;
-  for (long long u0 = (long long)blockIdx.x * blockDim.x + threadIdx.x; u0 < words; u0 += kU * step) {
+  constexpr int kU = deq_runs(kDt);
+  constexpr int step = 256;
+  const long long first = (long long)blockIdx.x * (kU * step) + threadIdx.x;
+  for (long long u0 = first; u0 < words; u0 += (long long)gridDim.x * (kU * step)) {
     uint32_t w[kU];
     __half s[kU];
 #pragma unroll
@@ -559,9 +565,10 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
 }
 
 // ---------------------------------------------------------------- launchers
-static int stream_grid(long long work, int per_block, int sm_count, int waves) {
-  const long long g = (work + per_block - 1) / per_block, cap = (long long)sm_count * waves;
-  return (int)(g < 1 ? 1 : g > cap ? cap : g);
+// Blocks of a streaming kernel that takes one round each.  132 M values (bf16) unpack in 56 us so, 59 with
+// 32 blocks an SM and 65 with 8; packing is capped at 64 blocks an SM: 61 us, 68 without, 71 with 8.
+static int stream_grid(long long work, int per_block) {
+  return (int)std::min<long long>((work + per_block - 1) / per_block, 1 << 30);
 }
 
 int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long long n2,
@@ -580,7 +587,7 @@ int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long 
   p.units = n0 * n1 * n2 * p.upr;
   // rows K elements apart: unit u starts at 8 u
   const bool contiguous = (n2 == 1 || s2 == K) && (n1 == 1 || s1 == n2 * K) && (n0 == 1 || s0 == n1 * n2 * K);
-  const int grid = stream_grid(p.units, 512, sm_count, 8);
+  const int grid = std::min(64 * sm_count, stream_grid(p.units, 512));
   if (dtype == ANIMA_DTYPE_BF16)
     (contiguous ? quantize4_kernel<true, true> : quantize4_kernel<true, false>)<<<grid, 256, 0, st>>>(p);
   else
@@ -589,9 +596,9 @@ int quantize4_launch(const void* x, int dtype, long long n0, long long n1, long 
 }
 
 int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype, long long rows,
-                       int K, int sm_count, cudaStream_t st) {
+                       int K, cudaStream_t st) {
   const long long words = rows * (K / 8);
-  const int grid = stream_grid(words, 1024, sm_count, 8);
+  const int grid = stream_grid(words, 256 * deq_runs(dtype));
   const uint32_t* c = static_cast<const uint32_t*>(codes);
   const __half* s = static_cast<const __half*>(scales);
   if (dtype == ANIMA_DTYPE_F32)
