@@ -31,7 +31,10 @@ _MATVEC_ARGS = struct.Struct("@Pi2qPPP2qPi2qiiiii0q")
 _ATTN_ARGS = struct.Struct("@PPPPPiP3qiiiiifIPPQ")
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current = getattr(torch._C, "_cuda_getDevice", None)
-_U8, _F16 = torch.uint8, torch.float16
+_U8, _F16, _F32 = torch.uint8, torch.float16, torch.float32
+_quantize, _dequantize = L.lib.anima_quantize4, L.lib.anima_dequantize4
+_matvec, _attn = L.lib.anima_matvec4, L.lib.anima_attn_kv4_fwd
+_SCALE = 1.0 / math.sqrt(128)
 
 
 class Packed4(NamedTuple):
@@ -61,12 +64,11 @@ def _here(t, *ts) -> int:
     return _raw_stream(dev)
 
 
-def _check_packed(p: Packed4, what: str) -> torch.Size:
+def _check_packed(c: torch.Tensor, s: torch.Tensor, what: str) -> tuple:
     """The codes' shape [..., K/2], after checking that codes and scales belong together."""
-    c, s = p
     if c.dtype is not _U8 or s.dtype is not _F16 or not c.is_contiguous() or not s.is_contiguous():
         raise ValueError(f"{what}: packed codes are contiguous uint8, scales contiguous float16")
-    cs, ss = c.shape, s.shape
+    cs, ss = tuple(c.shape), tuple(s.shape)
     half = cs[-1] if cs and ss else 0
     if half == 0 or half % 64 or ss[-1] * 16 != half or cs[:-1] != ss[:-1]:
         raise ValueError(f"{what}: codes [..., K/2] and scales [..., K/32], K a multiple of 128")
@@ -107,15 +109,18 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
     stream = _here(x)
     if x.dtype not in _HALF:
         raise ValueError("x must be float16 or bfloat16")
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 128:
+    shape = tuple(x.shape)
+    K = shape[-1] if shape else 0
+    if K == 0 or K % 128:
         raise ValueError("the last axis must be a positive multiple of 128")
-    K, lead = x.shape[-1], x.shape[:-1]
+    lead = shape[:-1]
     if out is None:
-        out = Packed4(x.new_empty(lead + (K // 2,), dtype=_U8), x.new_empty(lead + (K // 32,), dtype=_F16))
+        codes, scales = x.new_empty(lead + (K // 2,), dtype=_U8), x.new_empty(lead + (K // 32,), dtype=_F16)
+        out = Packed4(codes, scales)
     else:
-        _here(*out)
-        _check_packed(out, "out")
-        if out.codes.shape != lead + (K // 2,):
+        codes, scales = out
+        _here(x, codes, scales)
+        if _check_packed(codes, scales, "out") != lead + (K // 2,):
             raise ValueError("out must be packed with x's shape")
     n = x.numel()
     if n == 0:
@@ -129,10 +134,10 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
         if x.stride(-1) != 1 or axes is None or any(s % 8 for _, s in axes):
             raise ValueError("x needs a contiguous last axis and at most three row strides, all multiples of 8")
         (n0, s0), (n1, s1), (n2, s2) = axes
-    if x.data_ptr() % 16:
+    xp = x.data_ptr()
+    if xp % 16:
         raise ValueError("x must be 16-byte aligned")
-    rc = L.lib.anima_quantize4(x.data_ptr(), _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K,
-                               out.codes.data_ptr(), out.scales.data_ptr(), stream)
+    rc = _quantize(xp, _TORCH_DT[x.dtype], n0, n1, n2, s0, s1, s2, K, codes.data_ptr(), scales.data_ptr(), stream)
     if rc:
         L.check(rc, "anima_quantize4")
     return out
@@ -141,14 +146,15 @@ def quantize4(x: torch.Tensor, out: Optional[Packed4] = None) -> Packed4:
 def dequantize4(p: Packed4, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values [..., K] that a packed tensor stands for: exact in float32, rounded once in
     float16 and bfloat16."""
-    stream = _here(*p)
-    cs = _check_packed(p, "p")
-    if dtype not in _TORCH_DT:
+    codes, scales = p
+    stream = _here(codes, scales)
+    cs = _check_packed(codes, scales, "p")
+    dt = _TORCH_DT.get(dtype)
+    if dt is None:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     K = 2 * cs[-1]
-    y = p.scales.new_empty(cs[:-1] + (K,), dtype=dtype)
-    rc = L.lib.anima_dequantize4(p.codes.data_ptr(), p.scales.data_ptr(), y.data_ptr(),
-                                 _TORCH_DT[dtype], y.numel() // K, K, stream)
+    y = scales.new_empty(cs[:-1] + (K,), dtype=dtype)
+    rc = _dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), dt, y.numel() // K, K, stream)
     if rc:
         L.check(rc, "anima_dequantize4")
     return y
@@ -166,45 +172,51 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     fp32 over exact products, and of float32 x only what is below 2^-31 of its group's largest
     is lost, so the result is an fp32 one rounded once.  8 float32 rows or 16 16-bit ones
     share a pass over W."""
-    stream = _here(x, add, out, *w)
-    ws = _check_packed(w, "w")
-    K = 2 * ws[-1]
-    if x.dtype not in _TORCH_DT:
+    codes, scales = w
+    stream = _here(x, codes, scales, add, out)
+    ws, xs, xst = _check_packed(codes, scales, "w"), tuple(x.shape), x.stride()
+    K, nd = 2 * ws[-1], len(xs)
+    xdt = _TORCH_DT.get(x.dtype)
+    if xdt is None:
         raise ValueError("x must be float32, float16 or bfloat16")
-    if len(ws) == 2 and x.dim() in (1, 2):
-        E, xv = 1, x if x.dim() == 2 else x.unsqueeze(0)
-        M, xe, xm = xv.shape[0], 0, xv.stride(0)
-    elif len(ws) == 3 and x.dim() == 3 and x.shape[0] == ws[0]:
-        E, M, xe, xm = ws[0], x.shape[1], x.stride(0), x.stride(1)
+    E, M, xe, xm = 1, 1, 0, 0
+    if len(ws) == 2 and (nd == 2 or nd == 1):
+        if nd == 2:
+            M, xm = xs[0], xst[0]
+    elif len(ws) == 3 and nd == 3 and xs[0] == ws[0]:
+        E, M, _ = xs
+        xe, xm, _ = xst
     else:
         raise ValueError("w [N, K] takes x [M, K] or [K]; w [E, N, K] takes x [E, M, K]")
     N = ws[-2]
-    if x.shape[-1] != K or x.stride(-1) != 1:
+    if xs[-1] != K or xst[-1] != 1:
         raise ValueError(f"x needs a contiguous last axis of K = {K}")
     if K > 32768:
         raise ValueError("K must be at most 32768")
-    shape = x.shape[:-1] + (N,)
+    shape = xs[:-1] + (N,)
     if out is None:
-        if out_dtype not in _TORCH_DT:
+        odt = _TORCH_DT.get(out_dtype)
+        if odt is None:
             raise ValueError("out_dtype must be float32, float16 or bfloat16")
         out = x.new_empty(shape, dtype=out_dtype)
-    elif out.shape != shape or out.dtype not in _TORCH_DT or (N > 1 and out.stride(-1) != 1) or _repeats(out):
-        raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous, none repeated")
-    ostr = out.stride()
-    oe, om = ((0, 0) if len(shape) == 1 else (0, ostr[0])) if len(ws) == 2 else (ostr[0], ostr[1])
+        oe, om = M * N, N
+    else:
+        odt = _TORCH_DT.get(out.dtype)
+        if tuple(out.shape) != shape or odt is None or (N > 1 and out.stride(-1) != 1) or _repeats(out):
+            raise ValueError("out must be float32, float16 or bfloat16 of the result's shape, its last axis contiguous, none repeated")
+        oe, om, _ = ((0, 0) + out.stride())[-3:]
     aptr = ae = am = 0
     if add is not None:
-        if add.dtype != torch.float32 or (N > 1 and (add.dim() == 0 or add.shape[-1] != N or add.stride(-1) != 1)):
+        ash, ast, na = tuple(add.shape), add.stride(), add.dim()
+        if add.dtype is not _F32 or (N > 1 and (na == 0 or ash[-1] != N or ast[-1] != 1)):
             raise ValueError("add must be float32 with a contiguous last axis of N values")
-        try:
-            av = add.expand(E, M, N)
-        except RuntimeError:
-            raise ValueError("add must broadcast to the result") from None
-        aptr, (ae, am, _) = av.data_ptr(), av.stride()
-    a = _MATVEC_ARGS.pack(x.data_ptr(), _TORCH_DT[x.dtype], xe, xm, w.codes.data_ptr(),
-                          w.scales.data_ptr(), aptr, ae, am, out.data_ptr(), _TORCH_DT[out.dtype],
-                          oe, om, E, M, N, K, 1 if silu else 0)
-    rc = L.lib.anima_matvec4(a, stream)
+        (ne, nm, nn), (ae, am, _) = ((1, 1, 1) + ash)[na:], ((0, 0, 0) + ast)[na:]
+        if na > 3 or (ne != E and ne != 1) or (nm != M and nm != 1) or nn != N:
+            raise ValueError("add must broadcast to the result")
+        aptr, ae, am = add.data_ptr(), (0 if ne == 1 else ae), (0 if nm == 1 else am)
+    a = _MATVEC_ARGS.pack(x.data_ptr(), xdt, xe, xm, codes.data_ptr(), scales.data_ptr(), aptr, ae, am,
+                          out.data_ptr(), odt, oe, om, E, M, N, K, 1 if silu else 0)
+    rc = _matvec(a, stream)
     if rc:
         L.check(rc, "anima_matvec4")
     return out
@@ -223,44 +235,51 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     ``out`` overlaps no operand.  Few query rows have fp32 accuracy up to the output's rounding;
     many run on fp16 operands (unpacked K and V, probabilities), whose products are summed in
     fp32 (anima_attn_kv4_fwd)."""
-    stream = _here(q, kv_valid_len, out, *k, *v)
-    if q.dim() != 3 or q.dtype not in _HALF or not q.is_contiguous():
+    kc, ks = k
+    vc, vs = v
+    stream = _here(q, kc, ks, vc, vs, kv_valid_len, out)
+    qs, qdt = tuple(q.shape), q.dtype
+    if len(qs) != 3 or qdt not in _HALF or not q.is_contiguous():
         raise ValueError("q must be [B*H, S_q, 128], contiguous, float16 or bfloat16")
-    BH, Sq, D = q.shape
+    BH, Sq, D = qs
     if BH != B * H or D != 128 or BH == 0 or Sq == 0:
         raise ValueError("q must be [B*H, S_q, 128] with at least one row")
-    ks = _check_packed(k, "k")
-    if ks != _check_packed(v, "v") or len(ks) != 3 or ks[0] != BH or ks[1] == 0 or ks[2] != 64:
+    cs = _check_packed(kc, ks, "k")
+    if cs != _check_packed(vc, vs, "v") or len(cs) != 3 or cs[0] != BH or cs[1] == 0 or cs[2] != 64:
         raise ValueError("k and v must be packed [B*H, S_kv, 128] with at least one key")
-    Skv = ks[1]
-    if out_layout not in ("bshd", "bhsd"):
+    Skv = cs[1]
+    if out_layout == "bshd":
+        shape = (B, Sq, H, D)
+    elif out_layout == "bhsd":
+        shape = (B, H, Sq, D)
+    else:
         raise ValueError("out_layout must be 'bshd' or 'bhsd'")
-    shape = (B, Sq, H, D) if out_layout == "bshd" else (B, H, Sq, D)
     if out is None:
         out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1 or _repeats(out):
-        raise ValueError("out must have q's type, the layout's shape, a contiguous head dimension and no repeated axis")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+        ob, s1, s2, _ = out.stride()
+    else:
+        ob, s1, s2, sd = out.stride() if out.dim() == 4 else (0, 0, 0, 0)
+        if tuple(out.shape) != shape or out.dtype is not qdt or sd != 1 or _repeats(out):
+            raise ValueError("out must have q's type, the layout's shape, a contiguous head dimension and no repeated axis")
+    oh, os = (s2, s1) if out_layout == "bshd" else (s1, s2)
+    scale = _SCALE if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")
-    st = out.stride()
-    strides = (st[0], st[2], st[1]) if out_layout == "bshd" else (st[0], st[1], st[2])
-    flags, vl = 0, None
+    flags = vp = 0
     if kv_valid_len is not None:
         vl = kv_valid_len if kv_valid_len.dtype is torch.int32 else kv_valid_len.to(torch.int32)
         vl = vl.contiguous()
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")
-        flags = L.FLAG_MASK
-    nbytes = _kv4_workspace(q.get_device(), q.dtype, B, H, Sq, Skv)
+        flags, vp = L.FLAG_MASK, vl.data_ptr()
+    nbytes = _kv4_workspace(q.get_device(), qdt, B, H, Sq, Skv)
     # Scratch of this call alone, from the caching allocator: freed on return, its block goes
     # to work enqueued later on this stream, and a captured graph keeps it in its own pool.
     ws = q.new_empty(nbytes, dtype=_U8) if nbytes else None
-    a = _ATTN_ARGS.pack(q.data_ptr(), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
-                        v.scales.data_ptr(), _TORCH_DT[q.dtype], out.data_ptr(), *strides, B, H, Sq, Skv,
-                        D, scale, flags, 0 if vl is None else vl.data_ptr(),
+    a = _ATTN_ARGS.pack(q.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), _TORCH_DT[qdt],
+                        out.data_ptr(), ob, oh, os, B, H, Sq, Skv, D, scale, flags, vp,
                         0 if ws is None else ws.data_ptr(), nbytes)
-    rc = L.lib.anima_attn_kv4_fwd(a, stream)
+    rc = _attn(a, stream)
     if rc:
         L.check(rc, "anima_attn_kv4_fwd")
     return out
