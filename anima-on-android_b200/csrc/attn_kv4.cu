@@ -557,7 +557,7 @@ static RowsPlan rows_plan(long long bh, int S_q, int S_kv, int sm_count) {
   // warp at least.
   r.nsplit = 1;
   const int per_warp = nblk / (8 * r.warps);
-  if (r.ncta == 8 && per_warp >= 8) r.nsplit = (int)std::max(1LL, std::min<long long>(room / 8, per_warp / 4));
+  if (r.ncta == 8 && per_warp >= 8) r.nsplit = (int)std::max(1LL, std::min({room / 8, (long long)per_warp / 4, 64LL}));
   r.bytes = r.nsplit > 1 ? (size_t)r.nsplit * r.units * kv4_part_floats(r.rows) * sizeof(float) : 0;
   return r;
 }

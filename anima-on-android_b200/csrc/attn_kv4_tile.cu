@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
 }
 
 // Joins the slices of every query row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, in
-// slice order.  One warp per row, four columns per lane.  part: [slice][unit][kv4_part_floats(rows)].
+// slice order.  One warp per row, four columns per lane; up to 64 slices.  part: [slice][unit][kv4_part_floats(rows)].
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
     kv4_merge_kernel(const float* part, void* out, long long ob, long long oh, long long os, int H, int S_q,
@@ -661,21 +661,44 @@ __global__ void __launch_bounds__(256)
     const int unit = bh * nqb + s / rows, r = s % rows;
     const float* const base = part + (long long)unit * kv4_part_floats(rows);
     const float* const mp = base + (long long)rows * kD + r;
-    float M = -INFINITY;
-    for (int k = 0; k < nsplit; ++k) M = fmaxf(M, mp[k * stride]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    for (int k = 0; k < nsplit; ++k) {
-      const float mk = mp[k * stride], lk = mp[k * stride + rows];
-      if (lk == 0.f) continue;  // a slice without keys, whose O may not be written
+    // lane k holds m and l of slices k and k + 32; a slice without keys has l = 0, and its O may not be
+    // written
+    float m[2], f[2], den = 0.f, M = -INFINITY;
+    uint32_t some[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = lane + 32 * h;
+      m[h] = k < nsplit ? mp[k * stride] : -INFINITY;
+      f[h] = k < nsplit ? mp[k * stride + rows] : 0.f;
+      M = fmaxf(M, m[h]);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       // only NaN scores leave the maximum at its start: their NaN sums come through
-      const float f = mk == -INFINITY ? 0.f : ex2_approx(mk - M);
-      const float4 o = *reinterpret_cast<const float4*>(base + k * stride + (long long)r * kD + lane * 4);
-      acc.x = fmaf(f, o.x, acc.x);
-      acc.y = fmaf(f, o.y, acc.y);
-      acc.z = fmaf(f, o.z, acc.z);
-      acc.w = fmaf(f, o.w, acc.w);
-      den = fmaf(f, lk, den);
+      const float l = f[h];
+      some[h] = __ballot_sync(0xffffffffu, l != 0.f);
+      f[h] = m[h] == -INFINITY ? 0.f : ex2_approx(m[h] - M);
+      den = fmaf(f[h], l, den);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) den += __shfl_xor_sync(0xffffffffu, den, d);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* const op = base + (long long)r * kD + lane * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll 8
+      for (int k = 32 * h; k < min(nsplit, 32 * h + 32); ++k) {
+        const bool take = some[h] >> (k & 31) & 1u;
+        const float fk = __shfl_sync(0xffffffffu, f[h], k & 31);  // finite where O is taken as 0
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (take) o = *reinterpret_cast<const float4*>(op + k * stride);
+        acc.x = fmaf(fk, o.x, acc.x);
+        acc.y = fmaf(fk, o.y, acc.y);
+        acc.z = fmaf(fk, o.z, acc.z);
+        acc.w = fmaf(fk, o.w, acc.w);
+      }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
     uint32_t w0, w1;
