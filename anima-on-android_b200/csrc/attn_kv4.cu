@@ -26,11 +26,12 @@
 // few and the cache long, several clusters share a unit's keys and write fp32 partials, which
 // kv4_merge_kernel joins.  No atomics; the order of all sums is fixed.
 //
-// One row against 65536 keys, 32 heads: 60 us, 5.0 TB/s of the cache (46 us at the copy rate); 65536
+// One row against 65536 keys, 32 heads: 59 us, 5.1 TB/s of the cache (46 us at the copy rate); 65536
 // blocks of 32 keys take 525 instructions each, 0.57 a cycle and scheduler, nearly half of them on the
 // integer pipe, which takes one every other cycle.  One SM's two CTAs are no faster with more warps.  One
 // row against 512 keys takes 4.7 us, seven rows against 1237 9.4.
 #include <algorithm>
+#include <atomic>
 
 #include "attn_kv4.cuh"
 #include "packed4.cuh"
@@ -535,6 +536,48 @@ static bool core_path(const int dtype, long long bh, long long S_q, int sm_count
   return dtype == ANIMA_DTYPE_F16 && bh * ((S_q + 255) / 256) >= 2LL * sm_count;
 }
 
+constexpr int kRowsStages = 3;
+template <bool kBf16, bool kOne, int kW>
+static int rows_t(const kv4::Params& p, int ncta, cudaStream_t st) {
+  auto kern = kv4::kv4_rows_kernel<kBf16, kOne, kW, kRowsStages>;
+  constexpr size_t smem = kv4::smem_bytes<kW>(kRowsStages, kOne ? 1 : 8);
+  static SmemAttr attr;
+  if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
+  return launch_clusters(kern, p.units * p.nsplit * ncta, ncta, 32 * kW, smem, st, p);
+}
+
+// Clusters of `ncta` CTAs of eight warps that the device holds at once; one cluster lies in one group of SMs,
+// and what is left over of a group stays empty, so this is less than two CTAs an SM (32 of eight on 148 SMs).  Asked for once.
+template <bool kOne>
+static int clusters_held(int ncta, int sm_count) {
+  constexpr int kMaxDev = 64;
+  static std::atomic<int> held[kMaxDev][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return std::max(1, 2 * sm_count / ncta);
+  int n = held[dev][ncta].load(std::memory_order_acquire);
+  if (n > 0) return n;
+  auto kern = kv4::kv4_rows_kernel<true, kOne, 8, kRowsStages>;
+  constexpr size_t smem = kv4::smem_bytes<8>(kRowsStages, kOne ? 1 : 8);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ncta);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)ncta;
+  at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, 2 * sm_count / ncta);
+  }
+  held[dev][ncta].store(n, std::memory_order_release);
+  return n;
+}
+
 // How a call on rows_path is cut.
 struct RowsPlan {
   int rows, nqb;   // query rows per unit, units per (batch, head)
@@ -547,29 +590,41 @@ static RowsPlan rows_plan(long long bh, int S_q, int S_kv, int sm_count) {
   r.rows = S_q > 1 ? 8 : 1;
   r.nqb = (S_q + r.rows - 1) / r.rows;
   r.units = bh * r.nqb;
-  // CTAs per cluster: as many as two to an SM have room for, while each of their warps has a block;
-  // eight warps where there are blocks for them.
+  r.nsplit = 1;
   const int nblk = (S_kv + kv4::kKeys - 1) / kv4::kKeys;
   r.warps = nblk >= 128 ? 8 : 4;
-  const long long room = std::max(1LL, 2LL * sm_count / r.units);
-  r.ncta = (int)std::min<long long>(std::min<long long>((nblk + r.warps - 1) / r.warps, room), 8);
-  // Several clusters where one leaves each warp eight blocks or more and SMs idle, four blocks a
-  // warp at least.
-  r.nsplit = 1;
-  const int per_warp = nblk / (8 * r.warps);
-  if (r.ncta == 8 && per_warp >= 8) r.nsplit = (int)std::max(1LL, std::min({room / 8, (long long)per_warp / 4, 64LL}));
+  if (r.warps == 4) {
+    // CTAs per cluster: as many as two to an SM have room for, while each of their warps has a block
+    const long long room = std::max(1LL, 2LL * sm_count / r.units);
+    r.ncta = (int)std::min<long long>(std::min<long long>((nblk + 3) / 4, room), 8);
+  } else {
+    // CTAs per cluster and clusters per unit (slices of its keys, four blocks a warp at least): the
+    // shortest chain of blocks, in rounds of the clusters that the device holds, where a round's ends cost
+    // 1.5 blocks of some 2 us and joining s slices 1.5 + s / 8.  In us, one cluster of eight against slices of one CTA, one
+    // row, heads x keys: 20 x 65536 60.7 / 43.7, 32 x 65536 60.0 / 58.5, 32 x 16384 20.8 / 23.8, 37 x 16384
+    // 31.1 / 25.3; two clusters of eight against those: 16 x 65536 37.4 / 38.0.
+    r.ncta = 1;
+    const int units = (int)std::min<long long>(r.units, 1 << 20);  // beyond, the cut is the same
+    double best = 0;
+    for (int c = 8; c >= 1; --c) {
+      const int held = r.rows == 1 ? clusters_held<true>(c, sm_count) : clusters_held<false>(c, sm_count);
+      const int per = 8 * c;  // warps of a cluster
+      const int most = std::max(1, std::min(nblk / (4 * per), 64));
+      for (int k = 1; k <= 5; ++k) {
+        const int s = k < 5 ? k : held / units;  // the last: as many as fit in one round
+        if (s > most || (k == 5 && s < 5)) continue;
+        const double chain = (double)((nblk + per * s - 1) / (per * s));
+        const double cost = (double)((units * s + held - 1) / held) * (chain + 1.5) + (s > 1 ? 1.5 + s * 0.125 : 0.0);
+        if (best == 0 || cost < best) {
+          best = cost;
+          r.ncta = c;
+          r.nsplit = s;
+        }
+      }
+    }
+  }
   r.bytes = r.nsplit > 1 ? (size_t)r.nsplit * r.units * kv4_part_floats(r.rows) * sizeof(float) : 0;
   return r;
-}
-
-template <bool kBf16, bool kOne, int kW>
-static int rows_t(const kv4::Params& p, int ncta, cudaStream_t st) {
-  constexpr int kStages = 3;
-  auto kern = kv4::kv4_rows_kernel<kBf16, kOne, kW, kStages>;
-  constexpr size_t smem = kv4::smem_bytes<kW>(kStages, kOne ? 1 : 8);
-  static SmemAttr attr;
-  if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
-  return launch_clusters(kern, p.units * p.nsplit * ncta, ncta, 32 * kW, smem, st, p);
 }
 
 static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }
@@ -585,10 +640,10 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
   const long long bh = (long long)a->B * a->H;
   const bool bf = a->dtype == ANIMA_DTYPE_BF16;
   const int* valid = (a->flags & ANIMA_FLAG_MASK) ? a->kv_valid_len : nullptr;
-  const size_t need = attn_kv4_workspace_bytes(a->dtype, a->B, a->H, a->S_q, a->S_kv, sm_count);
-  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return ANIMA_ERR_NOMEM;
+  auto room = [&](size_t need) { return need == 0 || (a->workspace && a->workspace_bytes >= need); };
   if (rows_path(bh, a->S_q, a->S_kv)) {
     const RowsPlan r = rows_plan(bh, a->S_q, a->S_kv, sm_count);
+    if (!room(r.bytes)) return ANIMA_ERR_NOMEM;
     if (r.units * r.nsplit * r.ncta > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
     kv4::Params p;
     p.q = static_cast<const uint16_t*>(a->q);
@@ -619,9 +674,12 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     if (rc != ANIMA_OK || r.nsplit == 1) return rc;
     return kv4_merge_launch(a, p.part, r.nqb, r.rows, p.units, r.nsplit, sm_count, st);
   }
-  if (!core_path(a->dtype, bh, a->S_q, sm_count))
-    return kv4_tile_launch(a, kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count), status, sm_count, st);
+  if (!core_path(a->dtype, bh, a->S_q, sm_count)) {
+    const Kv4TilePlan t = kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count);
+    return room(t.bytes) ? kv4_tile_launch(a, t, status, sm_count, st) : ANIMA_ERR_NOMEM;
+  }
   const size_t side = expanded_bytes(bh, a->S_kv);
+  if (!room(2 * side)) return ANIMA_ERR_NOMEM;
   uint16_t* const k16 = static_cast<uint16_t*>(a->workspace);
   uint16_t* const v16 = k16 + side / 2;
   const long long quads = bh * a->S_kv * 4;

@@ -724,14 +724,15 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
   t.units = (long long)bh * t.nqb;
   const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
   // Slices: at most as many as the SMs hold in one round; the number with the least of the longest
-  // chain of key tiles, some 2 us each, plus, if more than one, the merge, which is two tiles and one
-  // more per 16384 rows of partials (32 units of 256 rows: 4 tiles whole 16.7 us, in 2 slices 20.3, in
-  // 4 19.3; 16 units, 16 tiles: 42.7 whole, 23.8 in 4, 21.0 in 8).
+  // chain of key tiles, some 2 us each, plus, if more than one, the merge: 2.2 tiles, and per slice 0.09
+  // and 0.01 for every 256 rows.  In us, by slices: 32 units, 4 tiles: 16.6 whole, 21.0 in 2, 20.7 in 4; 16
+  // units, 16 tiles: 42 whole, 24 in 4, 21 in 8; 8 units, 32 tiles: 24.2 in 8, 22.8 in 16, 24.1 in 18; one unit,
+  // 128 tiles: 49 in 8, 34 in 16, 28.8 in 32, 31.2 in 64.
   const long long most = std::min({sm_count / std::max(1LL, t.units), tiles, 64LL});
   t.nsplit = 1;
   double best = (double)tiles;
   for (int k = 2; k <= most; ++k) {
-    const double cost = (double)((tiles + k - 1) / k) + 2.0 + (double)k * t.units * t.nt * attn::kBM / 16384.0;
+    const double cost = (double)((tiles + k - 1) / k) + 2.2 + k * (0.09 + 0.005 * (double)(t.units * t.nt));
     if (cost < best) {
       best = cost;
       t.nsplit = k;

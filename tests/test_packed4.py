@@ -554,6 +554,15 @@ def test_attention_long_and_wide(Sq, Skv, B, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Sq,Skv,B,H,lens", [(1, 4103, 1, 37, None), (1, 4103, 2, 20, [4103, 130]), (1, 16411, 1, 20, None),
+                                             (8, 8205, 1, 21, None), (1, 33001, 2, 6, [0, 33001]), (3, 4097, 1, 160, None),
+                                             (1, 4100, 3, 40, [31, 0, 4100])])
+def test_attention_clusters_and_slices(Sq, Skv, B, H, lens):
+    """Unit counts that ask for clusters of every size, several rounds and slices of single CTAs."""
+    check_attention(B, H, Sq, Skv, BF16 if H % 2 else F16, lens=lens)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("Sq,Skv,lens", [(1, 20011, [5, 0]), (3, 20011, [20011, 700]), (200, 5000, [0, 130]),
                                          (200, 5000, [5000, 1]), (100, 5000, [4999, 257])])
 def test_attention_masked_slices(Sq, Skv, lens):
