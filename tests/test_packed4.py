@@ -548,7 +548,7 @@ def test_attention_masked(Sq, lens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("Sq,Skv,B,H", [(1, 4096, 2, 16), (1, 20011, 1, 1), (5, 9000, 1, 3), (12, 5003, 2, 2),
-                                        (200, 5000, 1, 2), (1, 100, 8, 32)])
+                                        (200, 5000, 1, 2), (300, 5000, 1, 3), (1, 100, 8, 32)])
 def test_attention_long_and_wide(Sq, Skv, B, H):
     check_attention(B, H, Sq, Skv, F16)
 
@@ -564,7 +564,8 @@ def test_attention_clusters_and_slices(Sq, Skv, B, H, lens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("Sq,Skv,lens", [(1, 20011, [5, 0]), (3, 20011, [20011, 700]), (200, 5000, [0, 130]),
-                                         (200, 5000, [5000, 1]), (100, 5000, [4999, 257])])
+                                         (200, 5000, [5000, 1]), (100, 5000, [4999, 257]), (300, 5000, [0, 130]),
+                                         (300, 5000, [5000, 1]), (230, 5000, [4999, 257])])
 def test_attention_masked_slices(Sq, Skv, lens):
     """Keys cut into slices, of which masks leave some without a key."""
     check_attention(2, 1, Sq, Skv, F16, lens=lens)
@@ -615,7 +616,7 @@ def test_attention_sharp_and_flat(Sq):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("Sq", [3, 100])
+@pytest.mark.parametrize("Sq", [3, 100, 1100])
 def test_attention_output_views(Sq):
     """An output view is filled and nothing around it is touched."""
     g = torch.Generator().manual_seed(9)
@@ -646,7 +647,8 @@ def test_attention_repeats_bit_for_bit(Sq):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,H,Sq,Skv,dtype", [(1, 2, 1, 60, F16), (1, 2, 5, 60, BF16), (1, 1, 1, 20011, BF16), (1, 1, 4, 20011, F16),
-                                              (1, 2, 40, 5000, F16), (1, 2, 200, 5000, BF16), (1, 4, 2000, 200, BF16),
+                                              (1, 2, 40, 5000, F16), (1, 2, 200, 5000, BF16), (1, 2, 300, 5000, F16),
+                                              (1, 4, 2000, 200, BF16),
                                               (2, 16, 2400, 130, F16)])
 def test_attention_nan_reaches_its_rows_only(B, H, Sq, Skv, dtype):
     """A NaN query value reaches its row; a NaN scale of a key or a value reaches its head (a value's: its
@@ -720,6 +722,31 @@ def test_matvec_and_packing_offsets_past_32_bits():
 
 
 # ------------------------------------------------------------------ as they are used
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Sq,Skv", [(2, 1, 20011), (20, 1, 16411), (3, 300, 5000), (40, 2100, 130)])
+def test_graphs_with_scratch(H, Sq, Skv):
+    """Calls that need scratch (slices, unpacked K and V) in two graphs whose replays overlap."""
+    g = torch.Generator().manual_seed(12)
+    k, v = (Packed4(*(t.expand(H, -1, -1).contiguous() for t in random_packed((1, Skv, 128), s)[0])) for s in (1, 2))
+    qs = [torch.randn(H, Sq, 128, generator=g).to(F16).cuda() for _ in range(2)]
+    want = [anima_attn.attention_core_kv4(q, k, v, 1, H) for q in qs]
+    graphs, outs, side = [], [], torch.cuda.Stream()
+    for q in qs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            outs.append([anima_attn.attention_core_kv4(q, k, v, 1, H) for _ in range(2)])
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[n]) for n in range(2) for o in outs[n])
+    assert anima_attn.status() == 0
+
+
 @pytest.mark.gpu
 def test_streams_and_graphs():
     """The operators on a side stream, and two graphs captured on one stream whose replays overlap
