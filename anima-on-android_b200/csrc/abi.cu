@@ -77,7 +77,7 @@ int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype
                        int K, cudaStream_t st);
 int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st);
 int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaStream_t st);
-size_t attn_kv4_workspace_bytes(int dtype, int B, int H, int S_q, int S_kv, int sm_count);
+size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv, int sm_count);
 }  // namespace anima
 
 using namespace anima;
@@ -1183,7 +1183,7 @@ uint64_t anima_attn_kv4_workspace_size(int dtype, int B, int H, int S_q, int S_k
   if (!d || B <= 0 || H <= 0 || S_q <= 0 || S_kv <= 0 || S_q > kMaxRows4 || S_kv > kMaxRows4 ||
       (long long)B * H > 0x7fffffffLL)
     return 0;
-  return attn_kv4_workspace_bytes(dtype, B, H, S_q, S_kv, d->sm_count);
+  return attn_kv4_workspace_bytes(B, H, S_q, S_kv, d->sm_count);
 }
 
 int anima_attn_selftest_timeout(unsigned timeout_us, void* stream) {

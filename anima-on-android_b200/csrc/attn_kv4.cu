@@ -1,11 +1,11 @@
 // attn_kv4.cu -- attention over K and V held packed in 4 bits (format: packed4.cuh):
 // out = softmax(q K^T * scale) V per (batch, head), D = 128, key-padding lengths per sample.
 //
-// Three ways, chosen by rows_path and core_path below:
+// Two ways, chosen by rows_path below:
 //   little work: kv4_rows_kernel reads the packed cache directly, eight query rows at a time;
-//   more:        attn_kv4_tile.cu, on the tensor cores, unpacks K and V in the kernel;
-//   very many fp16 rows: the cache is unpacked once to 16 bits (expand_kernel) and the attention core
-//                of attn_fwd.cu runs on it, which spares each 256-row unit unpacking it again.
+//   more:        attn_kv4_tile.cu, on the tensor cores, unpacks K and V in the kernel.
+// Neither writes the cache out in 16 bits: scratch holds partial results of slices only, at most 64
+// times 130 floats a query row.
 //
 // kv4_rows_kernel.  One cluster per (batch, head, block of query rows); its CTAs and their
 // warps take 32-key blocks in turn, each warp with its own running maximum, sum and output, so
@@ -37,10 +37,6 @@
 #include "packed4.cuh"
 
 namespace anima {
-
-int attn_fwd_launch(const AnimaAttnArgs* a, int* status, int sm_count, cudaStream_t st,
-                    void* const* peers = nullptr, int n_peers = 0, int peer_rows = 0,
-                    long long peer_row_stride = 0, int peer_head0 = 0);
 
 namespace kv4 {
 
@@ -476,49 +472,6 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
   cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// ---------------------------------------------------------------- many rows: unpack once
-// Packed rows of K (blockIdx.y = 0) and V (1) to the attention core's fp16 operands; rows at
-// or past a sample's length are written as zeros, whatever the cache holds there.
-__global__ void __launch_bounds__(256)
-    expand_kernel(const uint4* kc, const uint2* ks, const uint4* vc, const uint2* vs, uint16_t* ko,
-                  uint16_t* vo, const int* valid, int H, int S_kv, long long quads) {
-  grid_dependents_launch();  // the core sets up meanwhile; it waits for this grid before it reads
-  grid_dependency_wait();
-  const uint4* codes = blockIdx.y ? vc : kc;
-  const uint2* scales = blockIdx.y ? vs : ks;
-  uint16_t* out = blockIdx.y ? vo : ko;
-  for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < quads;
-       u += (long long)gridDim.x * blockDim.x) {
-    const long long row = u >> 2;
-    uint16_t* const at = out + row * kD + 8 * (u & 3);
-    uint4 c = make_uint4(0u, 0u, 0u, 0u);
-    uint2 s2 = make_uint2(0u, 0u);
-    bool take = true;
-    if (valid) {
-      const long long bh = row / S_kv;
-      take = row - bh * S_kv < __ldg(valid + bh / H);
-    }
-    if (take) {
-      c = __ldg(codes + u);
-      s2 = __ldg(scales + row);
-    }
-    const float4 s = p4::scales4(s2);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    const float sg[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uint32_t n[4], r[4];
-      p4::numbers_f16(w[g], n);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&n[k]));
-        r[k] = pack_f16x2(v.x * sg[g], v.y * sg[g]);
-      }
-      *reinterpret_cast<uint4*>(at + 32 * g) = make_uint4(r[0], r[1], r[2], r[3]);
-    }
-  }
-}
-
 }  // namespace kv4
 
 // Whether the packed cache is read directly.  Up to 16 rows always; beyond, the rows' passes over the
@@ -533,13 +486,6 @@ static bool rows_path(long long bh, long long S_q, long long S_kv) {
   const long long most = 1LL << (20 + (S_kv >= 4096) + (S_kv >= 32768));
   return S_q <= 16 || bh * S_q * std::max(S_kv, 256LL) <= most;
 }
-// Whether K and V are unpacked once for the attention core: fp16 calls of two rounds of 256-row units or
-// more (4096 x 512 at 32 heads 52 us against the tile kernel's 57, 16384 x 512 152 / 184; at one
-// round the two are even).  bf16 rows keep the tile kernel, whose fp16 operands are more exact.
-static bool core_path(const int dtype, long long bh, long long S_q, int sm_count) {
-  return dtype == ANIMA_DTYPE_F16 && bh * ((S_q + 255) / 256) >= 2LL * sm_count;
-}
-
 constexpr int kRowsStages = 3;
 template <bool kBf16, bool kOne, int kW>
 static int rows_t(const kv4::Params& p, int ncta, cudaStream_t st) {
@@ -631,12 +577,9 @@ static RowsPlan rows_plan(long long bh, int S_q, int S_kv, int sm_count) {
   return r;
 }
 
-static size_t expanded_bytes(long long bh, long long S_kv) { return (size_t)(bh * S_kv) * 256; }
-
-size_t attn_kv4_workspace_bytes(int dtype, int B, int H, int S_q, int S_kv, int sm_count) {
+size_t attn_kv4_workspace_bytes(int B, int H, int S_q, int S_kv, int sm_count) {
   const long long bh = (long long)B * H;
   if (rows_path(bh, S_q, S_kv)) return rows_plan(bh, S_q, S_kv, sm_count).bytes;
-  if (core_path(dtype, bh, S_q, sm_count)) return 2 * expanded_bytes(bh, S_kv);
   return kv4_tile_plan((int)bh, S_q, S_kv, sm_count).bytes;
 }
 
@@ -678,39 +621,8 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     if (rc != ANIMA_OK || r.nsplit == 1) return rc;
     return kv4_merge_launch(a, p.part, r.nqb, r.rows, p.units, r.nsplit, sm_count, st);
   }
-  if (!core_path(a->dtype, bh, a->S_q, sm_count)) {
-    const Kv4TilePlan t = kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count);
-    return room(t.bytes) ? kv4_tile_launch(a, t, status, sm_count, st) : ANIMA_ERR_NOMEM;
-  }
-  const size_t side = expanded_bytes(bh, a->S_kv);
-  if (!room(2 * side)) return ANIMA_ERR_NOMEM;
-  uint16_t* const k16 = static_cast<uint16_t*>(a->workspace);
-  uint16_t* const v16 = k16 + side / 2;
-  const long long quads = bh * a->S_kv * 4;
-  const dim3 grid((unsigned)std::min<long long>((quads + 255) / 256, (long long)sm_count * 8), 2);
-  kv4::expand_kernel<<<grid, 256, 0, st>>>(static_cast<const uint4*>(a->k_codes), static_cast<const uint2*>(a->k_scales),
-                             static_cast<const uint4*>(a->v_codes), static_cast<const uint2*>(a->v_scales),
-                             k16, v16, valid, a->H, a->S_kv, quads);
-  if (cudaGetLastError() != cudaSuccess) return ANIMA_ERR_CUDA;
-  AnimaAttnArgs c = {};
-  c.q = a->q;
-  c.k = k16;
-  c.v = v16;
-  c.op_dtype = a->dtype;
-  c.out = a->out;
-  c.out_dtype = a->dtype;
-  for (int k = 0; k < 3; ++k) c.out_stride[k] = a->out_stride[k];
-  c.B = a->B;
-  c.H = a->H;
-  c.S_q = a->S_q;
-  c.S_kv = a->S_kv;
-  c.D = kv4::kD;
-  c.scale = a->scale;
-  c.flags = a->flags;
-  c.kv_valid_len = a->kv_valid_len;
-  // No workspace for the core's cut schedule: its merge adds the slices in the order in which
-  // they finish, and these results are to repeat bit for bit.
-  return attn_fwd_launch(&c, status, sm_count, st);
+  const Kv4TilePlan t = kv4_tile_plan((int)bh, a->S_q, a->S_kv, sm_count);
+  return room(t.bytes) ? kv4_tile_launch(a, t, status, sm_count, st) : ANIMA_ERR_NOMEM;
 }
 
 }  // namespace anima

@@ -363,9 +363,10 @@ int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
  * not count, whatever is stored there; none left gives zero rows).
  * Little work reads the packed rows directly and has fp32 accuracy up to the output's rounding.
  * More runs on the tensor cores with fp16 operands (K and V, which are to be in fp16's range as
- * anima_quantize4 leaves them, and the probabilities); very many fp16 rows unpack K and V first.
- * `workspace`: anima_attn_kv4_workspace_size bytes (0 for some calls), 256-byte aligned, contents
- * irrelevant; calls that share one must be ordered.  Asynchronous on `stream`.
+ * anima_quantize4 leaves them, and the probabilities).  The cache is never written out unpacked.
+ * `workspace`: anima_attn_kv4_workspace_size bytes for partial results (0 for some calls; at most 64 x 130
+ * floats a query row, rows rounded up to 256), 256-byte aligned, contents irrelevant; calls that share
+ * one must be ordered.  Asynchronous on `stream`.
  */
 typedef struct AnimaAttnKv4Args {
   const void* q;
