@@ -232,9 +232,8 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
     S_q, 128].  ``kv_valid_len`` int32 [B]: keys at or past it do not count, whatever the
     cache holds there; a sample without any has zero rows.
 
-    ``out`` overlaps no operand.  Few query rows have fp32 accuracy up to the output's rounding;
-    many run on fp16 operands (unpacked K and V, probabilities), whose products are summed in
-    fp32 (anima_attn_kv4_fwd)."""
+    ``out`` overlaps no operand.  K and V enter exactly, probabilities to 2^-16; sums are fp32 and the
+    result is rounded once (anima_attn_kv4_fwd)."""
     kc, ks = k
     vc, vs = v
     stream = _here(q, kc, ks, vc, vs, kv_valid_len, out)

@@ -475,13 +475,13 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 }  // namespace kv4
 
 // Whether the packed cache is read directly.  Up to 16 rows always; beyond, the rows' passes over the
-// cache (and, below 256 keys, their starts) cost more than the tile kernel's start (some 6 us) once
+// cache (and, below 256 keys, their starts) cost more than the tile kernel's start (some 8 us) once
 // heads x rows x keys exceed 2^20, twice that from 4096 keys and four times that from 32768, where the
 // tile kernel has slices to join.  Measured, us, this way against the tile kernel, heads x rows x keys:
-// 4 x 1024 x 130 12.5 / 12.6, 32 x 128 x 130 12.7 / 9.9, 4 x 512 x 512 13.4 / 16.6, 32 x 64 x 512 13.3 / 12.1,
-// 4 x 1024 x 512 19.8 / 16.6, 32 x 64 x 2048 29.9 / 18.5, 1 x 512 x 4096 17.0 / 21.2, 16 x 32 x 4096
-// 17.0 / 18.9, 4 x 256 x 4096 27.4 / 21.5, 4 x 32 x 16384 19.1 / 24.5, 4 x 64 x 16384 27.0 / 24.4, 1 x 64 x
-// 65536 29.8 / 33.8.
+// 4 x 1024 x 130 12.2 / 12.1, 32 x 128 x 130 12.2 / 9.2, 4 x 512 x 512 12.2 / 16.7, 32 x 64 x 512 12.2 / 13.6,
+// 4 x 1024 x 512 18.8 / 17.7, 32 x 64 x 2048 28.0 / 21.0, 1 x 512 x 4096 16.2 / 23.6, 16 x 32 x 4096
+// 16.2 / 21.1, 4 x 256 x 4096 26.2 / 24.0, 4 x 32 x 16384 18.6 / 27.7, 4 x 64 x 16384 26.1 / 28.3, 1 x 64 x
+// 65536 28.9 / 41.7, 1 x 128 x 65536 45.3 / 41.7.
 static bool rows_path(long long bh, long long S_q, long long S_kv) {
   const long long most = 1LL << (20 + (S_kv >= 4096) + (S_kv >= 32768));
   return S_q <= 16 || bh * S_q * std::max(S_kv, 256LL) <= most;

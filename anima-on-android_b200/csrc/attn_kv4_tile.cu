@@ -3,36 +3,44 @@
 // CTA itself.  out = softmax(q K^T * scale) V per (batch, head), D = 128.
 //
 // Work unit = kNT 128-row query tiles of one (batch, head); its keys may be cut into slices, and
-// (unit, slice) is a segment, streamed in 128-key tiles.  The grid is persistent: a CTA takes
+// (unit, slice) is a segment, streamed in 64-key tiles.  The grid is persistent: a CTA takes
 // segments c, c + G, ..., and moves from one to the next without draining (the next Q tile, K and V
 // are under way while the last P V and the output of the segment before run).  A unit cut into
 // slices writes fp32 partials (O, running max, running sum), which kv4_merge_kernel joins in slice
 // order, so results repeat bit for bit.
 //
-// Operands are fp16 whatever q's type.  K and V: n * s rounded once (most codes make it exact).
-// q: fp16 as it is; bf16 rows are first scaled by the power of two that brings their largest
-// magnitude to [2^14, 2^15), which the row's softmax scale takes back, so a bf16 value keeps its
-// eight bits down to 2^-31 of the row's largest.
+// No operand loses bits that the result could show.  A value n s of K or V has up to 15 bits and is held as
+// the exact sum of two 16-bit parts, P as two as well:
+//   S = Q K_hi^T + Q K_lo^T                     fp16, q as it is, K exact
+//   O += P_hi V_hi + P_lo V_hi + P_hi V_lo      bf16, V exact, P to 2^-17; the part left out is below 2^-17
+// P is bf16 for its range: a weight is as right far below the row's largest as next to it, whatever the
+// length of the cache (fp16 has nothing below 2^-25).  As one fp16 product each, with K, V and P rounded
+// to 11 bits, the result was off by 3.1e-4 before its own rounding, and calls took two thirds of the time.
+// bf16 query rows are first scaled by the power of two that brings their largest magnitude to
+// [2^14, 2^15), which the row's softmax scale takes back, so a bf16 value keeps its eight bits down
+// to 2^-31 of the row's largest.
 //
 // Warp roles (16 warps):
 //   warps 0-3    softmax of query tile 0: thread = query row = TMEM lane.  Per key tile reads its S
-//                row, updates max / sum, writes P over S; at the end stores O.  A bf16 Q
+//                row, updates max / sum, writes P's parts over S; at the end stores O.  A bf16 Q
 //                tile is converted in place by its warpgroup before its first MMA.
 //   warps 4-7    softmax of query tile 1 (kNT = 2), or unpack (kNT = 1, where a key tile feeds
-//                half the MMA work and unpacking would bound it).
-//   warps 8-11   unpack: stream packed tiles through cp.async stages into 16-bit K / V tiles in the
-//                128-byte-swizzled layout of the MMA operands.
-//   warp 12      MMA issuer (one thread) + TMEM owner.
-//   warp 13      TMA producer of the Q tiles; warps 14 and 15 only fill the warpgroup.
-// Tensor memory: S_0, S_1, O_0, O_1 of 128 columns; P_i overlays S_i.  With two query tiles their
-// MMAs alternate, so one tile's softmax runs beside the other's MMAs; with one, its key tiles
-// alternate between S_0 and S_1, and a tile's QK^T runs beside the softmax of the tile before it.
+//                half the MMA work).
+//   warps 8-11   unpack: packed tiles into the parts' tiles in the 128-byte-swizzled layout of the MMA
+//                operands.
+//   warps 12, 14 MMA issuers of a query tile each (kNT = 2), or of Q K^T and P V; 12 owns the TMEM.
+//   warp 13      TMA producer of the Q tiles.
+//   warp 15      packed tiles from global memory by cp.async.
+// An issuing warp runs converged and one elected lane issues: descriptors stay in uniform registers.  With
+// one divergent thread issuing for both query tiles an MMA took 100 cycles beside busy softmax warps,
+// against 48 (Q K^T, N = 64, shared memory) and 64 (P V) of the tensor core.
+// Tensor memory: two S buffers of 64 columns per query tile, with P's parts over S, and O_0, O_1 of 128
+// columns.  Q K^T runs a step ahead of P V, so the softmax of one step runs beside the MMAs of its neighbours.
 //
-// What bounds it is the chain of the core kernel: softmax (an exponential a score), hand-off, MMAs.  A
-// step of two query tiles takes some 4,300 cycles against 2,050 of MMAs (traced); without any unpacking
-// it took 8 % less, without any exponential 2 %.  256 rows against 32768 keys, 32 heads: 160 us, 860
-// TFLOP/s of fp16 products; 64 rows 103 us.  Three or four K / V slots and two to four packed tiles in
-// flight measured alike; fewer registers for the softmax (184) cost 10 %.
+// What bounds it: a step of two query tiles and 64 keys takes 3,010 cycles (traced) of 3,072 that its MMAs
+// need, and the unpacking fills as much; the clock falls under that load (1.4 GHz).  256 rows against 8192
+// keys, 32 heads: 82 us; 64 rows 52 us, 2,500 cycles a step of 1,536 of MMAs, the rest unpacking and
+// hand-offs.
 #include <algorithm>
 
 #include "attn_kv4.cuh"
@@ -44,15 +52,15 @@ namespace kv4t {
 
 using namespace attn;  // kD, kBM, drain_wait, stage/store_block, pack2
 
-constexpr int kKeys = 128;                  // keys per tile
-constexpr int kRaw = 5;                     // stages of packed tiles
+constexpr int kKeys = 64;                   // keys per tile
 constexpr int kPanel = 128 * 128;           // [128 rows][64 x 16-bit]
-constexpr int kTile = 2 * kPanel;
-constexpr int kRawBytes = kKeys * 64 + kKeys * 8;
-constexpr int kMmaWarp12 = 12, kQWarp13 = 13;
+constexpr int kTile = 2 * kPanel;            // a Q tile
+constexpr int kKvPanel = kKeys * 128;
+constexpr int kPart = 2 * kKvPanel;          // the upper or lower parts of a K or V tile
+constexpr int kMmaWarp12 = 12, kQWarp13 = 13, kRawWarp15 = 15;
 constexpr int kThreads16 = 512;
-// 512 threads launch with 128 registers each: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
-constexpr uint32_t kRegsSoft = 192, kRegsUnpack = 72, kRegsMma = 56;
+// 512 threads launch with 128 registers each: 256 x 168 + 128 x 112 + 128 x 64 = 512 x 128.
+constexpr uint32_t kRegsSoft = 168, kRegsUnpack = 112, kRegsMma = 64;
 static_assert(2 * kRegsSoft + kRegsUnpack + kRegsMma == 4 * 128, "register split");
 
 struct Params {
@@ -74,22 +82,27 @@ struct Params {
 
 template <int kNT>
 struct Smem {
-  static constexpr int kSlots = kNT == 2 ? 3 : 4;  // unpacked K / V tiles
+  static constexpr int kUnpackWarps = kNT == 2 ? 4 : 8;
+  static constexpr int kGroups = kKeys / 8 / kUnpackWarps;  // of eight keys, per tile and warp
+  static constexpr int kRaw = kNT == 2 ? 3 : 8;             // stages of packed tiles
   uint8_t q[kNT][kTile];
-  uint8_t kv[kSlots][kTile];
-  uint8_t raw[kRaw][kRawBytes];
+  uint8_t kv[2][2][2][kPart];  // unpacked tiles of K, of V: two slots, upper and lower parts
+  uint8_t raw[kRaw][kKeys * 72];  // codes, then scales
   float4 stage[kNT * 4][128];  // per softmax warp: one 32 x 32 16-bit block on its way to global
   uint64_t q_raw[2];           // Q tile as loaded
   uint64_t q_conv[2];          // bf16: converted
   uint64_t q_empty[2];
-  uint64_t kv_full[kSlots];
-  uint64_t kv_empty[kSlots];
-  uint64_t s_full[2];
-  uint64_t p_full[2];
+  uint64_t raw_full[kRaw];
+  uint64_t raw_empty[kRaw];
+  uint64_t kv_full[2][2];   // [K, V][slot]
+  uint64_t kv_empty[2][2];
+  uint64_t s_full[2][2];    // [query tile][buffer]
+  uint64_t p_full[2][2];
   uint64_t o_full[2];
   uint64_t o_empty[2];
-  uint64_t pv_done;
-  uint64_t mma_done;
+  uint64_t pv_done[2];
+  uint64_t s_empty[2];      // [buffer], one query tile
+  uint64_t mma_done[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -115,6 +128,59 @@ __device__ __forceinline__ Seg segment(const Params& p, int seg, int rows) {
   s.k0 = (int)((long long)tiles * s.slice / p.nsplit);
   s.n = (int)((long long)tiles * (s.slice + 1) / p.nsplit) - s.k0;
   return s;
+}
+
+// One lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// Arrives on `bar` once all of this thread's asynchronous copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The m-th of the 2 n tiles of a segment in the order in which they are used: K_0 K_1 V_0 K_2 V_1 ...
+// K_(n-1) V_(n-2) V_(n-1).
+struct Item {
+  int v, tile;  // V or K, key tile
+};
+__device__ __forceinline__ Item item_of(int m, int n) {
+  if (m == 0 || m == 2 * n - 1) return {m > 0, m >> 1};
+  return {~m & 1, (m & 1) ? (m + 1) >> 1 : (m >> 1) - 1};
+}
+
+// n s of four pairs as the sum of two fp16 (n: numbers in, upper parts out).  n s is a multiple of 2^-24
+// of at most 15 bits, so what its rounding to 11 leaves is a value of fp16 too.
+__device__ __forceinline__ void split_f16(uint32_t (&n)[4], uint32_t (&lo)[4], __half2 s) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __half2 v = *reinterpret_cast<const __half2*>(&n[k]);
+    const __half2 h = __hmul2(v, s);
+    const __half2 l = __hfma2(v, s, __hneg2(h));
+    n[k] = *reinterpret_cast<const uint32_t*>(&h);
+    lo[k] = *reinterpret_cast<const uint32_t*>(&l);
+  }
+}
+// The same in bf16, s in two parts (lower half, upper half of `s2`): 8 bits above, and what is left of n s
+// below, at most 2^-8 of it and so at most 6 bits.
+__device__ __forceinline__ void split_bf16(uint32_t (&n)[4], uint32_t (&lo)[4], uint32_t s2) {
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+  const __nv_bfloat162 s0 = __low2bfloat162(s), s1 = __high2bfloat162(s);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&n[k]);
+    const __nv_bfloat162 h = __hmul2(v, s0);
+    const __nv_bfloat162 l = __hfma2(v, s1, __hfma2(v, s0, __hneg2(h)));
+    n[k] = *reinterpret_cast<const uint32_t*>(&h);
+    lo[k] = *reinterpret_cast<const uint32_t*>(&l);
+  }
 }
 
 // A thread's bf16 query row of a Q tile to fp16 in place, scaled; returns the factor that undoes it.
@@ -155,28 +221,32 @@ __global__ void __launch_bounds__(kThreads16, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   Smem<kNT>& sm = *reinterpret_cast<Smem<kNT>*>(smem_raw + pad);
-  constexpr int kUnpackWarps = kNT == 2 ? 4 : 8;
+  constexpr int kUnpackWarps = Smem<kNT>::kUnpackWarps, kGroups = Smem<kNT>::kGroups, kRaw = Smem<kNT>::kRaw;
   constexpr int kRows = kNT * kBM;
-  constexpr int kSlots = Smem<kNT>::kSlots;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&sm.kv_full[s], kUnpackWarps);
-      mbar_init(&sm.kv_empty[s], 1);
+    for (int k = 0; k < kRaw; ++k) {
+      mbar_init(&sm.raw_full[k], 32);
+      mbar_init(&sm.raw_empty[k], kUnpackWarps);
     }
     for (int i = 0; i < 2; ++i) {
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&sm.kv_full[i][k], kUnpackWarps);
+        mbar_init(&sm.kv_empty[i][k], kNT);
+        mbar_init(&sm.s_full[i][k], 1);
+        mbar_init(&sm.p_full[i][k], kBM);
+      }
+      mbar_init(&sm.pv_done[i], 1);
+      mbar_init(&sm.mma_done[i], 1);
+      mbar_init(&sm.s_empty[i], 1);
       mbar_init(&sm.q_raw[i], 1);
       mbar_init(&sm.q_conv[i], kBM);
       mbar_init(&sm.q_empty[i], 1);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], kBM);
       mbar_init(&sm.o_full[i], 1);
       mbar_init(&sm.o_empty[i], kBM);
     }
-    mbar_init(&sm.pv_done, 1);
-    mbar_init(&sm.mma_done, 1);
     sm.abort = 0;
     fence_barrier_init();
   }
@@ -223,122 +293,133 @@ __global__ void __launch_bounds__(kThreads16, 1)
           if (a > 0) drain_wait(&sm.q_raw[i], (uint32_t)(a - 1) & 1u);
           if (i == 0) drain_wait(&sm.q_raw[0], (uint32_t)a & 1u);
         }
-    } else if (warp == kMmaWarp12 && lane == 0) {
-      // ---------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc_qk = make_idesc_f16(0u, kBM, kKeys, 0);
-      constexpr uint32_t idesc_pv = make_idesc_f16(0u, kBM, kD, 1);
-      const uint64_t dk0 = sdesc_sw128(smem_u32(sm.kv[0]), 16, 1024);
-      const uint64_t dv0 = sdesc_sw128(smem_u32(sm.kv[0]), kPanel, 1024);
-      const uint64_t dq0 = sdesc_sw128(smem_u32(sm.q[0]), 16, 1024);
-      auto issue_qk = [&](int i, int slot) {
-        const uint64_t kb = desc_plus(dk0, (uint32_t)slot * kTile);
-        uint64_t bd[8], aq[8];
+    } else if (warp == kRawWarp15) {
+      // ---------------------------------------------------------- packed tiles
+      // 16-byte chunk c of key r's codes goes to row r ^ ((r >> 2) & 1), so that the two keys that a
+      // quarter-warp of the unpacking reads lie in different banks.
+      bool ok = true;
+      int raw = 0, use = 0;
+      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
+        const Seg s = segment(p, seg, kRows);
+        const long long row0 = (long long)s.bh * p.S_kv + (long long)s.k0 * kKeys;
+        for (int m = 0; m < 2 * s.n; ++m) {
+          const Item it = item_of(m, s.n);
+          const bool got = wait(&sm.raw_empty[raw], ((uint32_t)use & 1u) ^ 1u);
+          if (!(ok = __all_sync(0xffffffffu, got))) break;
+          const int left = s.len - (s.k0 + it.tile) * kKeys;  // valid keys from this tile's first on
+          const uint8_t* const codes = (it.v ? p.vc : p.kc) + (row0 + (long long)it.tile * kKeys) * 64 + lane * 16;
+          const uint8_t* const scales = (it.v ? p.vs : p.ks) + (row0 + (long long)it.tile * kKeys) * 8 + lane * 8;
+          const int r = lane >> 2;
+          const uint32_t dst = smem_u32(sm.raw[raw]) + (r ^ (r >> 2)) * 64 + (lane & 3) * 16;
+          const uint32_t sdst = smem_u32(sm.raw[raw]) + kKeys * 64 + lane * 8;
+          if (left >= kKeys) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
-          aq[kk] = desc_plus(dq0, (uint32_t)i * kTile + (kk >> 2) * kPanel + (kk & 3) * 32);
+            for (int c = 0; c < 8; ++c) p4::cp16(dst + c * 512, codes + c * 512);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) p4::cp8(sdst + c * 256, scales + c * 256);
+          } else {  // keys past the length read as zeros
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const bool take = 8 * c + r < left;
+              p4::cp16_if(dst + c * 512, take ? codes + c * 512 : p.kc, take);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const bool take = 32 * c + lane < left;
+              p4::cp8_if(sdst + c * 256, take ? scales + c * 256 : p.ks, take);
+            }
+          }
+          cp_arrive(&sm.raw_full[raw]);
+          if (++raw == kRaw) raw = 0, ++use;
         }
-        umma_ss_x8(tmem + i * 128, aq, bd, idesc_qk, 0u);
+      }
+      p4::cp_wait<0>();
+    } else if (warp == kMmaWarp12 || warp == kMmaWarp12 + 2) {
+      // ---------------------------------------------------------- MMA issuers: of a query tile each, or of Q K^T and P V
+      // The warp runs converged and one elected lane issues, so that descriptors stay in uniform registers.
+      const int who = __shfl_sync(0xffffffffu, (warp - kMmaWarp12) >> 1, 0);
+      const int i = kNT == 1 ? 0 : who;
+      const bool qk = kNT == 2 || who == 0, pv = kNT == 2 || who == 1;
+      const bool leader = elect_one();
+      constexpr uint32_t idesc_qk = make_idesc_f16(0u, kBM, kKeys, 0);  // fp16 Q and K
+      constexpr uint32_t idesc_pv = make_idesc_f16(1u, kBM, kD, 1);     // bf16 P and V
+      const uint64_t dk0 = sdesc_sw128(smem_u32(sm.kv[0]), 16, 1024);
+      const uint64_t dv0 = sdesc_sw128(smem_u32(sm.kv[1]), kKvPanel, 1024);
+      const uint64_t dq0 = sdesc_sw128(smem_u32(sm.q[0]), 16, 1024);
+      auto s_at = [&](int t) { return tmem + (2 * i + (t & 1)) * kKeys; };
+      // S_i of step t = Q_i (K_hi + K_lo)^T
+      auto issue_qk = [&](int t) {
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const uint64_t kb = desc_plus(dk0, (uint32_t)(2 * (t & 1) + part) * kPart);
+          uint64_t bd[8], aq[8];
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            bd[kk] = desc_plus(kb, (kk >> 2) * kKvPanel + (kk & 3) * 32);
+            aq[kk] = desc_plus(dq0, (uint32_t)i * kTile + (kk >> 2) * kPanel + (kk & 3) * 32);
+          }
+          if (leader) umma_ss_x8(s_at(t), aq, bd, idesc_qk, part);
+        }
       };
-      auto issue_pv = [&](int i, int slot, bool acc) {
-        const uint64_t vb = desc_plus(dv0, (uint32_t)slot * kTile);
+      // O_i (+)= P_hi V_hi + P_lo V_hi + P_hi V_lo of step t
+      auto issue_pv = [&](int t, bool acc) {
+        const uint64_t vb = desc_plus(dv0, (uint32_t)(2 * (t & 1)) * kPart);
+        const uint32_t tP = s_at(t), tO = tmem + 256 + i * kD;
         uint64_t bd[8];
         uint32_t a[8];
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          bd[kk] = desc_plus(vb, kk * 2048);
-          a[kk] = tmem + i * 128 + kk * 8;
+          bd[kk] = desc_plus(vb, (kk & 3) * 2048);
+          a[kk] = tP + kk * 8;
         }
-        umma_ts_x8(tmem + 256 + i * 128, a, bd, idesc_pv, acc ? 1u : 0u);
+        if (leader) umma_ts_x8(tO, a, bd, idesc_pv, acc ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (leader) umma_ts(tO, a[kk], desc_plus(bd[kk], kPart), idesc_pv, 1u);
       };
-      auto slot_of = [](int item) { return item % kSlots; };
-      auto par_of = [](int item) { return (uint32_t)(item / kSlots) & 1u; };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+      };
       bool ok = true;
-      auto key_tile = [&](int item) {
-        ok = ok && wait(&sm.kv_full[slot_of(item)], par_of(item));
-        tc_fence_after();
-      };
-      auto query_tile = [&](int i, int a) {
-        ok = ok && wait(kBf16 ? &sm.q_conv[i] : &sm.q_raw[i], (uint32_t)a & 1u);
+      auto get = [&](uint64_t* bar, int phase) {
+        const bool got = ok && wait(bar, (uint32_t)phase & 1u);
+        ok = __all_sync(0xffffffffu, got);
         tc_fence_after();
       };
       int a = 0, gg = 0;
       for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
         const int n = segment(p, seg, kRows).n;
         if (n <= 0) continue;
-        const uint32_t pa = (uint32_t)(a - 1) & 1u;
-        if (kNT == 2) {
-          for (int g = 0; g <= n && ok; ++g) {
-            const int ik = 2 * (gg + g), iv = ik - 1;  // K of this step, V of the one before
-            const uint32_t pp = (uint32_t)(gg + g - 1) & 1u;
-            if (g > 0) key_tile(iv);
-#pragma unroll
-            for (int i = 0; i < kNT; ++i) {
-              if (g > 0) {
-                if (!(ok = ok && wait(&sm.p_full[i], pp))) break;
-                if (g == 1 && a > 0 && !(ok = wait(&sm.o_empty[i], pa))) break;
-                tc_fence_after();
-                issue_pv(i, slot_of(iv), g > 1);
-                if (g == n) umma_commit(&sm.o_full[i]);
-                if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(iv)]);
-              }
-              if (g < n) {
-                if (g == 0) query_tile(i, a);
-                if (i == 0) key_tile(ik);
-                if (!ok) break;
-                issue_qk(i, slot_of(ik));
-                umma_commit(&sm.s_full[i]);
-                if (g == n - 1) umma_commit(&sm.q_empty[i]);
-                if (i == kNT - 1) umma_commit(&sm.kv_empty[slot_of(ik)]);
-              }
-            }
-          }
-        } else {
-          // S of step t in columns 128 (t % 2); Q is tile 0 and O columns 256 .. 383 throughout.
-          auto qk = [&](int t, bool last) {
-            key_tile(2 * t);
-            if (!ok) return;
-            const uint64_t kb = desc_plus(dk0, (uint32_t)slot_of(2 * t) * kTile);
-            uint64_t bd[8], aq[8];
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              bd[kk] = desc_plus(kb, (kk >> 2) * kPanel + (kk & 3) * 32);
-              aq[kk] = desc_plus(dq0, (kk >> 2) * kPanel + (kk & 3) * 32);
-            }
-            umma_ss_x8(tmem + (t & 1) * 128, aq, bd, idesc_qk, 0u);
-            umma_commit(&sm.s_full[t & 1]);
-            if (last) umma_commit(&sm.q_empty[0]);
-            umma_commit(&sm.kv_empty[slot_of(2 * t)]);
-          };
-          query_tile(0, a);
-          if (ok) qk(gg, n == 1);
-          for (int g = 0; g < n && ok; ++g) {
-            const int t = gg + g;
-            if (g + 1 < n) qk(t + 1, g + 2 == n);
+        // QK^T runs a step ahead of P V.  S of step t is in buffer t % 2, which P V of step t - 2 has to have left:
+        // with two query tiles it is the same thread's and earlier in the pipe.
+        if (qk) get(kBf16 ? &sm.q_conv[i] : &sm.q_raw[i], a);
+        for (int g = -1; g < n; ++g) {
+          const int t = gg + g, u = t + 1;
+          if (qk && g + 1 < n) {
+            if (kNT == 1 && u > 1) get(&sm.s_empty[u & 1], (u >> 1) - 1);
+            get(&sm.kv_full[0][u & 1], u >> 1);
             if (!ok) break;
-            key_tile(2 * t + 1);
-            if (!(ok = ok && wait(&sm.p_full[t & 1], (uint32_t)(t >> 1) & 1u))) break;
-            if (g == 0 && a > 0 && !(ok = wait(&sm.o_empty[0], pa))) break;
-            tc_fence_after();
-            const uint64_t vb = desc_plus(dv0, (uint32_t)slot_of(2 * t + 1) * kTile);
-            uint64_t bd[8];
-            uint32_t ap[8];
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              bd[kk] = desc_plus(vb, kk * 2048);
-              ap[kk] = tmem + (t & 1) * 128 + kk * 8;
-            }
-            umma_ts_x8(tmem + 256, ap, bd, idesc_pv, g > 0 ? 1u : 0u);
-            umma_commit(&sm.pv_done);
-            umma_commit(&sm.kv_empty[slot_of(2 * t + 1)]);
+            issue_qk(u);
+            commit(&sm.s_full[i][u & 1]);
+            if (g + 2 == n) commit(&sm.q_empty[i]);
+            commit(&sm.kv_empty[0][u & 1]);
           }
-          if (ok) umma_commit(&sm.o_full[0]);
+          if (!pv || g < 0) continue;
+          get(&sm.kv_full[1][t & 1], t >> 1);
+          get(&sm.p_full[i][t & 1], t >> 1);
+          if (g == 0 && a > 0) get(&sm.o_empty[i], a - 1);
+          if (!ok) break;
+          issue_pv(t, g > 0);
+          commit(&sm.pv_done[i]);
+          if (kNT == 1) commit(&sm.s_empty[t & 1]);
+          if (g + 1 == n) commit(&sm.o_full[i]);
+          commit(&sm.kv_empty[1][t & 1]);
         }
         gg += n;
         ++a;
       }
-      umma_commit(&sm.mma_done);
-      drain_wait(&sm.mma_done, 0);
+      commit(&sm.mma_done[who]);
+      drain_wait(&sm.mma_done[who], 0);
     }
     __syncwarp();
   } else if (warp >= 4 * kNT) {
@@ -349,99 +430,73 @@ __global__ void __launch_bounds__(kThreads16, 1)
     // a quarter-warp's store lie in different halves of the swizzled 128 bytes.
     const int w = warp - 4 * kNT;
     const int i = lane & 3, jr = (((lane >> 2) & 1) << 2) | (lane >> 3);
-    constexpr int kGroups = 16 / kUnpackWarps;  // of eight rows, per item and warp
-    const uint32_t raw0 = smem_u32(sm.raw[0]);
-    const int r0 = w * kGroups * 8 + jr;
-    // The loads run ahead of the conversion, across segments: their own walk.
-    int ld_seg = blockIdx.x - gridDim.x, ld_item = 0, ld_items = 0, ld_slot = 0, ld_left = 0;
-    long long ld_row = 0;
-    auto load = [&]() {
-      while (ld_item >= ld_items) {  // the next segment with keys
-        ld_seg += gridDim.x;
-        if (ld_seg >= segs) break;
-        const Seg s = segment(p, ld_seg, kRows);
-        ld_item = 0;
-        ld_items = 2 * s.n;
-        ld_row = (long long)s.bh * p.S_kv + (long long)s.k0 * kKeys + r0;
-        ld_left = s.len - s.k0 * kKeys;  // valid keys from the segment's first on
-      }
-      if (ld_seg < segs) {
-        const bool v = ld_item & 1;
-        const int left = ld_left - (ld_item >> 1) * kKeys;  // ... from this tile's first on
-        const long long row = ld_row + (long long)(ld_item >> 1) * kKeys;
-        const uint8_t* const codes = (v ? p.vc : p.kc) + row * 64 + i * 16;
-        const uint8_t* const scales = (v ? p.vs : p.ks) + row * 8;
-        const uint32_t dst = raw0 + ld_slot * kRawBytes + r0 * 64 + i * 16;
-        const uint32_t sdst = raw0 + ld_slot * kRawBytes + kKeys * 64 + r0 * 8;
-        if (left >= kKeys) {
-#pragma unroll
-          for (int c = 0; c < kGroups; ++c) {
-            p4::cp16(dst + c * 512, codes + c * 512);
-            if (i == 0) p4::cp8(sdst + c * 64, scales + c * 64);
-          }
-        } else {  // keys past the length read as zeros
-#pragma unroll
-          for (int c = 0; c < kGroups; ++c) {
-            const bool take = r0 + 8 * c < left;
-            p4::cp16_if(dst + c * 512, take ? codes + c * 512 : p.kc, take);
-            if (i == 0) p4::cp8_if(sdst + c * 64, take ? scales + c * 64 : p.ks, take);
-          }
-        }
-        ++ld_item;
-      }
-      p4::cp_commit();
-      ld_slot = ld_slot + 1 == kRaw ? 0 : ld_slot + 1;
-    };
+    constexpr uint32_t kRawStage = kKeys * 72;
+    const int r0 = w * kGroups * 8 + jr;  // this lane's first row of a tile; the others lie 8 apart
+    const uint32_t raw0 = smem_u32(sm.raw[0]) + (r0 ^ ((r0 >> 2) & 1)) * 64 + i * 16;  // its codes in a stage,
+    const uint32_t raws0 = smem_u32(sm.raw[0]) + kKeys * 64 + r0 * 8;                  // and the row's scales
     // where this lane's eight values of group g go: 16-byte chunk 4 (g % 2) + i of panel g / 2
     uint32_t put[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) put[g] = r0 * 128 + (((4 * g + i) ^ (jr & 7)) << 4);
-#pragma unroll
-    for (int k = 0; k < kRaw - 1; ++k) load();
     bool ok = true;
-    int raw = 0, item = 0;
-    for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x)
-    for (int todo = 2 * segment(p, seg, kRows).n; todo > 0; --todo, ++item) {
-      const int slot = item % kSlots;
-      p4::cp_wait<kRaw - 2>();
-      __syncwarp();
-      const uint32_t src = raw0 + raw * kRawBytes + r0 * 64 + i * 16;
-      const uint32_t ssrc = raw0 + raw * kRawBytes + kKeys * 64 + r0 * 8;
+    int raw = 0, use = 0, gg = 0;
+    for (int seg = blockIdx.x, n; seg < segs && ok; seg += gridDim.x, gg += n) {
+    n = segment(p, seg, kRows).n;
+#pragma unroll 1
+    for (int m = 0; m < 2 * n; ++m) {
+      const Item it = item_of(m, n);
+      const int t = gg + it.tile, slot = t & 1;
+      const bool here = wait(&sm.raw_full[raw], (uint32_t)use & 1u);
+      if (!(ok = __all_sync(0xffffffffu, here))) break;
       uint4 u[kGroups];
       uint2 s2[kGroups];
 #pragma unroll
       for (int c = 0; c < kGroups; ++c) {
-        u[c] = p4::lds16(src + c * 512);
-        s2[c] = p4::lds8(ssrc + c * 64);
+        u[c] = p4::lds16(raw0 + raw * kRawStage + c * 512);
+        s2[c] = p4::lds8(raws0 + raw * kRawStage + c * 64);
       }
-      raw = raw + 1 == kRaw ? 0 : raw + 1;
-      load();  // into the slot of the item before this one
-      const bool got = wait(&sm.kv_empty[slot], ((uint32_t)(item / kSlots) & 1u) ^ 1u);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.raw_empty[raw]);
+      if (++raw == kRaw) raw = 0, ++use;
+      const bool got = wait(&sm.kv_empty[it.v][slot], ((uint32_t)(t >> 1) & 1u) ^ 1u);
       if (!(ok = __all_sync(0xffffffffu, got))) break;
-      const uint32_t dst = smem_u32(sm.kv[slot]);
+      const uint32_t dst = smem_u32(sm.kv[it.v][slot]);
 #pragma unroll
       for (int c = 0; c < kGroups; ++c) {
         const uint32_t wd[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
         const __half2 sa = *reinterpret_cast<const __half2*>(&s2[c].x);
         const __half2 sb = *reinterpret_cast<const __half2*>(&s2[c].y);
-        const __half2 sg[4] = {__low2half2(sa), __high2half2(sa), __low2half2(sb), __high2half2(sb)};
+        auto put_parts = [&](int g, const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
+          const uint32_t at = dst + (g >> 1) * kKvPanel + put[g & 1] + c * 1024;
+          st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+          st_shared_v4(at + kPart, lo[0], lo[1], lo[2], lo[3]);
+        };
+        uint32_t hi[4], lo[4];
+        if (it.v == 0) {
+          const __half2 sg[4] = {__low2half2(sa), __high2half2(sa), __low2half2(sb), __high2half2(sb)};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t v[4];
-          p4::numbers_f16(wd[g], v);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&v[k]), sg[g]);
-            v[k] = *reinterpret_cast<const uint32_t*>(&x);
+          for (int g = 0; g < 4; ++g) {
+            p4::numbers_f16(wd[g], hi);
+            split_f16(hi, lo, sg[g]);
+            put_parts(g, hi, lo);
           }
-          st_shared_v4(dst + (g >> 1) * kPanel + put[g & 1] + c * 1024, v[0], v[1], v[2], v[3]);
+        } else {
+          const float2 fa = __half22float2(sa), fb = __half22float2(sb);
+          const float f[4] = {fa.x, fa.y, fb.x, fb.y};
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float top = __bfloat162float(__float2bfloat16_rn(f[g]));
+            p4::numbers_bf16(wd[g], hi);
+            split_bf16(hi, lo, pack_bf16x2(top, f[g] - top));
+            put_parts(g, hi, lo);
+          }
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.kv_full[slot]);
+      if (lane == 0) mbar_arrive(&sm.kv_full[it.v][slot]);
     }
-    p4::cp_wait<0>();
+    }
   } else {
     regs_inc<kRegsSoft>();
     // ------------------------------------------------------------ softmax / epilogue
@@ -480,21 +535,21 @@ __global__ void __launch_bounds__(kThreads16, 1)
     float m = -INFINITY, l = 0.f;
     for (int g = 0; g < n; ++g) {
       const int t = gg + g;
-      const int buf = kNT == 2 ? i : t & 1;  // S and its barriers
-      const uint32_t tS = tmem + lane_field + buf * 128;
-      const bool got = wait(&sm.s_full[buf], (uint32_t)(kNT == 2 ? t : t >> 1) & 1u);
+      const int buf = t & 1;  // S and its barriers
+      const uint32_t tS = tmem + lane_field + (2 * i + buf) * kKeys;
+      const bool got = wait(&sm.s_full[i][buf], (uint32_t)(t >> 1) & 1u);
       if (!(ok = __all_sync(0xffffffffu, got))) break;
       tc_fence_after();
-      uint32_t r[4][32];
+      uint32_t r[2][32];
       const int lim = s.len - (s.k0 + g) * kKeys;
       const bool full = lim >= kKeys;
       auto load_s = [&]() {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld32(tS + c * 32, r[c]);
         tmem_ld_wait();
         if (!full) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (c * 32 + e >= lim) r[c][e] = __float_as_uint(-INFINITY);
@@ -506,26 +561,26 @@ __global__ void __launch_bounds__(kThreads16, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] = fmaxf(SV(2 * k), SV(2 * k + 1));
 #pragma unroll
-        for (int e = 16; e < 128; e += 16)
+        for (int e = 16; e < kKeys; e += 16)
 #pragma unroll
           for (int k = 0; k < 8; ++k) acc[k] = max3f(acc[k], SV(e + 2 * k), SV(e + 2 * k + 1));
         return max3f(max3f(acc[0], acc[1], acc[2]), max3f(acc[3], acc[4], acc[5]), fmaxf(acc[6], acc[7]));
       };
       uint64_t sum2[4];
-      uint32_t pk[2][32];
       auto exp_pass = [&](float mu) {
         const float nb = (mu == -INFINITY) ? 0.f : -mu;
         const uint64_t scale2 = f2pack(sl2, sl2), base2 = f2pack(nb, nb);
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum2[k] = 0ull;
 #pragma unroll
-        for (int pr = 0; pr < 64; ++pr) {
+        for (int pr = 0; pr < kKeys / 2; ++pr) {
           float x0, x1;
           f2unpack(fma2(f2pack(SV(2 * pr), SV(2 * pr + 1)), scale2, base2), x0, x1);
           x0 = ex2_approx(x0);
           x1 = ex2_approx(x1);
           sum2[pr & 3] = add2(sum2[pr & 3], f2pack(x0, x1));
-          pk[pr >> 5][pr & 31] = pack_f16x2(x0, x1);
+          r[pr >> 4][2 * (pr & 15)] = __float_as_uint(x0);
+          r[pr >> 4][2 * (pr & 15) + 1] = __float_as_uint(x1);
         }
       };
       auto row_sum = [&]() {
@@ -560,16 +615,24 @@ __global__ void __launch_bounds__(kThreads16, 1)
           sum = row_sum();
         }
       }
-      tmem_st32(tS, pk[0]);
-      tmem_st32(tS + 32, pk[1]);
+      {  // P in two bf16 parts over S: upper in the first 32 columns, lower in the other 32
+        uint32_t hi[32], lo[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float x0 = SV(2 * k), x1 = SV(2 * k + 1);
+          hi[k] = pack_bf16x2(x0, x1);
+          lo[k] = pack_bf16x2(x0 - __uint_as_float(hi[k] << 16), x1 - __uint_as_float(hi[k] & 0xffff0000u));
+        }
+        tmem_st32(tS, hi);
+        tmem_st32(tS + 32, lo);
+      }
 #undef SV
       l = l * alpha + sum;
       if (__any_sync(0xffffffffu, g > 0 && alpha != 1.f)) {
-        if (kNT == 1) {  // the PV before this step may still run (s_full covers it with two tiles)
-          const bool idle = wait(&sm.pv_done, (uint32_t)(t - 1) & 1u);
-          if (!(ok = __all_sync(0xffffffffu, idle))) break;
-          tc_fence_after();
-        }
+        // the P V before this step may still run
+        const bool idle = wait(&sm.pv_done[i], (uint32_t)(t - 1) & 1u);
+        if (!(ok = __all_sync(0xffffffffu, idle))) break;
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -582,7 +645,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&sm.p_full[buf]);
+      mbar_arrive(&sm.p_full[i][buf]);
       m = m_use;
     }
     if (!ok) break;
@@ -724,15 +787,15 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
   t.units = (long long)bh * t.nqb;
   const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
   // Slices: at most as many as the SMs hold in one round; the number with the least of the longest
-  // chain of key tiles, some 2 us each, plus, if more than one, the merge: 2.2 tiles, and per slice 0.09
-  // and 0.01 for every 256 rows.  In us, by slices: 32 units, 4 tiles: 16.6 whole, 21.0 in 2, 20.7 in 4; 16
-  // units, 16 tiles: 42 whole, 24 in 4, 21 in 8; 8 units, 32 tiles: 24.2 in 8, 22.8 in 16, 24.1 in 18; one unit,
-  // 128 tiles: 49 in 8, 34 in 16, 28.8 in 32, 31.2 in 64.
+  // chain of key tiles, some 1.65 us each, plus, if more than one, the merge: 2.7 tiles, and per slice 0.11
+  // and 0.012 for every 256 rows.  In us, by slices: 32 units, 8 tiles: 22.2 whole, 23.1 in 2, 21.0 in 4; 16
+  // units, 32 tiles: 63 whole, 30 in 4, 23.5 in 8; 8 units, 64 tiles: 30.0 in 8, 24.8 in 16; one unit,
+  // 256 tiles: 69 in 8, 45 in 16, 34.6 in 32, 33.3 in 64.
   const long long most = std::min({sm_count / std::max(1LL, t.units), tiles, 64LL});
   t.nsplit = 1;
   double best = (double)tiles;
   for (int k = 2; k <= most; ++k) {
-    const double cost = (double)((tiles + k - 1) / k) + 2.2 + k * (0.09 + 0.005 * (double)(t.units * t.nt));
+    const double cost = (double)((tiles + k - 1) / k) + 2.7 + k * (0.11 + 0.006 * (double)(t.units * t.nt));
     if (cost < best) {
       best = cost;
       t.nsplit = k;

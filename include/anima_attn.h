@@ -361,9 +361,9 @@ int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
  * 8) are of dtype (F16 or BF16), out overlapping no operand; scale is positive; S_q and S_kv go
  * up to 2^30.  flags: ANIMA_FLAG_MASK with kv_valid_len (keys at or past it are not read or do
  * not count, whatever is stored there; none left gives zero rows).
- * Little work reads the packed rows directly and has fp32 accuracy up to the output's rounding.
- * More runs on the tensor cores with fp16 operands (K and V, which are to be in fp16's range as
- * anima_quantize4 leaves them, and the probabilities).  The cache is never written out unpacked.
+ * Little work reads the packed rows directly, more runs on tcgen05 tiles.  Both keep K and V exact (their
+ * values are to be in fp16's range, as anima_quantize4 leaves them) and the probabilities to 2^-16, sum in
+ * fp32, and round the result once.  The cache is never written out unpacked.
  * `workspace`: anima_attn_kv4_workspace_size bytes for partial results (0 for some calls; at most 64 x 130
  * floats a query row, rows rounded up to 256), 256-byte aligned, contents irrelevant; calls that share
  * one must be ordered.  Asynchronous on `stream`.

@@ -58,3 +58,82 @@ def test_a_packed_cache_is_not_written_out(dtype, B, H, Sq, Skv):
     assert L.lib.anima_attn_kv4_workspace_size(dtype, B, H, Sq, Skv) == 0
     for sq in (1, 8, 64, 200):
         assert L.lib.anima_attn_kv4_workspace_size(dtype, 1, 1, sq, 1 << 20) <= 64 * (sq + 255) * 130 * 4
+
+
+# ------------------------------------------------------------------ attention: K, V and P keep their bits
+def crafted(way_, BH, Sq, dtype, q, k, v, scale=1.0):
+    """One cache for all heads, the same rows in each head: the result against 64 bits.
+    Tolerance: P is held in two bf16 parts, P (1 + 2^-17), and times V in two bf16 parts loses the product
+    of the lower parts, 2^-9 each; an exponential is off by 2^-22 and its argument, here of scores that
+    fp32 holds exactly, by 2^-22 more; a handful of fp32 sums.  Together below 2^-16 of sum p |v|.
+    The result is rounded once."""
+    (kp, kv), (vp, vv) = k, v
+    assert way(BH, Sq, kv.shape[1]) == way_
+    qd = q[None].expand(BH, -1, -1).to(dtype).contiguous().cuda()
+    assert torch.equal(qd[0].double().cpu(), q.double())  # the type holds q
+    got = anima_attn.attention_core_kv4(qd, every_head(kp, BH), every_head(vp, BH), 1, BH, scale=scale)
+    out, pv, _ = attention_ref(q.double().numpy()[None], kv, vv, 1, 1, None, scale)
+    err = np.abs(got.double().cpu().numpy() - out)
+    tol = pv * 2.0 ** -16 + np.abs(out) * half_step(dtype) + (3e-8 if dtype == F16 else 0.0)
+    assert (err <= tol).all(), float((err / np.maximum(tol, 1e-300)).max())
+    assert anima_attn.status() == 0
+
+
+def two_keys(a, sa, b, sb):
+    """Two keys (or values) whose 128 entries are a sa and b sb."""
+    return packed(np.stack([np.full(128, a), np.full(128, b)])[None], np.stack([np.full(4, sa), np.full(4, sb)])[None])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("way_,BH,Sq", WAYS)
+def test_keys_keep_their_bits(way_, BH, Sq, dtype):
+    """7 (1 + 2^-10) needs 13 bits.  Against a key of 7 the score differs by 128 * 7 * 2^-10 = 0.875; of
+    keys rounded to 16 bits it would by 1, or by 0."""
+    q = torch.zeros(Sq, 128)
+    q[:, 37] = 128.0
+    crafted(way_, BH, Sq, dtype, q, two_keys(7, 1 + 2.0 ** -10, 7, 1.0), two_keys(1, 1.0, -1, 1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("way_,BH,Sq", WAYS)
+def test_values_keep_their_bits(way_, BH, Sq, dtype):
+    """Equal weights on 7 (1 + 2^-10) and -7: what is left is what the 13th bit holds."""
+    crafted(way_, BH, Sq, dtype, torch.zeros(Sq, 128), two_keys(0, 1.0, 0, 1.0), two_keys(7, 1 + 2.0 ** -10, -7, 1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("way_,BH,Sq", WAYS)
+def test_probabilities_keep_their_bits(way_, BH, Sq, dtype):
+    """Weights 1 and p, p near 1/2, on values 1 and -2: 1 - 2 p is left, near 0."""
+    q = torch.zeros(Sq, 128)
+    step = 2.0 ** -11 if dtype == F16 else 2.0 ** -8
+    q[:, 5] = 0.6875 + step * (torch.arange(Sq) % 23 - 11)
+    crafted(way_, BH, Sq, dtype, q, two_keys(0, 1.0, -1, 1.0), two_keys(1, 1.0, -2, 1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("BH,Sq", [(75, 17), (75, 3), (38, 257)])
+@pytest.mark.parametrize("ahead", [16.5, 17.5, 20.0, 30.0])
+def test_a_long_cache_keeps_its_tail(dtype, BH, Sq, ahead):
+    """65536 keys of which one is `ahead` above the others, e^ahead times their weight, and has a value of
+    zero, theirs being 1: the others' share is a small number, and relative to it (it is sum p |v|) the
+    weights have to be right.  Sums of 65536 equal terms in fp32: each addition rounds by half a step, at
+    most 65536 / 16 additions of one accumulator on the tensor core and 4096 in a thread's sum."""
+    N = 65536
+    n = np.zeros((1, N, 128), np.int64)
+    n[0, 5, 0] = -8
+    k, kv = packed(n, np.full((1, N, 4), -ahead / 8))
+    n = np.ones((1, N, 128), np.int64)
+    n[0, 5] = 0
+    v, _ = packed(n, np.ones((1, N, 4)))
+    q = torch.zeros(BH, Sq, 128, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    got = anima_attn.attention_core_kv4(q, every_head(k, BH), every_head(v, BH), 1, BH, scale=1.0).double().cpu().numpy()
+    w = (N - 1) * math.exp(-kv[0, 5, 0])
+    want = w / (1 + w)
+    tol = want * (2.0 ** -16 + 2 * 4096 * 2.0 ** -24 + half_step(dtype)) + (3e-8 if dtype == F16 else 0.0)
+    assert np.abs(got - want).max() <= tol, (float(np.abs(got - want).max()), want)
