@@ -610,7 +610,7 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     p.nqb = r.nqb;
     p.units = (int)r.units;
     p.nsplit = r.nsplit;
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.scale_log2 = std::min(a->scale * 1.4426950408889634f, 3.402823466e38f);
     int rc;
     if (r.warps == 8)
       rc = r.rows == 1 ? (bf ? rows_t<true, true, 8>(p, r.ncta, st) : rows_t<false, true, 8>(p, r.ncta, st))

@@ -507,16 +507,17 @@ __global__ void __launch_bounds__(kThreads16, 1)
     const uint32_t tO = tmem + lane_field + 256 + i * 128;
     int a = 0, gg = 0;
     bool ok = true;
-    // The scale of this thread's row of segment round `round`; bf16: once its Q tile is loaded,
-    // converts the row.
+    // The scale of this thread's row of segment round `round`, never 0 or infinite; bf16: once its Q tile
+    // is loaded, converts the row.
+    auto in_range = [](float x) { return fminf(fmaxf(x, 1.4e-45f), 3.402823466e38f); };
     auto take_q = [&](int round) {
-      if (!kBf16) return p.scale_log2;
+      if (!kBf16) return in_range(p.scale_log2);
       const bool got = wait(&sm.q_raw[i], (uint32_t)round & 1u);
       if (!(ok = __all_sync(0xffffffffu, got))) return 0.f;
       const float back = convert_row(sm.q[i], row);
       fence_proxy_async_smem();
       mbar_arrive(&sm.q_conv[i]);
-      return p.scale_log2 * back;
+      return in_range(p.scale_log2 * back);
     };
     auto more = [&](int seg) {  // whether a segment with keys follows
       for (seg += gridDim.x; seg < segs; seg += gridDim.x)
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       sl2 = take_q(a);
       if (!ok) break;
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // m in units of S
     for (int g = 0; g < n; ++g) {
       const int t = gg + g;
       const int buf = t & 1;  // S and its barriers
@@ -567,6 +568,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
         return max3f(max3f(acc[0], acc[1], acc[2]), max3f(acc[3], acc[4], acc[5]), fmaxf(acc[6], acc[7]));
       };
       uint64_t sum2[4];
+      // 2^((S - mu) scale): the difference first, so that at the maximum itself it is exactly 0 however large
+      // scores are (S scale - m with a rounded m is off by 16 once they pass 2^28).
       auto exp_pass = [&](float mu) {
         const float nb = (mu == -INFINITY) ? 0.f : -mu;
         const uint64_t scale2 = f2pack(sl2, sl2), base2 = f2pack(nb, nb);
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
 #pragma unroll
         for (int pr = 0; pr < kKeys / 2; ++pr) {
           float x0, x1;
-          f2unpack(fma2(f2pack(SV(2 * pr), SV(2 * pr + 1)), scale2, base2), x0, x1);
+          f2unpack(fma2(add2(f2pack(SV(2 * pr), SV(2 * pr + 1)), base2), scale2, 0ull), x0, x1);
           x0 = ex2_approx(x0);
           x1 = ex2_approx(x1);
           sum2[pr & 3] = add2(sum2[pr & 3], f2pack(x0, x1));
@@ -593,7 +596,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       load_s();
       float m_use = m, alpha = 1.f, sum;
       if (g == 0) {
-        m_use = row_max() * sl2;
+        m_use = row_max();
         alpha = 0.f;
         exp_pass(m_use);
         sum = row_sum();
@@ -603,13 +606,13 @@ __global__ void __launch_bounds__(kThreads16, 1)
         const bool check = !(sum <= 256.f) || (m == -INFINITY && sum > 0.f);
         if (__any_sync(0xffffffffu, check)) {
           load_s();
-          const float m_tile = row_max() * sl2;
+          const float m_tile = row_max();
           if (m == -INFINITY) {
             m_use = m_tile;
             alpha = 0.f;
-          } else if (m_tile > m + kRescaleThreshold) {
+          } else if ((m_tile - m) * sl2 > kRescaleThreshold) {
             m_use = m_tile;
-            alpha = ex2_approx(m - m_tile);
+            alpha = ex2_approx((m - m_tile) * sl2);
           }
           exp_pass(m_use);
           sum = row_sum();
@@ -649,6 +652,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       m = m_use;
     }
     if (!ok) break;
+    const float sl2_of_m = sl2;  // the next segment's may be fetched before m is written
     if (n > 0) {
       // The next segment's Q tile, if any, has been loading since this one's last QK^T.
       have_q = kBf16 && more(seg);
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
                 make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
       }
       if (!direct) {
-        part[kRows * kD + urow + lane] = m;
+        part[kRows * kD + urow + lane] = m == -INFINITY ? m : m * sl2_of_m;
         part[kRows * kD + kRows + urow + lane] = l;
       }
     }
@@ -845,7 +849,7 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   p.nqb = t.nqb;
   p.units = (int)t.units;
   p.nsplit = t.nsplit;
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = std::min(a->scale * 1.4426950408889634f, 3.402823466e38f);
   CUtensorMap mq;
   int rc = attn_head_map(&mq, a->q, a->dtype, a->B * a->H, a->S_q);
   if (rc != ANIMA_OK) return rc;

@@ -137,3 +137,44 @@ def test_a_long_cache_keeps_its_tail(dtype, BH, Sq, ahead):
     want = w / (1 + w)
     tol = want * (2.0 ** -16 + 2 * 4096 * 2.0 ** -24 + half_step(dtype)) + (3e-8 if dtype == F16 else 0.0)
     assert np.abs(got - want).max() <= tol, (float(np.abs(got - want).max()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e8, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("BH,Sq,Skv", [(1, 1, 700), (2, 11, 700), (40, 100, 700), (16, 300, 700), (1, 100, 65000), (2, 200, 9000)])
+def test_rows_of_huge_scores(size, BH, Sq, Skv):
+    """bf16 rows whose scores are so large that one key takes all: the output is that key's value.  A row
+    is compared where the best key is ahead by more than the scores' own rounding (512 fp32 steps of
+    sum |q| |k| scale) and 40."""
+    g = torch.Generator().manual_seed(21)
+    q = (torch.randn(BH, Sq, 128, generator=g) * size).to(BF16).cuda()
+    k, kv = random_packed((1, Skv, 128), 22)
+    v, vv = random_packed((1, Skv, 128), 23)
+    got = anima_attn.attention_core_kv4(q, every_head(k, BH), every_head(v, BH), 1, BH)[0].transpose(0, 1).double().cpu().numpy()
+    sc = 1 / math.sqrt(128)
+    qd = q.double().cpu().numpy().reshape(-1, 128)
+    s = qd @ kv[0].T * sc
+    top2 = np.partition(s, Skv - 2, -1)[:, -2:]
+    far = top2[:, 1] - top2[:, 0] > 512 * 2.0 ** -23 * (np.abs(qd) @ np.abs(kv[0]).T * sc).max(-1) + 40
+    assert far.mean() > 0.95
+    want = vv[0][s.argmax(-1)]
+    err = np.abs(got.reshape(-1, 128) - want)
+    assert (err[far] <= np.abs(want[far]) * (half_step(BF16) + 2.0 ** -16)).all(), float(np.nanmax(err[far]))
+    assert anima_attn.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [1e-45, 1e-30, 3e38])
+@pytest.mark.parametrize("BH,Sq", [(2, 1), (2, 9), (40, 128), (16, 300), (2, 3000)])
+def test_scales_at_the_ends_of_fp32(dtype, scale, BH, Sq):
+    """Equal scores, keys cut off in the middle of a tile: the mean of the values, whatever the scale.
+    Rounding: weights of 1 are exact, sums of at most 333 values in fp32, the result once."""
+    Skv, n = 333, 201
+    k, _ = random_packed((1, Skv, 128), 51)
+    v, vv = random_packed((1, Skv, 128), 52)
+    q = torch.zeros(BH, Sq, 128, dtype=dtype, device="cuda")
+    got = anima_attn.attention_core_kv4(q, every_head(k, BH), every_head(v, BH), 1, BH, scale=scale,
+                                        kv_valid_len=torch.tensor([n], dtype=torch.int32, device="cuda")).double().cpu().numpy()
+    want, size = vv[0, :n].mean(0), np.abs(vv[0, :n]).mean(0)
+    assert (np.abs(got - want) <= np.abs(want) * half_step(dtype) + size * 400 * 2.0 ** -23 + (3e-8 if dtype == F16 else 0)).all()
