@@ -99,8 +99,9 @@ constexpr size_t smem_bytes(int stages, int rows) {
 // kBf16: type of q and out (else fp16); kOne: the form for a single row, else up to eight; kW:
 // warps; kNS: stages.
 //
-// A single row has the eight columns to itself.  For S^T its q is scaled by a power of two to whole
-// numbers below 2^30 and written in four signed base-256 digits, the columns (twice over), and the MMA
+// A single row has the eight columns to itself.  For S^T its q is scaled by a power of two below 2^30, and
+// the whole part and 2^31 times the rest are written in four signed base-256 digits each, the columns, so
+// that an fp16 value is exact and a bf16 one down to 2^-54 of the row's largest.  The MMA
 // is the one of whole numbers (m16n8k32) on c = n + 8: three instructions unpack eight codes where
 // fp16 takes nine and bf16 eleven, and the sums are exact (1 x 65536, 32 heads: 66 -> 60 us).  For O^T
 // the columns of P are the row's four group-scaled forms, high parts in columns 0 .. 3 and low parts in
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
       qf[g] = __ldg(reinterpret_cast<const uint4*>(p.q + ((long long)bh * p.S_q + qrow) * kD + 32 * g + 8 * i));
   }
   float sl2 = p.scale_log2;
-  uint2 qd[4];       // kOne: digit j % 4 of this lane's eight values of group g, in the codes' order
+  uint2 qd[4];       // kOne: digit j of this lane's eight values of group g, in the codes' order
   uint64_t base[4];  // and what its two columns' sums start from, 1.5 * 2^23 + 8 sum(digits)
   if constexpr (kOne) {
     uint32_t top = 0;
@@ -154,8 +155,15 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     const int e0 = (30 - E) / 2, e1 = 30 - E - e0;  // in two steps: neither factor leaves fp32
     const float f0 = __int_as_float((e0 + 127) << 23), f1 = __int_as_float((e1 + 127) << 23);
     const int s0 = (E - 6) / 2, s1 = E - 6 - s0;
-    sl2 = top >= 0x7f800000u ? NAN
-                             : sl2 * __int_as_float((s0 + 127) << 23) * __int_as_float((s1 + 127) << 23);
+    sl2 = top >= 0x7f800000u
+              ? NAN
+              : fminf(sl2 * __int_as_float((s0 + 127) << 23) * __int_as_float((s1 + 127) << 23), 3.402823466e38f);
+    auto whole = [&](float v) {  // this column's whole number of a value, its signed digits as bytes
+      const float y = v * f0 * f1;
+      const int n = __float2int_rn(y);
+      const int part = j < 4 ? n : __float2int_rn((y - (float)n) * 2147483648.f);
+      return ((uint32_t)part + 0x00808080u) ^ 0x00808080u;
+    };
     const uint32_t sel = (uint32_t)(3 - (j & 3)) | (uint32_t)(7 - (j & 3)) << 4;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -164,8 +172,8 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 v = widen<kBf16>(w[k]);
-        t[2 * k] = ((uint32_t)__float2int_rn(v.x * f0 * f1) + 0x00808080u) ^ 0x00808080u;
-        t[2 * k + 1] = ((uint32_t)__float2int_rn(v.y * f0 * f1) + 0x00808080u) ^ 0x00808080u;
+        t[2 * k] = whole(v.x);
+        t[2 * k + 1] = whole(v.y);
       }
       qd[g].x = __byte_perm(__byte_perm(t[0], t[4], sel), __byte_perm(t[1], t[5], sel), 0x5410);
       qd[g].y = __byte_perm(__byte_perm(t[2], t[6], sel), __byte_perm(t[3], t[7], sel), 0x5410);
@@ -264,14 +272,16 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
           s0 = fma2(f2pack(g0[g], g0[g]), add2(f2pack(__int_as_float(d[0]), __int_as_float(d[1])), base[g]), s0);
           s1 = fma2(f2pack(g1[g], g1[g]), add2(f2pack(__int_as_float(d[2]), __int_as_float(d[3])), base[g]), s1);
         }
-        // the digits 2 (i % 2) and the next together, then the other lane's two
-        const float f = (i & 1) ? 1.52587890625e-05f : 1.0f;  // 2^-16
+        // the digits 2 i and the next together, then the other lanes'
+        const float f = __int_as_float((127 - 16 * (i & 1) - 31 * (i >> 1)) << 23);
         float a, b;
         f2unpack(s0, a, b);
         a = fmaf(b, 0.00390625f, a) * f;
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
         sc[u][0] = a + __shfl_xor_sync(0xffffffffu, a, 1);
         f2unpack(s1, a, b);
         a = fmaf(b, 0.00390625f, a) * f;
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
         sc[u][2] = a + __shfl_xor_sync(0xffffffffu, a, 1);
       } else {
 #pragma unroll

@@ -178,3 +178,24 @@ def test_scales_at_the_ends_of_fp32(dtype, scale, BH, Sq):
                                         kv_valid_len=torch.tensor([n], dtype=torch.int32, device="cuda")).double().cpu().numpy()
     want, size = vv[0, :n].mean(0), np.abs(vv[0, :n]).mean(0)
     assert (np.abs(got - want) <= np.abs(want) * half_step(dtype) + size * 400 * 2.0 ** -23 + (3e-8 if dtype == F16 else 0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Sq", [1, 5])
+def test_a_large_query_value_leaves_the_others(dtype, Sq):
+    """One value of a row is far larger than the others and meets keys of zero there: the scores are
+    the others' alone (bound: as for any direct call, of sum |q| |k|, where it has no part)."""
+    rng = np.random.default_rng(31)
+    BH, Skv = 2, 300
+    n = rng.integers(-8, 8, (BH, Skv, 128))
+    n[..., 3] = 0
+    k, kv = packed(n, rng.uniform(50, 100, (BH, Skv, 4)))
+    v, vv = random_packed((BH, Skv, 128), 32)
+    q = torch.randn(BH, Sq, 128, generator=torch.Generator().manual_seed(33)) * 2.0 ** -7
+    q[..., 3] = 60000.0 if dtype == F16 else 1e9
+    q = q.to(dtype)
+    got = anima_attn.attention_core_kv4(q.cuda(), k, v, 1, BH).double().cpu().numpy()
+    out, pv, top = attention_ref(q.double().numpy(), kv, vv, 1, BH, None, 1 / math.sqrt(128))
+    err, tol = np.abs(got - out), attention_bound(out, pv, top, dtype, True)
+    assert (err <= tol).all(), float((err / tol).max())
