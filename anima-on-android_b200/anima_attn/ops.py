@@ -251,17 +251,20 @@ def attention_cached_kv(q: torch.Tensor, kh, vh,
     """Cross-attention whose K/V operands were prepared earlier: q [B, S_q, H, D] pre-norm
     projection -> [B, S_q, H, D].  kh/vh [B*H, S_kv, D] 16-bit head-major, as prologue(None,
     k, v) returns them, or both packed to 4 bits (quantize4 of those).  Runs the q side of the
-    prologue and the attention core only; with packed K/V on fp16 operands, or bf16 for a bf16
-    ``out_dtype`` (other output types are a cast of that result)."""
+    prologue and the attention core only; with packed K/V on fp16 queries, or bf16 for a bf16
+    ``out_dtype``."""
     B, Sq, H, D = q.shape
     if isinstance(kh, tuple):  # Packed4
         from .packed import attention_core_kv4
         op = torch.bfloat16 if out_dtype == torch.bfloat16 else torch.float16
         qh, _, _ = prologue(q, None, None, q_norm_w, None, None, eps, norm_q, False, op)
-        if out is not None and out.dtype != op:
-            return out.copy_(attention_core_kv4(qh, kh, vh, B, H, scale, kv_valid_len))
-        o = attention_core_kv4(qh, kh, vh, B, H, scale, kv_valid_len, out)
-        return o if out is not None else o.to(out_dtype)
+        to = out_dtype if out is None else out.dtype
+        if to == op or to == torch.float32:
+            return attention_core_kv4(qh, kh, vh, B, H, scale, kv_valid_len, out, out_dtype=to)
+        if out is not None and out.shape != q.shape:
+            raise ValueError("out must be [B, S_q, H, D]")
+        o = attention_core_kv4(qh, kh, vh, B, H, scale, kv_valid_len, out_dtype=torch.float32)
+        return o.to(to) if out is None else out.copy_(o)
     qh, _, _ = prologue(q, None, None, q_norm_w, None, None, eps, norm_q, False, kh.dtype)
     return attention_core(qh, kh, vh, B, H, scale, kv_valid_len, False, out=out,
                           out_layout="bshd", out_dtype=out_dtype)

@@ -224,12 +224,13 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
 
 def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
                        scale: Optional[float] = None, kv_valid_len: Optional[torch.Tensor] = None,
-                       out: Optional[torch.Tensor] = None, out_layout: str = "bshd") -> torch.Tensor:
+                       out: Optional[torch.Tensor] = None, out_layout: str = "bshd",
+                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """attention_core over packed K and V: softmax(q k^T * scale) v per head.
 
     q [B*H, S_q, 128] contiguous float16 or bfloat16, k/v packed [B*H, S_kv, 128].  Returns
-    (or fills) ``out`` in q's type and ``out_layout`` "bshd" [B, S_q, H, 128] or "bhsd" [B, H,
-    S_q, 128].  ``kv_valid_len`` int32 [B]: keys at or past it do not count, whatever the
+    (or fills) ``out`` in ``out_dtype`` (q's type, or float32) and ``out_layout`` "bshd" [B, S_q, H,
+    128] or "bhsd" [B, H, S_q, 128].  ``kv_valid_len`` int32 [B]: keys at or past it do not count, whatever the
     cache holds there; a sample without any has zero rows.
 
     ``out`` overlaps no operand.  K and V enter exactly, probabilities to 2^-16; sums are fp32 and the
@@ -253,24 +254,30 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
         shape = (B, H, Sq, D)
     else:
         raise ValueError("out_layout must be 'bshd' or 'bhsd'")
+    if out_dtype is None or out_dtype is qdt:
+        odt, flags = qdt, 0
+    elif out_dtype is _F32:
+        odt, flags = _F32, L.FLAG_OUT_F32
+    else:
+        raise ValueError("out_dtype must be q's type or float32")
     if out is None:
-        out = q.new_empty(shape)
+        out = q.new_empty(shape, dtype=odt)
         ob, s1, s2, _ = out.stride()
     else:
         ob, s1, s2, sd = out.stride() if out.dim() == 4 else (0, 0, 0, 0)
-        if tuple(out.shape) != shape or out.dtype is not qdt or sd != 1 or _repeats(out):
-            raise ValueError("out must have q's type, the layout's shape, a contiguous head dimension and no repeated axis")
+        if tuple(out.shape) != shape or out.dtype is not odt or sd != 1 or _repeats(out):
+            raise ValueError("out must have q's type (or out_dtype's), the layout's shape, a contiguous head dimension and no repeated axis")
     oh, os = (s2, s1) if out_layout == "bshd" else (s1, s2)
     scale = _SCALE if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive")
-    flags = vp = 0
+    vp = 0
     if kv_valid_len is not None:
         vl = kv_valid_len if kv_valid_len.dtype is torch.int32 else kv_valid_len.to(torch.int32)
         vl = vl.contiguous()
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")
-        flags, vp = L.FLAG_MASK, vl.data_ptr()
+        flags, vp = flags | L.FLAG_MASK, vl.data_ptr()
     nbytes = _kv4_workspace(q.get_device(), qdt, B, H, Sq, Skv)
     # Scratch of this call alone, from the caching allocator: freed on return, its block goes
     # to work enqueued later on this stream, and a captured graph keeps it in its own pool.

@@ -1158,7 +1158,7 @@ int anima_attn_kv4_fwd(const AnimaAttnKv4Args* a, void* stream) {
   if (!a || !a->q || !a->k_codes || !a->k_scales || !a->v_codes || !a->v_scales || !a->out)
     return ANIMA_ERR_ARG;
   if (a->dtype != ANIMA_DTYPE_F16 && a->dtype != ANIMA_DTYPE_BF16) return ANIMA_ERR_ARG;
-  if (a->flags & ~ANIMA_FLAG_MASK) return ANIMA_ERR_ARG;
+  if (a->flags & ~(ANIMA_FLAG_MASK | ANIMA_FLAG_OUT_F32)) return ANIMA_ERR_ARG;
   if (!(a->scale > 0.f && a->scale <= 3.402823466e38f)) return ANIMA_ERR_ARG;  // as the core needs it
   if ((a->flags & ANIMA_FLAG_MASK) && !a->kv_valid_len) return ANIMA_ERR_ARG;
   for (int i = 0; i < 3; ++i)

@@ -61,6 +61,7 @@ struct Params {
   int nqb;             // units (blocks of query rows) per (batch, head)
   int units;
   int nsplit;          // clusters that share a unit's keys
+  int out_f32;         // out is fp32, else of q's type
   float scale_log2;
 };
 
@@ -475,8 +476,11 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
     } else if (row0 + row < p.S_q) {
       const float v = sum == 0.f ? 0.f : acc / sum;  // no valid key: zeros
       const long long at = b * p.ob + (bh % p.H) * p.oh + (long long)(row0 + row) * p.os + e % kD;
-      static_cast<uint16_t*>(p.out)[at] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
-                                                : __half_as_ushort(__float2half_rn(v));
+      if (p.out_f32)
+        static_cast<float*>(p.out)[at] = v;
+      else
+        static_cast<uint16_t*>(p.out)[at] = kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v))
+                                                  : __half_as_ushort(__float2half_rn(v));
     }
   }
   cluster_sync();  // no CTA leaves while another reads its shared memory
@@ -620,6 +624,7 @@ int attn_kv4_launch(const AnimaAttnKv4Args* a, int* status, int sm_count, cudaSt
     p.nqb = r.nqb;
     p.units = (int)r.units;
     p.nsplit = r.nsplit;
+    p.out_f32 = (a->flags & ANIMA_FLAG_OUT_F32) != 0;
     p.scale_log2 = std::min(a->scale * 1.4426950408889634f, 3.402823466e38f);
     int rc;
     if (r.warps == 8)

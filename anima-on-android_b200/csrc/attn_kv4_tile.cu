@@ -77,6 +77,7 @@ struct Params {
   int nqb;             // units per (batch, head)
   int units;
   int nsplit;
+  int out_f32;         // out is fp32, else of q's type
   float scale_log2;
 };
 
@@ -669,8 +670,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;  // no key: zeros
       const long long urow = i * kBM + quarter * 32;
       float* const part = direct ? nullptr : p.part + ((long long)s.slice * p.units + s.unit) * kv4_part_floats(kRows);
-      char* const out_w = static_cast<char*>(p.out) +
-                          ((long long)s.b * p.ob + (long long)(s.bh % p.H) * p.oh + (long long)r0 * p.os) * 2;
+      const long long out_at = (long long)s.b * p.ob + (long long)(s.bh % p.H) * p.oh + (long long)r0 * p.os;
 #pragma unroll 1
       for (int c = 0; c < 4 && (direct || n > 0); ++c) {
         float v[32];
@@ -684,13 +684,16 @@ __global__ void __launch_bounds__(kThreads16, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0.f;
         }
-        if (direct)
-          store_block<kBf16 ? ANIMA_DTYPE_BF16 : ANIMA_DTYPE_F16>(out_w, p.os * 2, nvalid, v, c, inv, stage, lane);
-        else
+        if (direct && !p.out_f32) {
+          store_block<kBf16 ? ANIMA_DTYPE_BF16 : ANIMA_DTYPE_F16>(static_cast<char*>(p.out) + out_at * 2, p.os * 2,
+                                                                   nvalid, v, c, inv, stage, lane);
+        } else if (!direct || lane < nvalid) {  // fp32: a partial, or the output
+          float* const to = direct ? static_cast<float*>(p.out) + out_at + lane * p.os : part + (urow + lane) * kD;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(part + (urow + lane) * kD + c * 32 + 4 * e) =
-                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            *reinterpret_cast<float4*>(to + c * 32 + 4 * e) =
+                make_float4(v[4 * e] * inv, v[4 * e + 1] * inv, v[4 * e + 2] * inv, v[4 * e + 3] * inv);
+        }
       }
       if (!direct) {
         part[kRows * kD + urow + lane] = m == -INFINITY ? m : m * sl2_of_m;
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
 
 // Joins the slices of every query row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, in
 // slice order.  One warp per row, four columns per lane; up to 64 slices.  part: [slice][unit][kv4_part_floats(rows)].
-template <bool kBf16>
+template <int kOut>
 __global__ void __launch_bounds__(256)
     kv4_merge_kernel(const float* part, void* out, long long ob, long long oh, long long os, int H, int S_q,
                      int nqb, int rows, int units, int nsplit, long long total) {
@@ -768,15 +771,20 @@ __global__ void __launch_bounds__(256)
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
+    const long long at = (long long)(bh / H) * ob + (long long)(bh % H) * oh + (long long)s * os + lane * 4;
+    if (kOut == ANIMA_DTYPE_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(out) + at) =
+          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      continue;
+    }
     uint32_t w0, w1;
-    if (kBf16) {
+    if (kOut == ANIMA_DTYPE_BF16) {
       w0 = pack_bf16x2(acc.x * inv, acc.y * inv);
       w1 = pack_bf16x2(acc.z * inv, acc.w * inv);
     } else {
       w0 = pack_f16x2(acc.x * inv, acc.y * inv);
       w1 = pack_f16x2(acc.z * inv, acc.w * inv);
     }
-    const long long at = (long long)(bh / H) * ob + (long long)(bh % H) * oh + (long long)s * os + lane * 4;
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(w0, w1);
   }
 }
@@ -821,7 +829,9 @@ static int tile_t(const CUtensorMap& mq, const kv4t::Params& p, int grid, cudaSt
 int kv4_merge_launch(const AnimaAttnKv4Args* a, const float* part, int nqb, int rows, int units, int nsplit,
                      int sm_count, cudaStream_t st) {
   const long long total = (long long)a->B * a->H * a->S_q;
-  auto merge = a->dtype == ANIMA_DTYPE_BF16 ? kv4t::kv4_merge_kernel<true> : kv4t::kv4_merge_kernel<false>;
+  auto merge = (a->flags & ANIMA_FLAG_OUT_F32)   ? kv4t::kv4_merge_kernel<ANIMA_DTYPE_F32>
+               : a->dtype == ANIMA_DTYPE_BF16 ? kv4t::kv4_merge_kernel<ANIMA_DTYPE_BF16>
+                                              : kv4t::kv4_merge_kernel<ANIMA_DTYPE_F16>;
   const int grid = (int)std::min<long long>((total + 7) / 8, (long long)sm_count * 8);
   return launch_dependent(merge, grid, 256, 0, st, part, a->out, (long long)a->out_stride[0],
                           (long long)a->out_stride[1], (long long)a->out_stride[2], a->H, a->S_q, nqb, rows,
@@ -849,6 +859,7 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   p.nqb = t.nqb;
   p.units = (int)t.units;
   p.nsplit = t.nsplit;
+  p.out_f32 = (a->flags & ANIMA_FLAG_OUT_F32) != 0;
   p.scale_log2 = std::min(a->scale * 1.4426950408889634f, 3.402823466e38f);
   CUtensorMap mq;
   int rc = attn_head_map(&mq, a->q, a->dtype, a->B * a->H, a->S_q);

@@ -59,6 +59,7 @@ enum { ANIMA_DTYPE_F32 = 0, ANIMA_DTYPE_BF16 = 1, ANIMA_DTYPE_F16 = 2 };
 #define ANIMA_FLAG_UNIT 0x80u  /* one CTA per 256-row unit                                */
 #define ANIMA_FLAG_WHOLE 0x100u /* persistent grid, whole units only (no workspace)       */
 /* Kernel choice of anima_attn_fwd(_noalloc): */
+#define ANIMA_FLAG_OUT_F32 0x400u /* anima_attn_kv4_fwd: out is fp32 (else of the operands' dtype) */
 #define ANIMA_FLAG_KV64 0x200u /* 64-key tiles with P in tensor-memory columns of its own,
                                   so a query tile's next QK^T overlaps its softmax (the
                                   default kernel uses 128-key tiles with P over S)       */
@@ -360,7 +361,7 @@ int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
  * q [B*H, S_q, 128] contiguous and out (strides {b, h, s} as in anima_attn_fwd, multiples of
  * 8) are of dtype (F16 or BF16), out overlapping no operand; scale is positive; S_q and S_kv go
  * up to 2^30.  flags: ANIMA_FLAG_MASK with kv_valid_len (keys at or past it are not read or do
- * not count, whatever is stored there; none left gives zero rows).
+ * not count, whatever is stored there; none left gives zero rows); ANIMA_FLAG_OUT_F32 for an fp32 out.
  * Little work reads the packed rows directly, more runs on tcgen05 tiles.  Both keep K and V exact (their
  * values are to be in fp16's range, as anima_quantize4 leaves them) and the probabilities to 2^-16, sum in
  * fp32, and round the result once.  The cache is never written out unpacked.

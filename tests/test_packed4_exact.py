@@ -199,3 +199,76 @@ def test_a_large_query_value_leaves_the_others(dtype, Sq):
     out, pv, top = attention_ref(q.double().numpy(), kv, vv, 1, BH, None, 1 / math.sqrt(128))
     err, tol = np.abs(got - out), attention_bound(out, pv, top, dtype, True)
     assert (err <= tol).all(), float((err / tol).max())
+
+
+# ------------------------------------------------------------------ fp32 results
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,H,Sq,Skv,lens", [(2, 3, 1, 77, None), (1, 2, 1, 20011, None), (2, 2, 9, 300, [300, 0]), (1, 1, 5, 9000, [5000]),
+                                             (2, 20, 128, 200, [200, 63]), (1, 2, 2100, 300, None), (2, 1, 300, 5000, [0, 4999]),
+                                             (3, 13, 2049, 130, [0, 130, 40])])
+def test_fp32_results(B, H, Sq, Skv, lens, dtype):
+    """out_dtype float32, in each way, whole and in slices: the result before any 16-bit rounding.  Bound: scores
+    by 512 fp32 steps of sum |q k| scale, exponentials by 2^-20, P in two bf16 parts and V's parts by
+    2^-16, sums and merges by 2^-17; numerator and denominator, so twice."""
+    g = torch.Generator().manual_seed(61)
+    q = torch.randn(B * H, Sq, 128, generator=g).to(dtype).cuda()
+    k, kv = random_packed((1, Skv, 128), 62)
+    v, vv = random_packed((1, Skv, 128), 63)
+    k, v = every_head(k, B * H), every_head(v, B * H)
+    kv, vv = (np.broadcast_to(t, (B * H,) + t.shape[1:]) for t in (kv, vv))
+    vl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=vl, out_dtype=F32)
+    assert got.dtype == F32 and got.shape == (B, Sq, H, 128)
+    out, pv, top = attention_ref(q.double().cpu().numpy(), kv, vv, B, H, lens, 1 / math.sqrt(128))
+    err = np.abs(got.double().cpu().numpy() - out)
+    tol = pv * 2 * (512 * 2.0 ** -23 * top + 2.0 ** -20 + 2.0 ** -16 + 2.0 ** -17) + 1e-37
+    assert (err <= tol).all(), float((err / np.maximum(tol, 1e-300)).max())
+    if np.abs(out).max() > 0:
+        assert np.linalg.norm(err) <= 2.0 ** -15 * np.linalg.norm(out)  # a 16-bit rounding alone is 2^-12 and more
+    # the 16-bit result is this one rounded
+    assert torch.equal(anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=vl), got.to(dtype))
+    buf = torch.full((B, H + 1, Sq + 1, 136), 7.0, device="cuda")
+    view = buf[:, :H, 1:, :128]
+    assert anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=vl, out=view, out_layout="bhsd", out_dtype=F32) is view
+    assert torch.equal(view.transpose(1, 2), got)
+    view.fill_(7.0)
+    assert (buf == 7).all()
+
+
+@pytest.mark.gpu
+def test_cached_kv_results_are_fp32_by_default():
+    """attention_cached_kv over packed K/V writes fp32 results, as it does over 16-bit ones; other types are
+    theirs rounded."""
+    from anima_attn.ops import attention_cached_kv, prologue
+    g = torch.Generator(device="cuda").manual_seed(64)
+    B, S, H, N = 2, 300, 2, 130
+    q = torch.randn(B, S, H, 128, device="cuda", generator=g)
+    k, kv = random_packed((B * H, N, 128), 65)
+    v, vv = random_packed((B * H, N, 128), 66)
+    got = attention_cached_kv(q, k, v)
+    qh, _, _ = prologue(q, None, None, None, None, None, 1e-6, True, False, F16)
+    out, _, _ = attention_ref(qh.double().cpu().numpy(), kv, vv, B, H, None, 1 / math.sqrt(128))
+    assert got.dtype == F32 and np.linalg.norm(got.double().cpu().numpy() - out) <= 2.0 ** -15 * np.linalg.norm(out)
+    assert torch.equal(attention_cached_kv(q, k, v, out_dtype=F16), got.half())
+    for dt in (F32, F16, BF16):
+        buf = torch.empty(B, S, H, 128, dtype=dt, device="cuda")
+        assert attention_cached_kv(q, k, v, out=buf) is buf and torch.equal(buf, got.to(dt))
+    for bad in (torch.empty(2 * B, S, H, 128, dtype=dt, device="cuda") for dt in (F32, F16, BF16)):
+        with pytest.raises(ValueError):
+            attention_cached_kv(q, k, v, out=bad)
+    with pytest.raises(ValueError):
+        attention_cached_kv(q[:1], k, v)
+    one = torch.empty(2, 1, S, H, 128, dtype=BF16, device="cuda")  # would broadcast
+    with pytest.raises(ValueError):
+        attention_cached_kv(q, k, v, out=one.expand(2, B, S, H, 128))
+
+
+def test_output_types_that_are_refused(monkeypatch):
+    monkeypatch.setattr(anima_attn.packed, "_here", lambda *ts: 0)
+    q = torch.zeros(4, 3, 128, dtype=F16)
+    k = Packed4(torch.zeros(4, 5, 64, dtype=torch.uint8), torch.zeros(4, 5, 4, dtype=F16))
+    for kw in ({"out_dtype": BF16}, {"out_dtype": torch.float64}, {"out": torch.zeros(2, 3, 2, 128)},
+               {"out_dtype": F32, "out": torch.zeros(2, 3, 2, 128, dtype=F16)}):
+        with pytest.raises(ValueError):
+            anima_attn.attention_core_kv4(q, k, k, 2, 2, **kw)
