@@ -169,8 +169,7 @@ def matvec4(x: torch.Tensor, w: Packed4, silu: bool = False, add: Optional[torch
     float16 or bfloat16 with a contiguous last axis (other strides are free); ``add`` is float32
     and broadcasts to the result [.., M, N] over its leading axes; the result has ``out``'s or
     ``out_dtype``'s type; ``out`` may be ``add`` itself, and overlaps no other operand.  Sums are
-    fp32 over exact products, and of float32 x only what is below 2^-31 of its group's largest
-    is lost, so the result is an fp32 one rounded once.  8 float32 rows or 16 16-bit ones
+    fp32 over exact products, every value of x with all its bits; the result is rounded once.  8 float32 rows or 16 16-bit ones
     share a pass over W."""
     codes, scales = w
     stream = _here(x, codes, scales, add, out)

@@ -200,18 +200,15 @@ __global__ void __launch_bounds__(256)
 //
 // 16-bit rows (kF16, kBf16) are a column each of m16n8k16, codes unpacked to n in their type.
 //
-// fp32 rows and SiLU's results (kDigits) are four columns each of the whole-number MMA m16n8k32.  Per
-// group of 32, x is scaled by the power of two that takes the largest below 2^30, rounded to a whole
-// number and written in four signed base-256 digits, so nothing above 2^-31 of the group's largest
-// magnitude is lost, more than an fp32 sum keeps.  A word's codes are its bytes' halves, c = n + 8, three
-// instructions for eight where bf16 takes eleven; the 8 goes into the accumulator's start value, -8
-// sum(digits), together with the 1.5 * 2^23 that makes the whole sum an fp32's low bits.
+// fp32 rows and SiLU's results (kParts) are three bf16 columns each: a value cut after 8 and after 16 bits is
+// the exact sum of three bf16, whatever stands beside it.  Per group of 32, x is first scaled by the power of
+// two that takes the largest to 2^100 (2^126 at most), so that sums of parts stay in fp32's range and the
+// lowest parts in bf16's.  (As whole numbers of 2^-30 of a group's largest value, in four base-256 digits for the
+// whole-number MMA, 84 x 6144 x 256 took a fifth less, and values far below the group's largest lost their bits.)
 //
-// 84 matrices of 6144 x 256 with two fp32 rows take 19.6 us (4.0 TB/s of codes, scales and results; 12 at
-// the copy rate): 194 instructions a block of 16 x 128 weights at 0.65 a cycle and scheduler, of which
-// the tile's ends are a fifth with two blocks a row, and about 3 us of start, when x is staged.
-// As three bf16 columns a row, codes unpacked to bf16, they took 24.  One 6144 x 2048 matrix and row
-// takes 5.1 us, one 21504 x 2048 with SiLU and two rows 10.8.
+// 84 matrices of 6144 x 256 with two fp32 rows take 23.4 us (3.3 TB/s of codes, scales and results; 12 at
+// the copy rate), bound by instruction issue, the unpacking to bf16 first, and some 3 us of start, when x
+// is staged.  One 6144 x 2048 matrix and row takes 5.4 us, one 21504 x 2048 with SiLU and two rows 11.9.
 //
 // A CTA of 8 warps works on one matrix, on a run of tiles of 16 rows of W; `split` warps share a
 // tile, taking its 128-value blocks in turn, and their sums meet in shared memory in a fixed
@@ -244,17 +241,15 @@ __device__ __forceinline__ float load_x(const Mv4Params& p, long long at) {
                                        : __half2float(__ushort_as_half(u));
 }
 
-enum { kF16 = 0, kBf16 = 1, kDigits = 2 };
+enum { kF16 = 0, kBf16 = 1, kParts = 2 };
 
 // Bytes between staged columns, and of all staged data.
-template <int kMode>
 __host__ __device__ constexpr int mv4_stride(int K) {
-  return kMode == kDigits ? K + 32 : 2 * K + 64;
+  return 2 * K + 64;
 }
 template <int kMode>
 __host__ __device__ constexpr size_t mv4_staged(int M, int K, int nb) {
-  return kMode == kDigits ? (size_t)4 * M * mv4_stride<kMode>(K) + (size_t)(K / 32) * nb * 72
-                          : (size_t)M * mv4_stride<kMode>(K);
+  return kMode == kParts ? (size_t)3 * M * mv4_stride(K) + (size_t)(K / 32) * nb * 8 : (size_t)M * mv4_stride(K);
 }
 
 // Eight values of x, SiLU applied if asked for.
@@ -272,63 +267,43 @@ __device__ __forceinline__ void load_x8(const Mv4Params& p, long long at, float 
     for (int k = 0; k < 8; ++k) v[k] = __fdividef(v[k], 1.0f + expf(-v[k]));
 }
 
-// Stages the rows of x as digits.  A lane takes 8 values; the four lanes of a group share its
-// exponent.  cols: digit q of value e at [4 m + q][32 g + 8 i + place of e], in the order in which the
-// code words' halves come (values 0 4 1 5, then 2 6 3 7).  start[g][pair of columns]: the start values of
-// a lane's four accumulators; xscale[g][m]: the group's scale 2^(E - 6), E with largest magnitude
-// below 2^E.
-__device__ __forceinline__ void stage_digits(const Mv4Params& p, int e, int nb, uint8_t* cols, uint4* start,
-                                             float* xscale) {
-  const int stride = mv4_stride<kDigits>(p.K), runs = p.K / 8;
+// Stages the rows of x in three parts.  A lane takes 8 values; the four lanes of a group share its scale.
+// cols: part q of row m at column 3 m + q; xscale[g][m]: what the group's sums are multiplied by, 2^-a.
+__device__ __forceinline__ void stage_parts(const Mv4Params& p, int e, int nb, uint8_t* cols, float* xscale) {
+  const int stride = mv4_stride(p.K), runs = p.K / 8;
+  const uint32_t group = 0xfu << (threadIdx.x & 28);  // K / 8 is a multiple of 16: its lanes stay together
   for (int c = threadIdx.x; c < p.M * runs; c += kMvThreads) {
-    const uint32_t mask = __activemask();  // K / 8 is a multiple of 16: a group's lanes stay together
     const int m = c / runs, r = c - m * runs;
     float v[8];
     load_x8(p, (long long)e * p.xe + (long long)m * p.xm + 8 * r, v);
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(group, top, 1));
+    top = max(top, __shfl_xor_sync(group, top, 2));
+    const bool finite = top < 0x7f800000u;
+    const int E = max((int)(top >> 23), 1) - 126;  // largest magnitude below 2^E
+    const int a = finite ? min(100 - E, 126) : 0;
+    const float f = __int_as_float((a + 127) << 23);
+    uint32_t part[3][8];
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-    const int E = max((int)(top >> 23), 1) - 126;
-    uint32_t t[8];
-    float scale;
-    if (top < 0x7f800000u) {
-      const int s0 = (30 - E) / 2, s1 = 30 - E - s0;  // in two steps: neither leaves fp32
-      const float f0 = __int_as_float((s0 + 127) << 23), f1 = __int_as_float((s1 + 127) << 23);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)  // the signed digits as bytes: add 128 to the lower three, then flip
-        t[k] = ((uint32_t)__float2int_rn(v[k] * f0 * f1) + 0x00808080u) ^ 0x00808080u;
-      scale = E - 6 >= -126 ? __int_as_float((E - 6 + 127) << 23) : __int_as_float(1 << (E - 6 + 149));
-    } else {
-      // one infinity makes its products infinite or NaN and hides the rest; anything else is NaN
-      int odd = 0;  // infinities of the group, two for a NaN
-#pragma unroll
-      for (int k = 0; k < 8; ++k) odd += isnan(v[k]) ? 2 : isinf(v[k]) ? 1 : 0;
-      const uint32_t group = 0xfu << (threadIdx.x & 28);  // its four lanes come here together
-      odd += __shfl_xor_sync(group, odd, 1);
-      odd += __shfl_xor_sync(group, odd, 2);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        t[k] = isinf(v[k]) ? (v[k] > 0.f ? 0x01010101u : 0xffffffffu) : 0u;
-      scale = odd == 1 ? INFINITY : NAN;
+    for (int k = 0; k < 8; ++k) {
+      const float y = v[k] * f;
+      part[0][k] = __float_as_uint(y) & 0xffff0000u;
+      const float y1 = y - __uint_as_float(part[0][k]);
+      part[1][k] = __float_as_uint(y1) & 0xffff0000u;
+      part[2][k] = __float_as_uint(y1 - __uint_as_float(part[1][k]));
+      if (!finite) {  // infinities and NaN decide the sums alone
+        part[0][k] = isnan(v[k]) ? 0x7fff0000u : isinf(v[k]) ? __float_as_uint(v[k]) : 0u;
+        part[1][k] = part[2][k] = 0u;
+      }
     }
-    uint32_t sum[4];
-    const int g = r >> 2, i = r & 3;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {  // digit q is byte 3 - q
-      const uint32_t sel = (uint32_t)(3 - q) | (uint32_t)(7 - q) << 4;
-      const uint32_t lo = __byte_perm(__byte_perm(t[0], t[4], sel), __byte_perm(t[1], t[5], sel), 0x5410);
-      const uint32_t hi = __byte_perm(__byte_perm(t[2], t[6], sel), __byte_perm(t[3], t[7], sel), 0x5410);
-      *reinterpret_cast<uint2*>(cols + (size_t)(4 * m + q) * stride + 32 * g + 8 * i) = make_uint2(lo, hi);
-      int s = __dp4a((int)lo, 0x01010101, __dp4a((int)hi, 0x01010101, 0));
-      s += __shfl_xor_sync(mask, s, 1);
-      s += __shfl_xor_sync(mask, s, 2);
-      sum[q] = 0x4b400000u - 8u * (uint32_t)s;
-    }
-    if (i < 2)  // pair 2 m: digits 0 and 1; pair 2 m + 1: digits 2 and 3
-      start[g * 4 * nb + 2 * m + i] = i ? make_uint4(sum[2], sum[3], sum[2], sum[3]) : make_uint4(sum[0], sum[1], sum[0], sum[1]);
-    if (i == 2) xscale[g * 2 * nb + m] = scale;
+    for (int q = 0; q < 3; ++q)
+      *reinterpret_cast<uint4*>(cols + (size_t)(3 * m + q) * stride + 16 * r) =
+          make_uint4(__byte_perm(part[q][0], part[q][1], 0x7632), __byte_perm(part[q][2], part[q][3], 0x7632),
+                     __byte_perm(part[q][4], part[q][5], 0x7632), __byte_perm(part[q][6], part[q][7], 0x7632));
+    if ((r & 3) == 0) xscale[(r >> 2) * 2 * nb + m] = __int_as_float((127 - a) << 23);
   }
 }
 
@@ -339,16 +314,15 @@ template <int kMode, int kNB, int kStages>
 __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   grid_dependency_wait();  // launched while the kernel before it drains
-  constexpr bool kDig = kMode == kDigits;
-  constexpr int kOuts = kDig ? 1 : 4;  // results of a lane per block of columns
+  constexpr bool kWide = kMode == kParts;
+  constexpr int kOuts = kWide ? 1 : 4;  // results of a lane per block of columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = lane >> 2, i = lane & 3;
-  const int stride = mv4_stride<kMode>(p.K);
+  const int stride = mv4_stride(p.K);
   const uint32_t ring = smem_u32(smem) + warp * kStages * kMvStage;
   float* const red = reinterpret_cast<float*>(smem + 8 * kStages * kMvStage);
   uint8_t* const cols = reinterpret_cast<uint8_t*>(red + 8 * 32 * kNB * kOuts);
-  uint4* const start = reinterpret_cast<uint4*>(cols + (size_t)4 * p.M * stride);  // kDigits
-  float* const xscale = reinterpret_cast<float*>(start + (p.K / 32) * 4 * kNB);
+  float* const xscale = reinterpret_cast<float*>(cols + (size_t)3 * p.M * stride);  // kParts
   const int split = 1 << p.log_split;
   const int s = warp & (split - 1), t = warp >> p.log_split, tiles = 8 >> p.log_split;
   const int blocks = p.K / p4::kBlock;
@@ -403,8 +377,8 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
 #pragma unroll
   for (int k = 0; k < kStages - 1; ++k) fetch();
 
-  if constexpr (kDig) {
-    stage_digits(p, e, kNB, cols, start, xscale);
+  if constexpr (kWide) {
+    stage_parts(p, e, kNB, cols, xscale);
   } else {  // 16-bit rows as they are
     const uint16_t* const x = static_cast<const uint16_t*>(p.x) + (long long)e * p.xe;
     if (p.x_aligned) {
@@ -426,16 +400,16 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
   uint32_t xa[kNB];  // this lane's column of x, at its eight values of a group
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
-    const int col = kDig ? 4 * min(nb * 2 + (j >> 2), p.M - 1) + (j & 3) : min(nb * 8 + j, p.M - 1);
-    xa[nb] = smem_u32(cols) + col * stride + (kDig ? 8 : 16) * i;
+    const int col = kWide ? 3 * min(nb * 2 + (j >> 2), p.M - 1) + min(j & 3, 2) : min(nb * 8 + j, p.M - 1);
+    xa[nb] = smem_u32(cols) + col * stride + 16 * i;
   }
-  const uint32_t sa = smem_u32(start) + 16 * i, fa = smem_u32(xscale) + 4 * (i >> 1);
+  const uint32_t fa = smem_u32(xscale) + 4 * (i >> 1);
   __syncthreads();
 
   // Result r of this lane for column block nb is row `row + out_row(r)`, row m = out_m(nb, r) of x.
-  auto out_row = [&](int r) { return kDig ? 0 : 8 * (r >> 1); };
-  auto out_m = [&](int nb, int r) { return kDig ? nb * 2 + (i >> 1) : nb * 8 + 2 * i + (r & 1); };
-  int row = (g_lo * tiles + t) * 16 + j + (kDig ? 8 * (i & 1) : 0);
+  auto out_row = [&](int r) { return kWide ? 0 : 8 * (r >> 1); };
+  auto out_m = [&](int nb, int r) { return kWide ? nb * 2 + (i >> 1) : nb * 8 + 2 * i + (r & 1); };
+  int row = (g_lo * tiles + t) * 16 + j + (kWide ? 8 * (i & 1) : 0);
   long long out_at[kNB], add_at[kNB];
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
@@ -459,7 +433,7 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
     for (int b = 0; b < kNB; ++b)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[b][c] = 0.f;
-    uint64_t acc2[kNB][2];  // kDigits: the same as pairs
+    uint64_t acc2[kNB][2];  // kParts: the same as pairs
 #pragma unroll
     for (int b = 0; b < kNB; ++b) acc2[b][0] = acc2[b][1] = 0ull;
     for (int blk = s; blk < blocks; blk += split) {
@@ -474,34 +448,21 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
       const float g0[4] = {f0.x, f0.y, f0.z, f0.w}, g1[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        if constexpr (kDig) {
-          constexpr uint32_t kHalf = 0x0f0f0f0fu;
-          const uint32_t a0 = w0[g] & kHalf, a2 = (w0[g] >> 4) & kHalf;
-          const uint32_t a1 = w1[g] & kHalf, a3 = (w1[g] >> 4) & kHalf;
+        uint32_t a[4], b[4];
+        p4::numbers<kMode != kF16>(w0[g], a);
+        p4::numbers<kMode != kF16>(w1[g], b);
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
-            const uint2 xv = p4::lds8(xa[nb] + blk * p4::kBlock + 32 * g);
-            const uint4 c4 = p4::lds16(sa + ((blk * 4 + g) * kNB + nb) * 64);
+        for (int nb = 0; nb < kNB; ++nb) {
+          const uint4 xv = p4::lds16(xa[nb] + blk * (2 * p4::kBlock) + 64 * g);
+          float d[4];
+          p4::mma16816_zero<kMode != kF16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+          p4::mma16816<kMode != kF16>(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
+          if constexpr (kWide) {  // the scale of W first: that of x may be near fp32's ends
             const float sx = p4::lds4(fa + ((blk * 4 + g) * kNB + nb) * 8);
-            int d[4];
-            p4::mma16832(d, a0, a1, a2, a3, xv.x, xv.y, c4);
-            const float s0 = g0[g] * sx, s1 = g1[g] * sx;
-            const uint64_t off = f2pack(-12582912.f, -12582912.f);
-            const uint64_t v0 = add2(f2pack(__int_as_float(d[0]), __int_as_float(d[1])), off);
-            const uint64_t v1 = add2(f2pack(__int_as_float(d[2]), __int_as_float(d[3])), off);
-            acc2[nb][0] = fma2(f2pack(s0, s0), v0, acc2[nb][0]);
-            acc2[nb][1] = fma2(f2pack(s1, s1), v1, acc2[nb][1]);
-          }
-        } else {
-          uint32_t a[4], b[4];
-          p4::numbers<kMode == kBf16>(w0[g], a);
-          p4::numbers<kMode == kBf16>(w1[g], b);
-#pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
-            const uint4 xv = p4::lds16(xa[nb] + blk * (2 * p4::kBlock) + 64 * g);
-            float d[4];
-            p4::mma16816_zero<kMode == kBf16>(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
-            p4::mma16816<kMode == kBf16>(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
+            const uint64_t s0 = f2pack(g0[g], g0[g]), s1 = f2pack(g1[g], g1[g]), sx2 = f2pack(sx, sx);
+            acc2[nb][0] = fma2(fma2(f2pack(d[0], d[1]), s0, 0ull), sx2, acc2[nb][0]);
+            acc2[nb][1] = fma2(fma2(f2pack(d[2], d[3]), s1, 0ull), sx2, acc2[nb][1]);
+          } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[nb][c] = fmaf(c < 2 ? g0[g] : g1[g], d[c], acc[nb][c]);
           }
@@ -510,12 +471,11 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
     }
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
-      if constexpr (kDig) {  // digits 2 (i % 2) and the next of rows j and j + 8, then the other lane's
-        const float f = (i & 1) ? 1.52587890625e-05f : 1.0f;  // 2^-16
+      if constexpr (kWide) {  // parts 0 and 1 of rows j and j + 8, or part 2 (twice), and the other lane's
         f2unpack(acc2[nb][0], acc[nb][0], acc[nb][1]);
         f2unpack(acc2[nb][1], acc[nb][2], acc[nb][3]);
-        float v0 = fmaf(acc[nb][1], 0.00390625f, acc[nb][0]) * f;
-        float v1 = fmaf(acc[nb][3], 0.00390625f, acc[nb][2]) * f;
+        float v0 = (i & 1) ? acc[nb][0] : acc[nb][0] + acc[nb][1];
+        float v1 = (i & 1) ? acc[nb][2] : acc[nb][2] + acc[nb][3];
         v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
         v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
         y[nb][0] += (i & 1) ? v1 : v0;
@@ -618,7 +578,7 @@ constexpr size_t mv4_fixed_smem(int nb, int outs, int stages) {
 template <int kMode, int kNB, int kStages>
 static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
   auto kern = matvec4_kernel<kMode, kNB, kStages>;
-  const size_t smem = mv4_fixed_smem(kNB, kMode == kDigits ? 1 : 4, kStages) + mv4_staged<kMode>(p.M, p.K, kNB);
+  const size_t smem = mv4_fixed_smem(kNB, kMode == kParts ? 1 : 4, kStages) + mv4_staged<kMode>(p.M, p.K, kNB);
   if (smem > kMaxSmem) return ANIMA_ERR_SHAPE;
   static SmemAttr attr;
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
@@ -648,21 +608,21 @@ static int mv4_t(Mv4Params p, int E, int sm_count, cudaStream_t st) {
 
 // Rows of x of one launch: eight fp32 rows or sixteen 16-bit ones; fewer where their columns
 // would not fit shared memory, and a shorter ring where not even one would.
-static int mv4_rows(int K, bool digits, int* stages) {
+static int mv4_rows(int K, bool wide, int* stages) {
   *stages = 4;
-  for (int m = digits ? 8 : 16; m > 0; --m) {
-    const size_t staged = digits ? mv4_staged<kDigits>(m, K, m <= 2 ? 1 : m <= 4 ? 2 : 4) : mv4_staged<kF16>(m, K, 1);
-    if (staged + mv4_fixed_smem(digits ? 4 : 2, digits ? 1 : 4, 4) <= kMaxSmem) return m;
+  for (int m = wide ? 8 : 16; m > 0; --m) {
+    const size_t staged = wide ? mv4_staged<kParts>(m, K, m <= 2 ? 1 : m <= 4 ? 2 : 4) : mv4_staged<kF16>(m, K, 1);
+    if (staged + mv4_fixed_smem(wide ? 4 : 2, wide ? 1 : 4, 4) <= kMaxSmem) return m;
   }
   *stages = 2;
-  const size_t staged = digits ? mv4_staged<kDigits>(1, K, 1) : mv4_staged<kF16>(1, K, 1);
-  return staged + mv4_fixed_smem(1, digits ? 1 : 4, 2) <= kMaxSmem ? 1 : 0;
+  const size_t staged = wide ? mv4_staged<kParts>(1, K, 1) : mv4_staged<kF16>(1, K, 1);
+  return staged + mv4_fixed_smem(1, wide ? 1 : 4, 2) <= kMaxSmem ? 1 : 0;
 }
 
 int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
-  const bool digits = a->x_dtype == ANIMA_DTYPE_F32 || a->silu;
+  const bool wide = a->x_dtype == ANIMA_DTYPE_F32 || a->silu;
   int stages;
-  const int rows = mv4_rows(a->K, digits, &stages);
+  const int rows = mv4_rows(a->K, wide, &stages);
   if (rows < 1) return ANIMA_ERR_SHAPE;
   Mv4Params p;
   p.codes = static_cast<const uint8_t*>(a->codes);
@@ -688,13 +648,13 @@ int matvec4_launch(const AnimaMatvec4Args* a, int sm_count, cudaStream_t st) {
     const bool bf = a->x_dtype == ANIMA_DTYPE_BF16, one = p.M <= 8;
     int rc;
     if (stages == 2)
-      rc = digits ? mv4_t<kDigits, 1, 2>(p, a->E, sm_count, st)
+      rc = wide ? mv4_t<kParts, 1, 2>(p, a->E, sm_count, st)
            : bf   ? mv4_t<kBf16, 1, 2>(p, a->E, sm_count, st)
                   : mv4_t<kF16, 1, 2>(p, a->E, sm_count, st);
-    else if (digits)
-      rc = p.M <= 2   ? mv4_t<kDigits, 1, 4>(p, a->E, sm_count, st)
-           : p.M <= 4 ? mv4_t<kDigits, 2, 4>(p, a->E, sm_count, st)
-                      : mv4_t<kDigits, 4, 4>(p, a->E, sm_count, st);
+    else if (wide)
+      rc = p.M <= 2   ? mv4_t<kParts, 1, 4>(p, a->E, sm_count, st)
+           : p.M <= 4 ? mv4_t<kParts, 2, 4>(p, a->E, sm_count, st)
+                      : mv4_t<kParts, 4, 4>(p, a->E, sm_count, st);
     else if (bf)
       rc = one ? mv4_t<kBf16, 1, 4>(p, a->E, sm_count, st) : mv4_t<kBf16, 2, 4>(p, a->E, sm_count, st);
     else

@@ -330,11 +330,9 @@ int anima_dequantize4(const void* codes, const void* scales, void* y, int dtype,
  * Matrix-vector products with packed weights: for e < E, m < M, n < N
  *   out[e, m, n] = sum_k f(x[e, m, k]) W[e, n, k] + add[e, m, n],  f = SiLU if silu, else x.
  * W: packed rows [E, N] of K values.  x, add (fp32, or NULL) and out are addressed by element
- * strides {e, m} (0 repeats), their last axis contiguous; x and out F32, F16 or BF16.  The
- * products are exact, sums are fp32; fp32 rows (and SiLU of any) enter as whole numbers below
- * 2^30, one scale per group of 32 (values below 2^-31 of the group's largest count as 0), so the
- * result has fp32 accuracy before its one rounding.  One infinity in a group of x gives what
- * it should, several give NaN.  Up to 8 fp32 or 16 16-bit rows share one pass over W; more rows
+ * strides {e, m} (0 repeats), their last axis contiguous; x and out F32, F16 or BF16.  Every
+ * value of x enters with all its bits, also beside far larger ones, products are exact, sums are
+ * fp32, and the result is rounded once.  Infinities and NaN give what an fp32 sum gives.  Up to 8 fp32 or 16 16-bit rows share one pass over W; more rows
  * take further passes.  K up to ANIMA_MATVEC4_MAX_K, N up to 2^30.  E, M or N = 0 does nothing.
  * out may be add at the same strides, else it overlaps no operand.  Asynchronous on `stream`.
  */

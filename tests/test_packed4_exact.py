@@ -272,3 +272,65 @@ def test_output_types_that_are_refused(monkeypatch):
                {"out_dtype": F32, "out": torch.zeros(2, 3, 2, 128, dtype=F16)}):
         with pytest.raises(ValueError):
             anima_attn.attention_core_kv4(q, k, k, 2, 2, **kw)
+
+
+# ------------------------------------------------------------------ matvec4: every value keeps its bits
+def matvec_bound_each(ax, aw, K, y, out_dtype, steps=0):
+    """Rounding bound of one result of sum |x| |w| alone, wherever the other values of a group lie.  A
+    value is three bf16 parts, together exact; their products with whole numbers are exact.  A group's 3 x
+    32 products are summed by the tensor core (one fp32 step each), K/32 scaled sums are rounded, at most 8
+    warps', the three parts', the addend: 96 + K/32 + 16 steps.  `steps` more for what x itself is off by.
+    Results and sums below fp32's normal range round to multiples of 2^-149."""
+    S = ax @ np.swapaxes(aw, -1, -2)
+    return S * 2.0 ** -23 * (96 + K / 32 + 16 + steps) + (K / 32 + 16) * 2.0 ** -148 + np.abs(y) * half_step(out_dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 8, 9])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e20, 3.4e38])
+def test_matvec_outliers_leave_the_others(size, M):
+    """A group's largest value meets weights of zero: what is left is the other values' sum, to fp32's
+    accuracy (relative to sum |x| |w|, in which the large value has no part)."""
+    rng = np.random.default_rng(41)
+    N, K = 50, 384
+    n = rng.integers(-8, 8, (N, K))
+    n[:, [7, 40, 200]] = 0
+    w, wv = packed(n, rng.uniform(0.01, 0.1, (N, K // 32)))
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(42))
+    x[:, 7], x[:, 40], x[:, 200] = size, -size, size / 3
+    y = anima_attn.matvec4(x.cuda(), w).double().cpu().numpy()
+    xv = x.double().numpy()
+    want = xv @ wv.T
+    err, tol = np.abs(y - want), matvec_bound_each(np.abs(xv), np.abs(wv), K, want, F32)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("std", [1e-43, 1e-38, 1e-30, 1e30, 2e36])
+def test_matvec_over_the_range_of_fp32(std):
+    g = torch.Generator().manual_seed(43)
+    w, wv = random_packed((64, 256), 44, std=0.05)
+    x = torch.randn(2, 256, generator=g) * std
+    y = anima_attn.matvec4(x.cuda(), w).double().cpu().numpy()
+    xv = x.double().numpy()
+    want = xv @ wv.T
+    err, tol = np.abs(y - want), matvec_bound_each(np.abs(xv), np.abs(wv), 256, want, F32)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.gpu
+def test_matvec_several_infinities():
+    """Infinities of a group whose products agree give that infinity, as a sum in fp32 does."""
+    n = np.ones((4, 256), np.int64)
+    n[1], n[2, 9] = -1, 0
+    w, _ = packed(n, np.full((4, 8), 0.5))
+    x = torch.ones(1, 256)
+    x[0, 9] = x[0, 20] = x[0, 100] = math.inf
+    y = anima_attn.matvec4(x.cuda(), w).cpu()[0]
+    assert y[0] == math.inf and y[1] == -math.inf and y[2].isnan() and y[3] == math.inf
+    x[0, 20] = -math.inf
+    assert anima_attn.matvec4(x.cuda(), w).isnan().all()
+    # a NaN whose upper 16 bits alone are an infinity's
+    x = torch.ones(1, 256)
+    x.view(torch.int32)[0, 9] = 0x7F800001
+    assert anima_attn.matvec4(x.cuda(), w).isnan().all()
