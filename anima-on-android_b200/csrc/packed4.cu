@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256)
 //
 // 84 matrices of 6144 x 256 with two fp32 rows take 23.4 us (3.3 TB/s of codes, scales and results; 12 at
 // the copy rate), bound by instruction issue, the unpacking to bf16 first, and some 3 us of start, when x
-// is staged.  One 6144 x 2048 matrix and row takes 5.4 us, one 21504 x 2048 with SiLU and two rows 11.9.
+// is staged.  One 6144 x 2048 matrix and row takes 5.7 us, one 21504 x 2048 with SiLU and two rows 12.6.
 //
 // A CTA of 8 warps works on one matrix, on a run of tiles of 16 rows of W; `split` warps share a
 // tile, taking its 128-value blocks in turn, and their sums meet in shared memory in a fixed
@@ -264,7 +264,7 @@ __device__ __forceinline__ void load_x8(const Mv4Params& p, long long at, float 
   }
   if (p.silu)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = __fdividef(v[k], 1.0f + expf(-v[k]));
+    for (int k = 0; k < 8; ++k) v[k] = v[k] / (1.0f + expf(-v[k]));  // a true quotient: __fdividef is 0 from 2^126 on
 }
 
 // Stages the rows of x in three parts.  A lane takes 8 values; the four lanes of a group share its scale.

@@ -334,3 +334,23 @@ def test_matvec_several_infinities():
     x = torch.ones(1, 256)
     x.view(torch.int32)[0, 9] = 0x7F800001
     assert anima_attn.matvec4(x.cuda(), w).isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_matvec_silu_of_large_negative_values(dtype):
+    """SiLU(-88) is -88 e^-88 = -5e-37, inside fp32's range; further down it goes to 0, and -infinity to NaN.
+    Bound on x: 8 steps as elsewhere, and |x| + 2 steps for the rounding of the exponential of x."""
+    w, wv = packed(np.ones((16, 128), np.int64), np.ones((16, 4)))
+    for lo, hi in ((-88.6, -87.0), (-103.0, -88.5), (-87.0, -60.0)):
+        x = torch.linspace(lo, hi, 128)[None].to(dtype)
+        xv = x.double().numpy()
+        sv = xv / (1 + np.exp(-xv))
+        sv[xv < -88.72] = 0  # e^-x leaves fp32: below 2^-121 in the result
+        y = anima_attn.matvec4(x.cuda(), w, silu=True).double().cpu().numpy()
+        want = sv @ wv.T
+        tol = matvec_bound_each(np.abs(sv), np.abs(wv), 128, want, F32, steps=8 + 105)
+        near = (np.abs(xv + 88.72) < 0.01).sum() * 88.73 * math.exp(-88.71)  # may fall on either side
+        assert (np.abs(y - want) <= tol + near).all()
+    x = torch.full((1, 128), -math.inf, dtype=dtype)
+    assert anima_attn.matvec4(x.cuda(), w, silu=True).isnan().all()
