@@ -570,7 +570,6 @@ int dequantize4_launch(const void* codes, const void* scales, void* y, int dtype
   return cudaGetLastError() == cudaSuccess ? ANIMA_OK : ANIMA_ERR_CUDA;
 }
 
-constexpr size_t kMaxSmem = 227 * 1024;
 constexpr size_t mv4_fixed_smem(int nb, int outs, int stages) {
   return 8 * stages * kMvStage + 8 * 32 * nb * outs * sizeof(float);
 }

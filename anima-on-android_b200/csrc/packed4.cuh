@@ -13,10 +13,10 @@
 // numbers n, exact in fp16 and bf16.  Within a word, nibbles p and p + 4 are neighbours e =
 // 2 p, 2 p + 1, so masking with 0x000f000f leaves a pair in consecutive order.
 #pragma once
-#include <atomic>
 #include <utility>
 
 #include "common.cuh"
+#include "smem_attr.cuh"
 
 namespace anima {
 namespace p4 {
@@ -198,28 +198,5 @@ static int launch_dependent(void (*kern)(Params...), int grid, int threads, size
                             Args&&... args) {
   return launch_clusters(kern, grid, 0, threads, smem, st, std::forward<Args>(args)...);
 }
-
-// Largest dynamic shared memory asked for a kernel so far, per device: the attribute is set when
-// a launch needs more, not at every launch.
-struct SmemAttr {
-  std::atomic<size_t> most[64];
-  SmemAttr() {
-    for (auto& m : most) m.store(0);
-  }
-  bool raise(const void* kern, size_t bytes) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    if (bytes <= most[dev].load(std::memory_order_acquire)) return true;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-      cudaGetLastError();
-      return false;
-    }
-    // a larger size set by another thread in between stays recorded or is set again
-    size_t seen = most[dev].load();
-    while (seen < bytes && !most[dev].compare_exchange_weak(seen, bytes)) {
-    }
-    return true;
-  }
-};
 
 }  // namespace anima
