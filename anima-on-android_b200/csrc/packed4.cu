@@ -73,8 +73,8 @@ __device__ __forceinline__ const uint4* unit_ptr(const Quant4Params& p, long lon
 }
 
 template <bool kBf16>
-__device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u, const uint4& v, uint32_t mask) {
-  constexpr uint32_t kSign = 0x80008000u;
+__device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u, const uint4& v, bool store) {
+  constexpr uint32_t kSign = 0x80008000u, mask = 0xffffffffu;
   const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
   const uint32_t hi2 = max2<kBf16>(max2<kBf16>(v.x, v.y), max2<kBf16>(v.z, v.w));
   const uint32_t lo2 = min2<kBf16>(min2<kBf16>(v.x, v.y), min2<kBf16>(v.z, v.w)) ^ kSign;
@@ -111,23 +111,33 @@ __device__ __forceinline__ void quantize_unit(const Quant4Params& p, long long u
     }
   }
   w -= 0xfb000000u;  // what the exponent bits 0x4b000000 of the eight sums added up to
-  p.codes[(u & ~15ll) + 4 * (u & 3) + ((u >> 2) & 3)] = fine ? w : 0x88888888u;
-  if ((u & 3) == 0) p.scales[u >> 2] = s;
+  if (store) {
+    p.codes[(u & ~15ll) + 4 * (u & 3) + ((u >> 2) & 3)] = fine ? w : 0x88888888u;
+    if ((u & 3) == 0) p.scales[u >> 2] = s;
+  }
 }
 
 template <bool kBf16, bool kContiguous>
 __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
-  // units is a multiple of 16, so the lanes of a group leave the loop together
+  // A warp's lanes stay together to its last unit: those past the end (the upper half of a warp at most, units
+  // being a multiple of 16) exchange zeros and store nothing.  (Masks per group of four lanes: 84 us against 57.)
   constexpr int kStep = 256;  // a block takes runs of 512 units (rounds spread over the grid: 65 us against 61)
-  const long long first = (long long)blockIdx.x * (2 * kStep) + threadIdx.x;
-  for (long long u = first; u < p.units; u += (long long)gridDim.x * (2 * kStep)) {
-    const uint32_t mask = __activemask();
-    const bool two = u + kStep < p.units;
-    const uint4 v0 = __ldg(unit_ptr<kContiguous>(p, u));
-    uint4 v1 = make_uint4(0u, 0u, 0u, 0u);
+  const int lane = threadIdx.x & 31;
+  const long long first = (long long)blockIdx.x * (2 * kStep) + (threadIdx.x - lane);
+  for (long long w = first; w < p.units; w += (long long)gridDim.x * (2 * kStep)) {
+    const long long u = w + lane;
+    if (w + kStep + 32 <= p.units) {
+      const uint4 v0 = __ldg(unit_ptr<kContiguous>(p, u)), v1 = __ldg(unit_ptr<kContiguous>(p, u + kStep));
+      quantize_unit<kBf16>(p, u, v0, true);
+      quantize_unit<kBf16>(p, u + kStep, v1, true);
+      continue;
+    }
+    const bool one = u < p.units, two = u + kStep < p.units;
+    uint4 v0 = make_uint4(0u, 0u, 0u, 0u), v1 = v0;
+    if (one) v0 = __ldg(unit_ptr<kContiguous>(p, u));
     if (two) v1 = __ldg(unit_ptr<kContiguous>(p, u + kStep));
-    quantize_unit<kBf16>(p, u, v0, mask);
-    if (two) quantize_unit<kBf16>(p, u + kStep, v1, __activemask());
+    quantize_unit<kBf16>(p, u, v0, one);
+    if (w + kStep < p.units) quantize_unit<kBf16>(p, u + kStep, v1, two);
   }
 }
 

@@ -102,3 +102,11 @@ def test_first_calls_of_long_and_short_rows_in_four_threads():
     """A fresh process whose first matvec4 calls, of K = 128 and 8192 in every kernel, meet in four threads."""
     r = subprocess.run([sys.executable, "-c", CHILD, PKG_ROOT], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.split() == ["done", "0"], r.stdout + r.stderr[-2000:]
+
+
+def test_lanes_exchange_under_masks_that_are_known():
+    """A group's lanes exchange under the group's mask: __activemask() names whichever lanes happen to be
+    together, which nothing promises to be whole groups after a branch."""
+    for name in os.listdir(CSRC):
+        with open(os.path.join(CSRC, name)) as f:
+            assert "__activemask" not in f.read(), name
