@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
       for (int r = 0; r < kOuts; ++r) {
         y[nb][r] = 0.f;
         if (p.add && s == 0 && row + out_row(r) < p.N && out_m(nb, r) < p.M)
-          y[nb][r] = __ldg(p.add + add_at[nb] + (r & 1) * p.am + out_row(r));
+          y[nb][r] = p.add[add_at[nb] + (r & 1) * p.am + out_row(r)];  // may be out: a plain load
       }
     float acc[kNB][4];
 #pragma unroll

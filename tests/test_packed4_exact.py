@@ -354,3 +354,42 @@ def test_matvec_silu_of_large_negative_values(dtype):
         assert (np.abs(y - want) <= tol + near).all()
     x = torch.full((1, 128), -math.inf, dtype=dtype)
     assert anima_attn.matvec4(x.cuda(), w, silu=True).isnan().all()
+
+
+# ------------------------------------------------------------------ matvec4 in place
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,N,K", [(1, 77, 128), (1, 33, 4096), (5, 96, 256), (3, 1003, 1024)])
+@pytest.mark.parametrize("M", [1, 2, 9, 17])
+@pytest.mark.parametrize("xdt", [F32, F16, BF16])
+def test_matvec_adds_in_place(E, N, K, M, xdt):
+    """out = add, the same tensor, over several passes of rows, several warps a tile and views: bit for bit what
+    comes out beside it."""
+    g = torch.Generator().manual_seed(71)
+    w, _ = random_packed((E, N, K), 72, std=0.05)
+    x = torch.randn(E, M, K, generator=g).to(xdt).cuda()
+    add = torch.randn(E, M, N, generator=g).cuda()
+    want = anima_attn.matvec4(x, w, add=add)
+    inplace = add.clone()
+    assert anima_attn.matvec4(x, w, add=inplace, out=inplace) is inplace and torch.equal(inplace, want)
+    buf = torch.full((E, M + 1, N + 3), 7.0, device="cuda")
+    view = buf[:, :M, 1:N + 1]
+    view.copy_(add)
+    anima_attn.matvec4(x, w, add=view, out=view)
+    assert torch.equal(view, want)
+    view.fill_(7.0)
+    assert (buf == 7).all()
+    if E == 1:  # accumulating into a gradient-like buffer, call after call
+        a, b = torch.zeros(M, N, device="cuda"), torch.zeros(M, N, device="cuda")
+        one = Packed4(w.codes[0], w.scales[0])
+        for _ in range(3):
+            anima_attn.matvec4(x[0], one, add=a, out=a)
+            b = anima_attn.matvec4(x[0], one, add=b)
+        assert torch.equal(a, b)
+
+
+def test_the_addend_is_not_read_through_the_read_only_path():
+    """out may be add: __ldg is only defined for memory that nothing writes while the kernel runs."""
+    import os
+    from conftest import PKG_ROOT
+    with open(os.path.join(PKG_ROOT, "csrc", "packed4.cu")) as f:
+        assert "__ldg(p.add" not in f.read()
