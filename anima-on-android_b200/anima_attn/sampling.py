@@ -54,7 +54,7 @@ class EulerCFGSampler:
         self.x = torch.zeros(latent_shape, device=dev, dtype=torch.float32)
         self.sig = torch.zeros(1, device=dev, dtype=torch.float32)
         self.sig_next = torch.zeros(1, device=dev, dtype=torch.float32)
-        self.cache = model.context_cache(self.cc, self.cu, kv_bits) if cache_context else None
+        self.cache = self._context() if cache_context else None
         self.graph = self.ctx_graph = None
         if graph:
             if not self.x.is_cuda:
@@ -76,8 +76,13 @@ class EulerCFGSampler:
                 with torch.cuda.graph(self.ctx_graph):
                     self._fill_cache()
 
+    def _context(self):
+        if self.kv_bits == 16:
+            return self.model.context_cache(self.cc, self.cu)
+        return self.model.context_cache(self.cc, self.cu, kv_bits=self.kv_bits)
+
     def _fill_cache(self):
-        fresh = self.model.context_cache(self.cc, self.cu, self.kv_bits)
+        fresh = self._context()
         for key, entry in fresh.items():
             for name, t in entry.items():
                 self.cache[key][name].copy_(t)
