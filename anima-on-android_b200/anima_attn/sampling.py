@@ -121,7 +121,10 @@ def run_ksampler(model, ctx_cond: torch.Tensor, ctx_uncond: torch.Tensor, H: int
                  shift: float = 3.0, graph: bool = True,
                  sampler: Optional[EulerCFGSampler] = None, kv_bits: int = 16) -> torch.Tensor:
     """run_ksampler (sampling.py:183-209) with the z_image schedule and the Euler sampler:
-    seeded noise, the sigma schedule, then the loop.  Returns [1, 16, H, W] fp32."""
+    seeded noise, the sigma schedule, then the loop.  Returns [1, 16, H, W] fp32.  ``kv_bits`` is for the
+    sampler built here; a given ``sampler`` has its own."""
+    if sampler is not None and kv_bits not in (16, sampler.kv_bits):
+        raise ValueError("the given sampler was built with other kv_bits")
     dev = ctx_cond.device
     noise = torch.from_numpy(seeded_noise(seed, H, W)).to(dev)
     s = sampler or EulerCFGSampler(model, ctx_cond, ctx_uncond, cfg, noise.shape, graph=graph,
