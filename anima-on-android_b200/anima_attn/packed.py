@@ -80,6 +80,13 @@ def _kv4_workspace(dev: int, dtype: torch.dtype, B: int, H: int, Sq: int, Skv: i
     return int(L.lib.anima_attn_kv4_workspace_size(_TORCH_DT[dtype], B, H, Sq, Skv))
 
 
+def _lengths32(t: torch.Tensor, most: int) -> torch.Tensor:
+    """Lengths of another type as int32: what int32 does not hold is cut to [0, most] first."""
+    if t.is_floating_point():
+        t = t.double()
+    return t.clamp(0, most).to(torch.int32) if t.element_size() == 8 else t.to(torch.int32)
+
+
 def _repeats(t: torch.Tensor) -> bool:
     """Whether an axis of a tensor to be written repeats the same memory (an expanded view)."""
     return 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride()))
@@ -229,14 +236,14 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
 
     q [B*H, S_q, 128] contiguous float16 or bfloat16, k/v packed [B*H, S_kv, 128].  Returns
     (or fills) ``out`` in ``out_dtype`` (q's type, or float32) and ``out_layout`` "bshd" [B, S_q, H,
-    128] or "bhsd" [B, H, S_q, 128].  ``kv_valid_len`` int32 [B]: keys at or past it do not count, whatever the
-    cache holds there; a sample without any has zero rows.
+    128] or "bhsd" [B, H, S_q, 128].  ``kv_valid_len`` [B], int32 best: keys at or past it do not count,
+    whatever the cache holds there; a sample without any has zero rows.
 
     ``out`` overlaps no operand.  K and V enter exactly, probabilities to 2^-16; sums are fp32 and the
     result is rounded once (anima_attn_kv4_fwd)."""
     kc, ks = k
     vc, vs = v
-    stream = _here(q, kc, ks, vc, vs, kv_valid_len, out)
+    stream = _here(q, kc, ks, vc, vs, out)
     qs, qdt = tuple(q.shape), q.dtype
     if len(qs) != 3 or qdt not in _HALF or not q.is_contiguous():
         raise ValueError("q must be [B*H, S_q, 128], contiguous, float16 or bfloat16")
@@ -272,7 +279,9 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
         raise ValueError("scale must be positive")
     vp = 0
     if kv_valid_len is not None:
-        vl = kv_valid_len if kv_valid_len.dtype is torch.int32 else kv_valid_len.to(torch.int32)
+        vl = kv_valid_len if kv_valid_len.dtype is torch.int32 else _lengths32(kv_valid_len, Skv)
+        if vl.device != q.device:
+            vl = vl.to(q.device)
         vl = vl.contiguous()
         if vl.numel() != B:
             raise ValueError("kv_valid_len must have B entries")

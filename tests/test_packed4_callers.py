@@ -43,3 +43,29 @@ def test_ksampler_does_not_ignore_kv_bits():
     with pytest.raises(ValueError):
         run_ksampler(m, cc, cu, 16, 16, steps=1, sampler=s, kv_bits=4)
     assert np.isfinite(run_ksampler(m, cc, cu, 16, 16, steps=1, sampler=s).numpy()).all()
+
+
+def test_lengths_of_other_types():
+    """Lengths as int32: what that type does not hold means all keys, or none."""
+    from anima_attn.packed import _lengths32
+    big = torch.tensor([-(1 << 40), -1, 0, 5, 77, 78, 1 << 31, 1 << 40, (1 << 63) - 1])
+    assert _lengths32(big, 77).tolist() == [0, 0, 0, 5, 77, 77, 77, 77, 77]
+    assert _lengths32(torch.tensor([-3.0, 5.5, 60000.0, float("inf")], dtype=torch.float16), 77).tolist() == [0, 5, 77, 77]
+    assert _lengths32(torch.tensor([0, 200], dtype=torch.uint8), 77).tolist() == [0, 200]
+    assert _lengths32(torch.tensor([True, False]), 77).tolist() == [1, 0]
+    assert _lengths32(big, 77).dtype == torch.int32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 9, 2200])
+def test_lengths_of_other_types_and_devices(Sq):
+    """int64 lengths past 2^31 (a mark for "all"), lengths on the host, float lengths: the int32 call's results."""
+    import anima_attn
+    from test_packed4 import random_packed
+    B, H, S = 3, 2, 150
+    q = torch.randn(B * H, Sq, 128, generator=torch.Generator().manual_seed(5)).half().cuda()
+    k, v = random_packed((B * H, S, 128), 1)[0], random_packed((B * H, S, 128), 2)[0]
+    want = anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=torch.tensor([S, 0, 70], dtype=torch.int32, device="cuda"))
+    for lens in (torch.tensor([1 << 40, -(1 << 40), 70], device="cuda"), torch.tensor([S, 0, 70]), torch.tensor([S, 0, 70], dtype=torch.int32),
+                 torch.tensor([float("inf"), 0, 70.5], device="cuda"), torch.tensor([[S, 0, 70]] * 2, dtype=torch.int32, device="cuda").t()[:, 0]):
+        assert torch.equal(anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=lens), want)
