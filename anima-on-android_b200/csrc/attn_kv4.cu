@@ -4,8 +4,8 @@
 // Two ways, chosen by rows_path below:
 //   little work: kv4_rows_kernel reads the packed cache directly, eight query rows at a time;
 //   more:        attn_kv4_tile.cu, on the tensor cores, unpacks K and V in the kernel.
-// Neither writes the cache out in 16 bits: scratch holds partial results of slices only, at most 64
-// times 130 floats a query row.
+// Neither writes the cache out in 16 bits: scratch holds partial results only, of slices at most 64
+// times 130 floats a query row, and of long chains 128 KB a CTA.
 //
 // kv4_rows_kernel.  One cluster per (batch, head, block of query rows); its CTAs and their
 // warps take 32-key blocks in turn, each warp with its own running maximum, sum and output, so

@@ -20,7 +20,10 @@ struct Kv4TilePlan {
   int nqb;          // units per (batch, head)
   long long units;
   int nsplit;       // slices of a unit's keys
-  size_t bytes;     // workspace for the slices' partials
+  int runs;         // runs of a slice's keys, one after another
+  int grid;         // CTAs
+  size_t part_bytes;  // workspace for the slices' partials,
+  size_t bytes;       // and with a CTA's sums over runs behind them
 };
 Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count);
 // Joins partials [slice][unit][kv4_part_floats(rows)] into a->out.

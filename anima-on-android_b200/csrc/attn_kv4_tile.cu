@@ -3,7 +3,8 @@
 // CTA itself.  out = softmax(q K^T * scale) V per (batch, head), D = 128.
 //
 // Work unit = kNT 128-row query tiles of one (batch, head); its keys may be cut into slices, and
-// (unit, slice) is a segment, streamed in 64-key tiles.  The grid is persistent: a CTA takes
+// (unit, slice) is a segment, streamed in 64-key tiles (one of more than kRun tiles in several runs, whose sums a CTA
+// joins in scratch of its own).  The grid is persistent: a CTA takes
 // segments c, c + G, ..., and moves from one to the next without draining (the next Q tile, K and V
 // are under way while the last P V and the output of the segment before run).  A unit cut into
 // slices writes fp32 partials (O, running max, running sum), which kv4_merge_kernel joins in slice
@@ -53,6 +54,10 @@ namespace kv4t {
 using namespace attn;  // kD, kBM, drain_wait, stage/store_block, pack2
 
 constexpr int kKeys = 64;                   // keys per tile
+// Tiles of one chain of sums in tensor memory.  The tensor core cuts a sum off to fp32 after each of its 12 products a
+// tile instead of rounding it, so what a chain loses grows with its length: 2e-5 of sum p |v| at 128 tiles, 1.4e-4 at
+// 1024, 1.6e-3 at 4096.  Longer ones go on as runs, joined in rounded fp32 sums.
+constexpr int kRun = 128;
 constexpr int kPanel = 128 * 128;           // [128 rows][64 x 16-bit]
 constexpr int kTile = 2 * kPanel;            // a Q tile
 constexpr int kKvPanel = kKeys * 128;
@@ -71,12 +76,14 @@ struct Params {
   const int* valid;
   void* out;
   float* part;         // partials, or nullptr: write the output
+  float* fold;         // a CTA's O of the runs so far, [rows][128]
   long long ob, oh, os;
   int* status;
   int H, S_q, S_kv;
   int nqb;             // units per (batch, head)
   int units;
   int nsplit;
+  int runs;            // runs of a segment
   int out_f32;         // out is fp32, else of q's type
   float scale_log2;
 };
@@ -113,12 +120,24 @@ constexpr size_t smem_bytes() {
 }
 static_assert(smem_bytes<1>() <= 227 * 1024 && smem_bytes<2>() <= 227 * 1024, "shared memory budget");
 
-// A segment: key tiles [k0, k0 + n) of a unit.
+// A run of a segment: key tiles [k0, k0 + n) of a unit.  Runs are numbered through, those of a segment in a row, and
+// a CTA takes all of a segment.
 struct Seg {
   int unit, slice, bh, b, q0, len, k0, n;
+  bool last;  // of its segment
 };
-__device__ __forceinline__ Seg segment(const Params& p, int seg, int rows) {
+template <bool kLong>
+__device__ __forceinline__ int after(const Params& p, int run) {
+  if (!kLong) return run + (int)gridDim.x;
+  ++run;
+  return run % p.runs ? run : run + ((int)gridDim.x - 1) * p.runs;
+}
+template <bool kLong>
+__device__ __forceinline__ Seg segment(const Params& p, int run, int rows) {
   Seg s;
+  const int seg = kLong ? run / p.runs : run;
+  run -= kLong ? seg * p.runs : seg;
+  s.last = !kLong || run + 1 == p.runs;
   s.slice = seg / p.units;
   s.unit = seg - s.slice * p.units;
   s.bh = s.unit / p.nqb;
@@ -128,6 +147,10 @@ __device__ __forceinline__ Seg segment(const Params& p, int seg, int rows) {
   const int tiles = (s.len + kKeys - 1) / kKeys;
   s.k0 = (int)((long long)tiles * s.slice / p.nsplit);
   s.n = (int)((long long)tiles * (s.slice + 1) / p.nsplit) - s.k0;
+  if (kLong) {
+    s.n = min(max(s.n - run * kRun, 0), kRun);
+    s.k0 += run * kRun;
+  }
   return s;
 }
 
@@ -216,7 +239,8 @@ __device__ __forceinline__ float convert_row(uint8_t* tile, int row) {
   return __int_as_float((127 - s0) << 23) * __int_as_float((127 - s1) << 23);
 }
 
-template <bool kBf16, int kNT>
+// kLong: segments of more than one run.
+template <bool kBf16, int kNT, bool kLong>
 __global__ void __launch_bounds__(kThreads16, 1)
     kv4_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -259,7 +283,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  const int segs = p.units * p.nsplit;
+  const int segs = p.units * p.nsplit * (kLong ? p.runs : 1);
+  const int first = (int)blockIdx.x * (kLong ? p.runs : 1);
   // Launched as a programmatic dependent of the kernel before it on the stream: the set-up above
   // overlaps that kernel's end, and no global memory is touched before it has completed.
   grid_dependency_wait();
@@ -275,8 +300,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
       tma_prefetch_desc(&tmap_q);
       int a = 0;
       bool ok = true;
-      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
-        const Seg s = segment(p, seg, kRows);
+      for (int seg = first; seg < segs && ok; seg = after<kLong>(p, seg)) {
+        const Seg s = segment<kLong>(p, seg, kRows);
         if (s.n <= 0) continue;
         for (int i = 0; i < kNT && ok; ++i) {
           if (a > 0 && !(ok = wait(&sm.q_empty[i], (uint32_t)(a - 1) & 1u))) break;
@@ -300,8 +325,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
       // quarter-warp of the unpacking reads lie in different banks.
       bool ok = true;
       int raw = 0, use = 0;
-      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
-        const Seg s = segment(p, seg, kRows);
+      for (int seg = first; seg < segs && ok; seg = after<kLong>(p, seg)) {
+        const Seg s = segment<kLong>(p, seg, kRows);
         const long long row0 = (long long)s.bh * p.S_kv + (long long)s.k0 * kKeys;
         for (int m = 0; m < 2 * s.n; ++m) {
           const Item it = item_of(m, s.n);
@@ -388,8 +413,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
         tc_fence_after();
       };
       int a = 0, gg = 0;
-      for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
-        const int n = segment(p, seg, kRows).n;
+      for (int seg = first; seg < segs && ok; seg = after<kLong>(p, seg)) {
+        const int n = segment<kLong>(p, seg, kRows).n;
         if (n <= 0) continue;
         // QK^T runs a step ahead of P V.  S of step t is in buffer t % 2, which P V of step t - 2 has to have left:
         // with two query tiles it is the same thread's and earlier in the pipe.
@@ -441,8 +466,8 @@ __global__ void __launch_bounds__(kThreads16, 1)
     for (int g = 0; g < 2; ++g) put[g] = r0 * 128 + (((4 * g + i) ^ (jr & 7)) << 4);
     bool ok = true;
     int raw = 0, use = 0, gg = 0;
-    for (int seg = blockIdx.x, n; seg < segs && ok; seg += gridDim.x, gg += n) {
-    n = segment(p, seg, kRows).n;
+    for (int seg = first, n; seg < segs && ok; seg = after<kLong>(p, seg), gg += n) {
+    n = segment<kLong>(p, seg, kRows).n;
 #pragma unroll 1
     for (int m = 0; m < 2 * n; ++m) {
       const Item it = item_of(m, n);
@@ -521,14 +546,17 @@ __global__ void __launch_bounds__(kThreads16, 1)
       return in_range(p.scale_log2 * back);
     };
     auto more = [&](int seg) {  // whether a segment with keys follows
-      for (seg += gridDim.x; seg < segs; seg += gridDim.x)
-        if (segment(p, seg, kRows).n > 0) return true;
+      for (seg = after<kLong>(p, seg); seg < segs; seg = after<kLong>(p, seg))
+        if (segment<kLong>(p, seg, kRows).n > 0) return true;
       return false;
     };
     float sl2 = 0.f;
     bool have_q = false;
-    for (int seg = blockIdx.x; seg < segs && ok; seg += gridDim.x) {
-    const Seg s = segment(p, seg, kRows);
+    // Of the segment's runs before this one, with O in p.fold: whether there are any, maximum, sum, and the scale of m.
+    bool folded = false;
+    float m_sum = 0.f, l_sum = 0.f, sl2_sum = 0.f;
+    for (int seg = first; seg < segs && ok; seg = after<kLong>(p, seg)) {
+    const Seg s = segment<kLong>(p, seg, kRows);
     const int n = s.n, grow = s.q0 + i * kBM + row;
     if (n > 0 && !have_q) {
       sl2 = take_q(a);
@@ -653,7 +681,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       m = m_use;
     }
     if (!ok) break;
-    const float sl2_of_m = sl2;  // the next segment's may be fetched before m is written
+    float sl2_of_m = sl2;  // the next segment's may be fetched before m is written
     if (n > 0) {
       // The next segment's Q tile, if any, has been loading since this one's last QK^T.
       have_q = kBf16 && more(seg);
@@ -663,6 +691,22 @@ __global__ void __launch_bounds__(kThreads16, 1)
       tc_fence_after();
     }
     {
+      float f_old = 1.f, f_new = 1.f;  // factors of the O's
+      if (kLong && folded) {
+        if (n > 0) {
+          const float M = fmaxf(m_sum, m);
+          f_old = m_sum == -INFINITY ? 0.f : ex2_approx((m_sum - M) * sl2_of_m);
+          f_new = m == -INFINITY ? 0.f : ex2_approx((m - M) * sl2_of_m);
+          m = M;
+          l = fmaf(l_sum, f_old, l * f_new);
+        } else {
+          m = m_sum;
+          l = l_sum;
+          sl2_of_m = sl2_sum;
+        }
+      }
+      const bool some = n > 0 || (kLong && folded);
+      float* const fold = p.fold + ((long long)blockIdx.x * kRows + i * kBM + row) * kD;  // kLong
       float4* const stage = sm.stage[warp];
       const int r0 = grow - lane;  // the warp's first row
       const int nvalid = p.S_q - r0;
@@ -672,7 +716,7 @@ __global__ void __launch_bounds__(kThreads16, 1)
       float* const part = direct ? nullptr : p.part + ((long long)s.slice * p.units + s.unit) * kv4_part_floats(kRows);
       const long long out_at = (long long)s.b * p.ob + (long long)(s.bh % p.H) * p.oh + (long long)r0 * p.os;
 #pragma unroll 1
-      for (int c = 0; c < 4 && (direct || n > 0); ++c) {
+      for (int c = 0; c < 4 && (s.last ? direct || some : n > 0); ++c) {
         float v[32];
         if (n > 0) {
           uint32_t o[32];
@@ -684,7 +728,21 @@ __global__ void __launch_bounds__(kThreads16, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0.f;
         }
-        if (direct && !p.out_f32) {
+        if (kLong && folded) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 x = *reinterpret_cast<const float4*>(fold + c * 32 + 4 * e);
+            v[4 * e] = fmaf(x.x, f_old, v[4 * e] * f_new);
+            v[4 * e + 1] = fmaf(x.y, f_old, v[4 * e + 1] * f_new);
+            v[4 * e + 2] = fmaf(x.z, f_old, v[4 * e + 2] * f_new);
+            v[4 * e + 3] = fmaf(x.w, f_old, v[4 * e + 3] * f_new);
+          }
+        }
+        if (kLong && !s.last) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(fold + c * 32 + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        } else if (direct && !p.out_f32) {
           store_block<kBf16 ? ANIMA_DTYPE_BF16 : ANIMA_DTYPE_F16>(static_cast<char*>(p.out) + out_at * 2, p.os * 2,
                                                                    nvalid, v, c, inv, stage, lane);
         } else if (!direct || lane < nvalid) {  // fp32: a partial, or the output
@@ -695,9 +753,15 @@ __global__ void __launch_bounds__(kThreads16, 1)
                 make_float4(v[4 * e] * inv, v[4 * e + 1] * inv, v[4 * e + 2] * inv, v[4 * e + 3] * inv);
         }
       }
-      if (!direct) {
+      if (s.last && !direct) {
         part[kRows * kD + urow + lane] = m == -INFINITY ? m : m * sl2_of_m;
         part[kRows * kD + kRows + urow + lane] = l;
+      }
+      if (kLong) {
+        folded = !s.last && some;
+        m_sum = m;
+        l_sum = l;
+        sl2_sum = sl2_of_m;
       }
     }
     if (n > 0) {
@@ -813,13 +877,16 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
       t.nsplit = k;
     }
   }
-  t.bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4_part_floats(t.nt * attn::kBM)) * 4 : 0;
+  t.runs = (int)(((tiles + t.nsplit - 1) / t.nsplit + kv4t::kRun - 1) / kv4t::kRun);
+  t.grid = (int)std::min<long long>(t.units * t.nsplit, sm_count);
+  t.part_bytes = t.nsplit > 1 ? (size_t)(t.nsplit * t.units * kv4_part_floats(t.nt * attn::kBM)) * 4 : 0;
+  t.bytes = t.part_bytes + (t.runs > 1 ? (size_t)t.grid * (t.nt * attn::kBM) * attn::kD * 4 : 0);
   return t;
 }
 
-template <bool kBf16, int kNT>
+template <bool kBf16, int kNT, bool kLong>
 static int tile_t(const CUtensorMap& mq, const kv4t::Params& p, int grid, cudaStream_t st) {
-  auto kern = kv4t::kv4_tile_kernel<kBf16, kNT>;
+  auto kern = kv4t::kv4_tile_kernel<kBf16, kNT, kLong>;
   constexpr size_t smem = kv4t::smem_bytes<kNT>();
   static SmemAttr attr;
   if (!attr.raise((const void*)kern, smem)) return ANIMA_ERR_CUDA;
@@ -840,7 +907,7 @@ int kv4_merge_launch(const AnimaAttnKv4Args* a, const float* part, int nqb, int 
 
 int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status, int sm_count, cudaStream_t st) {
   const bool bf = a->dtype == ANIMA_DTYPE_BF16;
-  if (t.units * t.nsplit > 0x7fffffffLL) return ANIMA_ERR_SHAPE;
+  if (t.units * t.nsplit * t.runs > 1 << 30) return ANIMA_ERR_SHAPE;  // with one round of the grid below 2^31
   kv4t::Params p;
   p.kc = static_cast<const uint8_t*>(a->k_codes);
   p.ks = static_cast<const uint8_t*>(a->k_scales);
@@ -849,6 +916,7 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   p.valid = (a->flags & ANIMA_FLAG_MASK) ? a->kv_valid_len : nullptr;
   p.out = a->out;
   p.part = t.nsplit > 1 ? static_cast<float*>(a->workspace) : nullptr;
+  p.fold = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + t.part_bytes);
   p.ob = a->out_stride[0];
   p.oh = a->out_stride[1];
   p.os = a->out_stride[2];
@@ -859,14 +927,19 @@ int kv4_tile_launch(const AnimaAttnKv4Args* a, const Kv4TilePlan& t, int* status
   p.nqb = t.nqb;
   p.units = (int)t.units;
   p.nsplit = t.nsplit;
+  p.runs = t.runs;
   p.out_f32 = (a->flags & ANIMA_FLAG_OUT_F32) != 0;
   p.scale_log2 = std::min(a->scale * 1.4426950408889634f, 3.402823466e38f);
   CUtensorMap mq;
   int rc = attn_head_map(&mq, a->q, a->dtype, a->B * a->H, a->S_q);
   if (rc != ANIMA_OK) return rc;
-  const int grid = (int)std::min<long long>(t.units * t.nsplit, sm_count);
-  rc = t.nt == 1 ? (bf ? tile_t<true, 1>(mq, p, grid, st) : tile_t<false, 1>(mq, p, grid, st))
-                 : (bf ? tile_t<true, 2>(mq, p, grid, st) : tile_t<false, 2>(mq, p, grid, st));
+  auto go = [&](auto nt, auto is_long) {
+    constexpr int kNT = decltype(nt)::value;
+    constexpr bool kLong = decltype(is_long)::value;
+    return bf ? tile_t<true, kNT, kLong>(mq, p, t.grid, st) : tile_t<false, kNT, kLong>(mq, p, t.grid, st);
+  };
+  auto of = [&](auto nt) { return t.runs > 1 ? go(nt, std::true_type()) : go(nt, std::false_type()); };
+  rc = t.nt == 1 ? of(std::integral_constant<int, 1>()) : of(std::integral_constant<int, 2>());
   if (rc != ANIMA_OK || t.nsplit == 1) return rc;
   return kv4_merge_launch(a, p.part, t.nqb, t.nt * attn::kBM, p.units, t.nsplit, sm_count, st);
 }

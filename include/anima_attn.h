@@ -364,8 +364,8 @@ int anima_matvec4(const AnimaMatvec4Args* args, void* stream);
  * values are to be in fp16's range, as anima_quantize4 leaves them) and the probabilities to 2^-16, sum in
  * fp32, and round the result once.  The cache is never written out unpacked.
  * `workspace`: anima_attn_kv4_workspace_size bytes for partial results (0 for some calls; at most 64 x 130
- * floats a query row, rows rounded up to 256), 256-byte aligned, contents irrelevant; calls that share
- * one must be ordered.  Asynchronous on `stream`.
+ * floats a query row, rows rounded up to 256, and from 8192 keys 128 KB a multiprocessor), 256-byte aligned,
+ * contents irrelevant; calls that share one must be ordered.  Asynchronous on `stream`.
  */
 typedef struct AnimaAttnKv4Args {
   const void* q;

@@ -53,11 +53,12 @@ WAYS = [("direct", 1, 1), ("direct", 2, 9), ("tile1", 40, 128), ("tile1", 70, 65
 @pytest.mark.parametrize("dtype", [L.DTYPE_F16, L.DTYPE_BF16])
 @pytest.mark.parametrize("B,H,Sq,Skv", [(2, 16, 4096, 512), (2, 16, 16384, 512), (2, 16, 4096, 65536), (1, 1, 1 << 17, 1 << 20)])
 def test_a_packed_cache_is_not_written_out(dtype, B, H, Sq, Skv):
-    """Scratch is for slices' partial results: none where the query tiles alone fill the device, and never
-    near the 256 bytes a key and side of a cache in 16 bits."""
-    assert L.lib.anima_attn_kv4_workspace_size(dtype, B, H, Sq, Skv) == 0
+    """Scratch is for partial results: none for slices where the query tiles alone fill the device, 128 KB a
+    multiprocessor for chains of more than 8192 keys, and never the 256 bytes a key and side of a cache in 16 bits."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert L.lib.anima_attn_kv4_workspace_size(dtype, B, H, Sq, Skv) <= (sms * 256 * 512 if Skv > 8192 else 0)
     for sq in (1, 8, 64, 200):
-        assert L.lib.anima_attn_kv4_workspace_size(dtype, 1, 1, sq, 1 << 20) <= 64 * (sq + 255) * 130 * 4
+        assert L.lib.anima_attn_kv4_workspace_size(dtype, 1, 1, sq, 1 << 20) <= 64 * (sq + 255) * 130 * 4 + sms * 256 * 512
 
 
 # ------------------------------------------------------------------ attention: K, V and P keep their bits
@@ -393,3 +394,56 @@ def test_the_addend_is_not_read_through_the_read_only_path():
     from conftest import PKG_ROOT
     with open(os.path.join(PKG_ROOT, "csrc", "packed4.cu")) as f:
         assert "__ldg(p.add" not in f.read()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("BH,Sq,N", [(2, 1, 200000), (75, 3, 200000), (75, 17, 200000), (38, 129, 200000), (1, 100, 1000000)])
+@pytest.mark.parametrize("values", ["one", "two"])
+def test_sums_over_a_long_cache(BH, Sq, N, values):
+    """Values all alike: the result is that value whatever the weights are.  Chains of sums are of at most 8192
+    keys (or of a warp's share of a cache): 128 tiles of 12 products, each cut off by a step of fp32 at most, of
+    a sum that grows evenly, so half of that, 9.2e-5; weights and parts 2^-16, joining chains 64 half steps."""
+    rng = np.random.default_rng(81)
+    one, _ = packed(rng.integers(-8, 8, (1, 1000, 128)), np.full((1, 1000, 4), 0.1))
+    k = Packed4(*(t.repeat(1, (N + 999) // 1000, 1)[:, :N].expand(BH, -1, -1).contiguous() for t in one))
+    codes = torch.from_numpy(codes_of(np.full((1, 1, 128), 7))).cuda()
+    v = Packed4(codes.expand(BH, N, -1).contiguous(), torch.full((BH, N, 4), 1 + 2.0 ** -10, dtype=F16, device="cuda"))
+    if values == "two":  # the first half of the keys' values are twice the others', and so are the weights' halves
+        v.scales[:, :N // 2] *= 2
+        k.scales[:] = 0
+    q = torch.randn(BH, Sq, 128, generator=torch.Generator().manual_seed(82)).to(F16).cuda()
+    got = anima_attn.attention_core_kv4(q, k, v, 1, BH, out_dtype=F32).double()
+    want = 7 * (1 + 2.0 ** -10) * (1.5 if values == "two" else 1.0)
+    assert ((got - want).abs().max() / want).item() <= 9.2e-5 + 2.0 ** -16 + 64 * 2.0 ** -24
+    assert anima_attn.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,H,Sq,Skv,lens", [(1, 80, 40, 20000, None), (2, 40, 20, 20000, [20000, 8192]), (2, 40, 20, 20000, [8193, 64]),
+                                             (2, 40, 130, 20000, [100, 20000]), (2, 40, 20, 20000, [16385, 0])])
+def test_runs_of_a_long_cache(B, H, Sq, Skv, lens, dtype):
+    """Chains of more than 8192 keys go on as runs: whole, cut by lengths at, before and behind a run's end, with
+    maxima that rise and fall from run to run (keys twice as large in the middle)."""
+    size = np.ones(Skv)
+    size[7000:9000], size[18000:] = 2.0, 0.1
+    rng = np.random.default_rng(83)
+    k, kv = packed(rng.integers(-8, 8, (1, Skv, 128)), 0.2 * size[None, :, None] * rng.uniform(0.9, 1.1, (1, Skv, 4)))
+    v, vv = random_packed((1, Skv, 128), 84)
+    BH = B * H
+    q = torch.randn(BH, Sq, 128, generator=torch.Generator().manual_seed(85)).to(dtype).cuda()
+    vl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = anima_attn.attention_core_kv4(q, every_head(k, BH), every_head(v, BH), B, H, kv_valid_len=vl, out_dtype=F32)
+    kd, vd = torch.from_numpy(kv[0]).cuda(), torch.from_numpy(vv[0]).cuda()
+    for b in range(B):
+        n = Skv if lens is None else lens[b]
+        for h in range(0, H, 13):
+            if n == 0:
+                assert (got[b, :, h] == 0).all()
+                continue
+            s = q[b * H + h].double() @ kd[:n].T / math.sqrt(128)
+            p = torch.softmax(s, -1)
+            top = (q[b * H + h].double().abs() @ kd[:n].abs().T / math.sqrt(128)).amax(-1, keepdim=True)
+            tol = (p @ vd[:n].abs()) * (2 * (512 * 2.0 ** -23 * top + 2.0 ** -16) + 9.2e-5)
+            assert ((got[b, :, h].double() - p @ vd[:n]).abs() <= tol).all()
+    assert anima_attn.status() == 0
