@@ -69,3 +69,13 @@ def test_lengths_of_other_types_and_devices(Sq):
     for lens in (torch.tensor([1 << 40, -(1 << 40), 70], device="cuda"), torch.tensor([S, 0, 70]), torch.tensor([S, 0, 70], dtype=torch.int32),
                  torch.tensor([float("inf"), 0, 70.5], device="cuda"), torch.tensor([[S, 0, 70]] * 2, dtype=torch.int32, device="cuda").t()[:, 0]):
         assert torch.equal(anima_attn.attention_core_kv4(q, k, v, B, H, kv_valid_len=lens), want)
+
+
+@pytest.mark.parametrize("scale", [1e39, 1e-46, 0.0, -1.0, float("inf"), float("nan")])
+def test_scales_that_float32_does_not_hold(scale, monkeypatch):
+    import anima_attn
+    from anima_attn import packed as P
+    monkeypatch.setattr(P, "_here", lambda *ts: 0)
+    k = anima_attn.Packed4(torch.zeros(4, 5, 64, dtype=torch.uint8), torch.zeros(4, 5, 4, dtype=torch.float16))
+    with pytest.raises(ValueError):
+        anima_attn.attention_core_kv4(torch.zeros(4, 3, 128, dtype=torch.float16), k, k, 2, 2, scale=scale)
