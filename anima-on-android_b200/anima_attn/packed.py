@@ -275,7 +275,7 @@ def attention_core_kv4(q: torch.Tensor, k: Packed4, v: Packed4, B: int, H: int,
             raise ValueError("out must have q's type (or out_dtype's), the layout's shape, a contiguous head dimension and no repeated axis")
     oh, os = (s2, s1) if out_layout == "bshd" else (s1, s2)
     scale = _SCALE if scale is None else float(scale)
-    if not 2.0 ** -149 <= scale <= 3.4028234663852886e38:
+    if not 2.0 ** -150 < scale <= 3.4028234663852886e38:
         raise ValueError("scale must be positive and a float32")
     vp = 0
     if kv_valid_len is not None:

@@ -447,3 +447,23 @@ def test_runs_of_a_long_cache(B, H, Sq, Skv, lens, dtype):
             tol = (p @ vd[:n].abs()) * (2 * (512 * 2.0 ** -23 * top + 2.0 ** -16) + 9.2e-5)
             assert ((got[b, :, h].double() - p @ vd[:n]).abs() <= tol).all()
     assert anima_attn.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[1000000, 70], [0, 600001], [8192 * 64 + 1, 1]])
+def test_slices_of_several_runs_masked(lens):
+    """Slices so long that each is several runs, lengths that leave runs and slices empty: values all alike."""
+    B, Sq, N = 2, 70, 1000000
+    one, _ = packed(np.random.default_rng(86).integers(-8, 8, (1, 1000, 128)), np.full((1, 1000, 4), 0.1))
+    k = Packed4(*(t.repeat(1, N // 1000, 1).expand(B, -1, -1).contiguous() for t in one))
+    codes = torch.from_numpy(codes_of(np.full((1, 1, 128), 7))).cuda()
+    v = Packed4(codes.expand(B, N, -1).contiguous(), torch.ones(B, N, 4, dtype=F16, device="cuda"))
+    for b, n in enumerate(lens):
+        k.scales[b, n:] = v.scales[b, n:] = float("nan")
+    q = torch.randn(B, Sq, 128, generator=torch.Generator().manual_seed(87)).to(F16).cuda()
+    vl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = anima_attn.attention_core_kv4(q, k, v, B, 1, kv_valid_len=vl, out_dtype=F32).double()
+    assert way(B, Sq, N) == "tile1"
+    for b, n in enumerate(lens):  # bound as in test_sums_over_a_long_cache
+        assert ((got[b] - (7 if n else 0)).abs().max() / 7).item() <= 9.2e-5 + 2.0 ** -16 + 64 * 2.0 ** -24
+    assert anima_attn.status() == 0
