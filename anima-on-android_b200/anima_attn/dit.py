@@ -212,7 +212,9 @@ class AnimaDiT:
     ``close()`` releases the peer mappings (every rank, before the process group goes).
     ``adaln_bits``: 16, or 4 to hold the blocks' adaLN-LoRA modulation weights packed (CUDA;
     4.5 bits a value: 352 MB of the full model become 99 MB).  They are read whole once per
-    step by one row per sample, so their products (matvec4) are bound by that read.
+    step by one row per sample, so their products (matvec4) are bound by that read.  The weights
+    are then 4-bit ones, off by 0.085 of a value: the latent is outside the parity bar of 1e-2 (0.08 for
+    random weights of two blocks, 0.11 of 28).
     """
 
     def __init__(self, cfg: DiTConfig, weights: Dict[str, torch.Tensor], rank: int = 0,
@@ -679,7 +681,9 @@ class AnimaDiT:
         cond], the order euler_cfg_step uses).  The text context is the same in every step of
         a sampling run (anima_rt/scripts/sampling.py:127), while the reference projects and
         normalises its K/V in every step and block (numpy_dit.py:276-286); with the cache a
-        step runs only the query side of each cross-attention."""
+        step runs only the query side of each cross-attention.  ``kv_bits`` 4 holds K and V packed:
+        66 MB instead of 235 for a prompt pair of the full model, values off by 0.085, and a latent
+        outside the parity bar (0.03 for random weights)."""
         from .ops import attention as _lib_attention
         ctx = torch.cat([ctx_uncond, ctx_cond], dim=0).float()
         keep = ctx.is_cuda and self.attn_fn is _lib_attention

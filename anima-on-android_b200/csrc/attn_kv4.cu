@@ -26,10 +26,10 @@
 // few and the cache long, several clusters share a unit's keys and write fp32 partials, which
 // kv4_merge_kernel joins.  No atomics; the order of all sums is fixed.
 //
-// One row against 65536 keys, 32 heads: 59 us, 5.1 TB/s of the cache (46 us at the copy rate); 65536
-// blocks of 32 keys take 525 instructions each, 0.57 a cycle and scheduler, nearly half of them on the
+// One row against 65536 keys, 32 heads: 60 us replayed from a graph, 5.0 TB/s of the cache (46 us at the copy
+// rate), 67 a call whose inputs change; 65536 blocks of 32 keys take 544 instructions each, nearly half of them on the
 // integer pipe, which takes one every other cycle.  One SM's two CTAs are no faster with more warps.  One
-// row against 512 keys takes 4.7 us, seven rows against 1237 9.4.
+// row against 512 keys takes 5.3 us, seven rows against 1237 9.6 (calls from Python 10.7 and 11.3).
 #include <algorithm>
 #include <atomic>
 

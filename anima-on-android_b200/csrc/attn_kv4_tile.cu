@@ -40,7 +40,7 @@
 //
 // What bounds it: a step of two query tiles and 64 keys takes 3,010 cycles (traced) of 3,072 that its MMAs
 // need, and the unpacking fills as much; the clock falls under that load (1.4 GHz).  256 rows against 8192
-// keys, 32 heads: 82 us; 64 rows 52 us, 2,500 cycles a step of 1,536 of MMAs, the rest unpacking and
+// keys, 32 heads: 82 us replayed from a graph; 64 rows 55 us, 2,500 cycles a step of 1,536 of MMAs, the rest unpacking and
 // hand-offs.
 #include <algorithm>
 

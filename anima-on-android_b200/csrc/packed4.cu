@@ -20,7 +20,7 @@ namespace anima {
 // e_s the exponent of s), while products with an approximate 1 / s are off by less than 2^-19.  So
 // with t = saturate(x / (16 s) + 17/32 + 2^-18), the sum t (16 - 2^-14) + 2^23 - 1/2 rounds to
 // 2^23 + n + 8: at a border the bias leaves between 2^-18 and 2^-14 above it, and t = 1 gives 15.
-// 132 M bf16 values take 61 us (5.6 TB/s; 52 at the copy rate), bound by the integer pipe.  With tests
+// 132 M bf16 values take 59 us (5.7 TB/s; 52 at the copy rate), bound by the integer pipe.  With tests
 // of every value, clamps on both sides and a true reciprocal they took 106 (at 71 otherwise).
 struct Quant4Params {
   const void* x;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(256)
 // lowest parts in bf16's.  (As whole numbers of 2^-30 of a group's largest value, in four base-256 digits for the
 // whole-number MMA, 84 x 6144 x 256 took a fifth less, and values far below the group's largest lost their bits.)
 //
-// 84 matrices of 6144 x 256 with two fp32 rows take 23.4 us (3.3 TB/s of codes, scales and results; 12 at
+// Replayed from a graph, 84 matrices of 6144 x 256 with two fp32 rows take 23.4 us (3.3 TB/s of codes, scales and results; 12 at
 // the copy rate), bound by instruction issue, the unpacking to bf16 first, and some 3 us of start, when x
 // is staged.  One 6144 x 2048 matrix and row takes 5.7 us, one 21504 x 2048 with SiLU and two rows 12.6.
 //
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kMvThreads, 3) matvec4_kernel(const Mv4Params 
 
 // ---------------------------------------------------------------- launchers
 // Blocks of a streaming kernel that takes one round each.  132 M values (bf16) unpack in 56 us so, 59 with
-// 32 blocks an SM and 65 with 8; packing is capped at 64 blocks an SM: 61 us, 68 without, 71 with 8.
+// 32 blocks an SM and 65 with 8; packing is capped at 64 blocks an SM (by an earlier form: 61 us, 68 without, 71 with 8).
 static int stream_grid(long long work, int per_block) {
   return (int)std::min<long long>((work + per_block - 1) / per_block, 1 << 30);
 }

@@ -79,3 +79,26 @@ def test_scales_that_float32_does_not_hold(scale, monkeypatch):
     k = anima_attn.Packed4(torch.zeros(4, 5, 64, dtype=torch.uint8), torch.zeros(4, 5, 4, dtype=torch.float16))
     with pytest.raises(ValueError):
         anima_attn.attention_core_kv4(torch.zeros(4, 3, 128, dtype=torch.float16), k, k, 2, 2, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("adaln_bits,kv_bits", [(4, 16), (16, 4), (4, 4)])
+def test_what_four_bits_do_to_the_latent(adaln_bits, kv_bits):
+    """The packed options against the golden latents of the 16-bit model.  They are outside the parity bar of
+    1e-2: 4-bit storage is a choice of memory over exactness.  Bound: the largest of 32 normal values is
+    2.4 deviations, the step an eighth of that, its rounding 0.085 of a value (step / sqrt 12); two layers of
+    weights, or K and V, 0.12 of a modulation or of a cross-attention's result; twice that for what the later blocks
+    and the guidance make of it."""
+    import anima_attn
+    from anima_attn.dit import AnimaDiT, DiTConfig, make_weights
+    from anima_attn.sampling import EulerCFGSampler
+    from conftest import golden, rel_l2
+    from test_sampling import BLOCKS
+    g = golden("sampler_small.npz")
+    cfg = DiTConfig(blocks=BLOCKS)
+    m = AnimaDiT(cfg, make_weights(cfg, seed=1234, device="cuda"), adaln_bits=adaln_bits)
+    cc, cu = (t.cuda() for t in _contexts())
+    s = EulerCFGSampler(m, cc, cu, float(g["cfg"]), (1, 16, 32, 32), graph=False, kv_bits=kv_bits)
+    r = rel_l2(s.sample(torch.from_numpy(g["noise"]).cuda(), g["sigmas"]).cpu().numpy(), g["latent"])
+    print(f"adaln_bits {adaln_bits}, kv_bits {kv_bits}: latent against the golden one {r:.2e}")
+    assert r <= 0.25 and anima_attn.status() == 0
