@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(32 * kW) kv4_rows_kernel(const Params p) {
 // Whether the packed cache is read directly.  Up to 16 rows always; beyond, the rows' passes over the
 // cache (and, below 256 keys, their starts) cost more than the tile kernel's start (some 8 us) once
 // heads x rows x keys exceed 2^20, twice that from 4096 keys and four times that from 32768, where the
-// tile kernel has slices to join.  Measured, us, this way against the tile kernel, heads x rows x keys:
+// tile kernel has slices to join.  Measured, us, from graphs, this way against the tile kernel, heads x rows x keys:
 // 4 x 1024 x 130 12.2 / 12.1, 32 x 128 x 130 12.2 / 9.2, 4 x 512 x 512 12.2 / 16.7, 32 x 64 x 512 12.2 / 13.6,
 // 4 x 1024 x 512 18.8 / 17.7, 32 x 64 x 2048 28.0 / 21.0, 1 x 512 x 4096 16.2 / 23.6, 16 x 32 x 4096
 // 16.2 / 21.1, 4 x 256 x 4096 26.2 / 24.0, 4 x 32 x 16384 18.6 / 27.7, 4 x 64 x 16384 26.1 / 28.3, 1 x 64 x
@@ -564,7 +564,7 @@ static RowsPlan rows_plan(long long bh, int S_q, int S_kv, int sm_count) {
   } else {
     // CTAs per cluster and clusters per unit (slices of its keys, four blocks a warp at least): the
     // shortest chain of blocks, in rounds of the clusters that the device holds, where a round's ends cost
-    // 1.5 blocks of some 2 us and joining s slices 1.5 + s / 8.  In us, one cluster of eight against slices of one CTA, one
+    // 1.5 blocks of some 2 us and joining s slices 1.5 + s / 8.  In us from graphs, one cluster of eight against slices of one CTA, one
     // row, heads x keys: 20 x 65536 60.7 / 43.7, 32 x 65536 60.0 / 58.5, 32 x 16384 20.8 / 23.8, 37 x 16384
     // 31.1 / 25.3; two clusters of eight against those: 16 x 65536 37.4 / 38.0.
     r.ncta = 1;

@@ -864,7 +864,7 @@ Kv4TilePlan kv4_tile_plan(int bh, int S_q, int S_kv, int sm_count) {
   const long long tiles = (S_kv + kv4t::kKeys - 1) / kv4t::kKeys;
   // Slices: at most as many as the SMs hold in one round; the number with the least of the longest
   // chain of key tiles, some 1.65 us each, plus, if more than one, the merge: 2.7 tiles, and per slice 0.11
-  // and 0.012 for every 256 rows.  In us, by slices: 32 units, 8 tiles: 22.2 whole, 23.1 in 2, 21.0 in 4; 16
+  // and 0.012 for every 256 rows.  In us from graphs, by slices: 32 units, 8 tiles: 22.2 whole, 23.1 in 2, 21.0 in 4; 16
   // units, 32 tiles: 63 whole, 30 in 4, 23.5 in 8; 8 units, 64 tiles: 30.0 in 8, 24.8 in 16; one unit,
   // 256 tiles: 69 in 8, 45 in 16, 34.6 in 32, 33.3 in 64.
   const long long most = std::min({sm_count / std::max(1LL, t.units), tiles, 64LL});
